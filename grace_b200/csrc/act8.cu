@@ -1,0 +1,355 @@
+// 8-bit activation checkpoints: writing them, reading them back, and the activation functions of a feed-forward layer
+// that write them in the forward pass and read them in the backward pass.
+//
+//   pack      codes, scales = checkpoint(x)                               es + 1 1/32 bytes an element
+//   unpack    x~ = value of the checkpoint                                1 1/32 + es
+//   forward   y = f(x), checkpoint(x), optionally checkpoint(y)           2 es + 1 1/32 (+ 1 1/32)
+//             gated: x = [a | b], y = f(a) b, checkpoints of a and b      3 es + 2 1/16 (+ 1 1/32), for an element of y
+//   backward  dx = dy f'(x~);  gated: da = dy b~ f'(a~), db = dy f(a~)    2 es + 1 1/32;  3 es + 2 1/16
+//
+// All four are bound by memory: a thread takes chunks of eight neighbouring elements (16 bytes of a 16-bit type in, 8
+// bytes of codes out), four lanes share a group of 32 and agree on its largest magnitude by two shuffles; a thread
+// issues the loads of all its chunks before it computes.  The issue slots are the second limit: at 6.5 TB/s an SM has
+// about 16 of them an element of a bf16 pack and 25 of a forward pass, so the encoder takes one FMA, one clamp and
+// 7/8 of a byte shuffle an element, and the functions take one exponential and one reciprocal.
+//
+// f is GELU (erf form), GELU (tanh form) or SiLU.  For 16-bit tensors the error function is the rational approximation
+// 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error below 1.5e-7, 2^-22.6: far
+// below half a step of a 16-bit result, 2^-9 or 2^-12 of its value wherever the value is not itself below 2^-10),
+// whose exp(-z^2) is also the density that the derivative needs; the exponential is the hardware's.  For fp32
+// tensors erfc and exp are CUDA's.
+#include "act8.cuh"
+#include "act8.h"
+#include "gradio.cuh"
+
+namespace grace {
+namespace {
+
+constexpr int kBlock = 256;
+
+// n / d for 0 <= n < 2^31 as a multiplication: m = ceil(2^p / d) with p = 31 + ceil(log2 d) (Granlund and Montgomery)
+struct FastDiv {
+  unsigned d, m;
+  int p;
+};
+FastDiv make_div(unsigned d) {
+  int l = 0;
+  while ((1ull << l) < d) ++l;
+  const unsigned long long p = 31 + l;
+  return {d, (unsigned)(((1ull << p) + d - 1) / d), (int)p};
+}
+__device__ __forceinline__ void divmod(const FastDiv& f, unsigned n, unsigned& q, unsigned& r) {
+  q = (unsigned)(((unsigned long long)n * f.m) >> f.p);
+  r = n - q * f.d;
+}
+
+struct Rows {          // which chunks a launch covers
+  unsigned chunks;     // rows * (pitch / 8), below 2^31; a multiple of 4
+  FastDiv per_row;     // pitch / 8
+  int cols;
+};
+
+__device__ __forceinline__ void put_held(const Held& h, size_t row, int col, uint2 codes, unsigned s) {
+  *reinterpret_cast<uint2*>(h.codes + row * h.pitch + col) = codes;
+  if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
+}
+__device__ __forceinline__ void get_held(const Held& h, size_t row, int col, float (&v)[8]) {
+  const uint2 codes = __ldg(reinterpret_cast<const uint2*>(h.codes + row * h.pitch + col));
+  act8_decode(codes, (unsigned)__ldg(h.scales + row * h.spitch + (col >> 5)), v);
+}
+
+// ---- the functions: f and f' at x ----
+template <int KIND, bool FAST>
+__device__ __forceinline__ float2 function(float x) {
+  constexpr float kInvSqrt2Pi = 0.3989422804f;
+  if (KIND == kActGelu) {
+    float p, e;   // p: the normal distribution function, e: exp(-x^2 / 2)
+    if (FAST) {
+      const float z = fabsf(x) * 0.70710678f;
+      const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+      e = __expf(-z * z);
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
+      p = x < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);   // q = erfc(z)
+    } else {
+      e = expf(-0.5f * x * x);
+      p = 0.5f * erfcf(-0.70710678f * x);
+    }
+    return make_float2(x * p, fmaf(x * kInvSqrt2Pi, e, p));
+  }
+  if (KIND == kActGeluTanh) {
+    constexpr float c = 0.7978845608f, a = 0.044715f;
+    const float xx = fminf(x * x, 1e4f);   // past |x| = 100 the sigmoid is 0 or 1 to the last bit
+    const float u = 2.f * c * x * fmaf(a, xx, 1.f);
+    const float p = FAST ? __fdividef(1.f, 1.f + __expf(-u)) : 1.f / (1.f + expf(-u));   // (1 + tanh(u / 2)) / 2
+    return make_float2(x * p, fmaf(2.f * c * x * p * (1.f - p), fmaf(3.f * a, xx, 1.f), p));
+  }
+  const float p = FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+  return make_float2(x * p, p * fmaf(x, 1.f - p, 1.f));
+}
+
+// ---- kernels: thread t of a block takes the chunks base + t, base + t + 256, ... (U of them) ----
+template <class T, int U>
+__global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, long long stride, bool vec, Rows r, Held held) {
+  const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
+  Chunk8<T> c[U];
+  unsigned row[U], k[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const unsigned at = base + i * kBlock;
+    row[i] = k[i] = 0;
+    c[i].zero();
+    if (at < r.chunks) {
+      divmod(r.per_row, at, row[i], k[i]);
+      load_chunk(c[i], x + (long long)row[i] * stride, (int)k[i] * 8, r.cols, vec);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    float v[8];
+    unsigned s;
+    c[i].get(v);
+    const uint2 codes = act8_encode(v, s);
+    if (base + i * kBlock < r.chunks) put_held(held, row[i], (int)k[i] * 8, codes, s);
+  }
+}
+
+template <class T, int U>
+__global__ void __launch_bounds__(kBlock) unpack_kernel(Held held, T* __restrict__ out, long long stride, bool vec, Rows r) {
+  const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const unsigned at = base + i * kBlock;
+    if (at >= r.chunks) return;
+    unsigned row, k;
+    divmod(r.per_row, at, row, k);
+    float v[8];
+    get_held(held, row, (int)k * 8, v);
+    store_chunk(v, out + (long long)row * stride, (int)k * 8, r.cols, vec);
+  }
+}
+
+template <class T, int KIND, bool GATED, int U>
+__global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x, long long stride, bool vec_x, T* __restrict__ y,
+                                                        bool vec_y, Rows r, Held held, Held held_b, Held held_y) {
+  constexpr bool kFast = sizeof(T) == 2;
+  const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
+  Chunk8<T> ca[U], cb[GATED ? U : 1];
+  unsigned row[U], k[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const unsigned at = base + i * kBlock;
+    row[i] = k[i] = 0;
+    ca[i].zero();
+    if (GATED) cb[GATED ? i : 0].zero();
+    if (at < r.chunks) {
+      divmod(r.per_row, at, row[i], k[i]);
+      const T* p = x + (long long)row[i] * stride;
+      load_chunk(ca[i], p, (int)k[i] * 8, r.cols, vec_x);
+      if (GATED) load_chunk(cb[GATED ? i : 0], p + r.cols, (int)k[i] * 8, r.cols, vec_x);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const bool in = base + i * kBlock < r.chunks;
+    const int col = (int)k[i] * 8;
+    float v[8], w[8];
+    unsigned s;
+    uint2 codes;
+    ca[i].get(v);
+    if (held.codes) {
+      codes = act8_encode(v, s);
+      if (in) put_held(held, row[i], col, codes, s);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = function<KIND, kFast>(v[j]).x;
+    if (GATED) {
+      cb[GATED ? i : 0].get(w);
+      if (held_b.codes) {
+        codes = act8_encode(w, s);
+        if (in) put_held(held_b, row[i], col, codes, s);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= w[j];
+    }
+    if (in) store_chunk(v, y + (size_t)row[i] * r.cols, col, r.cols, vec_y);
+    if (held_y.codes) {
+      Chunk8<T> cy;   // the checkpoint is of y as the next layer sees it
+      cy.set(v);
+      cy.get(v);
+      codes = act8_encode(v, s);
+      if (in) put_held(held_y, row[i], col, codes, s);
+    }
+  }
+}
+
+template <class T, int KIND, bool GATED, int U>
+__global__ void __launch_bounds__(kBlock) backward_kernel(const T* __restrict__ grad, long long stride, bool vec_g, T* __restrict__ dx,
+                                                         bool vec_x, Rows r, Held held, Held held_b) {
+  constexpr bool kFast = sizeof(T) == 2;
+  const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
+  Chunk8<T> c[U];
+  uint2 qa[U], qb[GATED ? U : 1];
+  unsigned sa[U], sb[GATED ? U : 1], row[U], k[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const unsigned at = base + i * kBlock;
+    if (at < r.chunks) {
+      divmod(r.per_row, at, row[i], k[i]);
+      const int col = (int)k[i] * 8;
+      load_chunk(c[i], grad + (long long)row[i] * stride, col, r.cols, vec_g);
+      qa[i] = __ldg(reinterpret_cast<const uint2*>(held.codes + (size_t)row[i] * held.pitch + col));
+      sa[i] = __ldg(held.scales + (size_t)row[i] * held.spitch + (col >> 5));
+      if (GATED) {
+        qb[GATED ? i : 0] = __ldg(reinterpret_cast<const uint2*>(held_b.codes + (size_t)row[i] * held_b.pitch + col));
+        sb[GATED ? i : 0] = __ldg(held_b.scales + (size_t)row[i] * held_b.spitch + (col >> 5));
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (base + i * kBlock >= r.chunks) return;
+    const int col = (int)k[i] * 8;
+    float g[8], a[8], b[8];
+    c[i].get(g);
+    act8_decode(qa[i], sa[i], a);
+    T* const out = dx + (size_t)row[i] * (GATED ? 2 : 1) * r.cols;
+    if (GATED) {
+      act8_decode(qb[GATED ? i : 0], sb[GATED ? i : 0], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 f = function<KIND, kFast>(a[j]);
+        a[j] = g[j] * b[j] * f.y;
+        b[j] = g[j] * f.x;
+      }
+      store_chunk(b, out + r.cols, col, r.cols, vec_x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = g[j] * function<KIND, kFast>(a[j]).y;
+    }
+    store_chunk(a, out, col, r.cols, vec_x);
+  }
+}
+
+bool aligned(const void* p, long long stride_elems, int es) {
+  return (reinterpret_cast<uintptr_t>(p) % 16 == 0) && (stride_elems * es) % 16 == 0;
+}
+
+Held rows_from(Held h, long long row) {
+  if (h.codes) {
+    h.codes += (size_t)row * h.pitch;
+    h.scales += (size_t)row * h.spitch;
+  }
+  return h;
+}
+
+// Calls f(first row, Rows, grid for `per_thread` chunks a thread) for slabs of rows whose chunk count fits 31 bits.
+template <class F>
+cudaError_t over_slabs(long long rows, int cols, int per_thread, F f) {
+  const long long per_row = ((long long)cols + 31) / 32 * 4;
+  const long long slab = ((1ll << 31) - 1) / per_row;
+  for (long long at = 0; at < rows; at += slab) {
+    const long long n = rows - at < slab ? rows - at : slab;
+    Rows r{(unsigned)(n * per_row), make_div((unsigned)per_row), cols};
+    const long long per_block = (long long)kBlock * per_thread;
+    f(at, r, (unsigned)((n * per_row + per_block - 1) / per_block));
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+  }
+  return cudaSuccess;
+}
+
+constexpr int kUnroll = 2;
+
+template <class T>
+cudaError_t pack_typed(const void* x, long long stride, long long rows, int cols, Held held, cudaStream_t st) {
+  const T* p = static_cast<const T*>(x);
+  const bool vec = aligned(x, stride, sizeof(T));
+  return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
+    pack_kernel<T, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec, r, rows_from(held, at));
+  });
+}
+template <class T>
+cudaError_t unpack_typed(Held held, void* out, long long stride, long long rows, int cols, cudaStream_t st) {
+  T* p = static_cast<T*>(out);
+  const bool vec = aligned(out, stride, sizeof(T));
+  return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
+    unpack_kernel<T, kUnroll><<<grid, kBlock, 0, st>>>(rows_from(held, at), p + at * stride, stride, vec, r);
+  });
+}
+template <class T, int KIND, bool GATED>
+cudaError_t forward_typed(const void* x, long long stride, void* y, long long rows, int cols, Held a, Held b, Held hy, cudaStream_t st) {
+  const T* p = static_cast<const T*>(x);
+  T* q = static_cast<T*>(y);
+  const bool vec_x = aligned(x, stride, sizeof(T)) && (!GATED || aligned(x, cols, sizeof(T))), vec_y = aligned(y, cols, sizeof(T));
+  return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
+    forward_kernel<T, KIND, GATED, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec_x, q + at * cols, vec_y, r,
+                                                                     rows_from(a, at), rows_from(b, at), rows_from(hy, at));
+  });
+}
+template <class T, int KIND, bool GATED>
+cudaError_t backward_typed(const void* grad, long long stride, void* dx, long long rows, int cols, Held a, Held b, cudaStream_t st) {
+  const T* p = static_cast<const T*>(grad);
+  T* q = static_cast<T*>(dx);
+  const bool vec_g = aligned(grad, stride, sizeof(T)), vec_x = aligned(dx, cols, sizeof(T));
+  return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
+    backward_kernel<T, KIND, GATED, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec_g, q + at * cols * (GATED ? 2 : 1),
+                                                                      vec_x, r, rows_from(a, at), rows_from(b, at));
+  });
+}
+
+template <class F>
+cudaError_t by_type(int dtype, F f) {
+  switch (dtype) {
+    case kGradF32: return f(float{});
+    case kGradBF16: return f(__nv_bfloat16{});
+    case kGradF16: return f(__half{});
+  }
+  return cudaErrorInvalidValue;
+}
+template <int V> struct Int { static constexpr int value = V; };
+template <class F>
+cudaError_t by_kind(int kind, int gated, F f) {
+  switch (kind * 2 + (gated ? 1 : 0)) {
+    case 0: return f(Int<kActGelu>{}, Int<0>{});
+    case 1: return f(Int<kActGelu>{}, Int<1>{});
+    case 2: return f(Int<kActGeluTanh>{}, Int<0>{});
+    case 3: return f(Int<kActGeluTanh>{}, Int<1>{});
+    case 4: return f(Int<kActSilu>{}, Int<0>{});
+    case 5: return f(Int<kActSilu>{}, Int<1>{});
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_act8_pack(const void* x, long long x_stride, long long rows, int cols, int dtype, Held held, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  return by_type(dtype, [&](auto t) { return pack_typed<decltype(t)>(x, x_stride, rows, cols, held, stream); });
+}
+
+cudaError_t launch_act8_unpack(Held held, void* out, long long out_stride, long long rows, int cols, int dtype, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  return by_type(dtype, [&](auto t) { return unpack_typed<decltype(t)>(held, out, out_stride, rows, cols, stream); });
+}
+
+cudaError_t launch_act8_forward(const void* x, long long x_stride, void* y, long long rows, int cols, int dtype, int kind, int gated,
+                                Held held, Held held_b, Held held_y, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  return by_type(dtype, [&](auto t) {
+    return by_kind(kind, gated, [&](auto k, auto g) {
+      return forward_typed<decltype(t), decltype(k)::value, decltype(g)::value != 0>(x, x_stride, y, rows, cols, held, held_b, held_y, stream);
+    });
+  });
+}
+
+cudaError_t launch_act8_backward(const void* grad, long long grad_stride, void* dx, long long rows, int cols, int dtype, int kind,
+                                 int gated, Held held, Held held_b, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  return by_type(dtype, [&](auto t) {
+    return by_kind(kind, gated, [&](auto k, auto g) {
+      return backward_typed<decltype(t), decltype(k)::value, decltype(g)::value != 0>(grad, grad_stride, dx, rows, cols, held, held_b, stream);
+    });
+  });
+}
+
+}  // namespace grace

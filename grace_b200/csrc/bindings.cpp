@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "act8.h"
 #include "exchange.h"
 #include "host_exchange.h"
 #include "runtime.h"
@@ -35,6 +36,10 @@ PeerTable make_peers(int rank, int world, unsigned long long seq, unsigned long 
   for (int i = 0; i < world; ++i) t.heap[i] = reinterpret_cast<char*>(heaps[i]);
   t.ready_off = ready_off; t.ack_off = ack_off; t.slot_off = slot_off; t.slot_bytes = slot_bytes;
   return t;
+}
+
+Held held(uintptr_t codes, uintptr_t scales, int pitch, int spitch) {
+  return {ptr<signed char>(codes), ptr<unsigned char>(scales), pitch, spitch};
 }
 
 }  // namespace
@@ -275,6 +280,49 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
                            weight_decay, nesterov, first_step, zero_grad, grad_scale,
                            reinterpret_cast<cudaStream_t>(stream)),
           "multi_sgd");
+  });
+
+  // ---- 8-bit activation checkpoints ----
+  m.def("act8_pack", [](uintptr_t x, long long x_stride, long long rows, int cols, int dtype, uintptr_t codes, uintptr_t scales,
+                        int pitch, int spitch, uintptr_t stream) {
+    check(launch_act8_pack(ptr<const void>(x), x_stride, rows, cols, dtype, held(codes, scales, pitch, spitch),
+                           reinterpret_cast<cudaStream_t>(stream)), "act8_pack");
+  });
+  m.def("act8_unpack", [](uintptr_t codes, uintptr_t scales, int pitch, int spitch, uintptr_t out, long long out_stride,
+                          long long rows, int cols, int dtype, uintptr_t stream) {
+    check(launch_act8_unpack(held(codes, scales, pitch, spitch), ptr<void>(out), out_stride, rows, cols, dtype,
+                             reinterpret_cast<cudaStream_t>(stream)), "act8_unpack");
+  });
+  m.def("act8_forward", [](uintptr_t x, long long x_stride, uintptr_t y, long long rows, int cols, int dtype, int kind, int gated,
+                           uintptr_t codes, uintptr_t scales, uintptr_t codes_b, uintptr_t scales_b, uintptr_t codes_y,
+                           uintptr_t scales_y, int pitch, int spitch, uintptr_t stream) {
+    check(launch_act8_forward(ptr<const void>(x), x_stride, ptr<void>(y), rows, cols, dtype, kind, gated,
+                              held(codes, scales, pitch, spitch), held(codes_b, scales_b, pitch, spitch),
+                              held(codes_y, scales_y, pitch, spitch), reinterpret_cast<cudaStream_t>(stream)), "act8_forward");
+  });
+  m.def("act8_backward", [](uintptr_t grad, long long grad_stride, uintptr_t dx, long long rows, int cols, int dtype, int kind,
+                            int gated, uintptr_t codes, uintptr_t scales, uintptr_t codes_b, uintptr_t scales_b, int pitch,
+                            int spitch, uintptr_t stream) {
+    if (gated && !codes_b) throw std::invalid_argument("act8_backward: a gated function needs two checkpoints");
+    check(launch_act8_backward(ptr<const void>(grad), grad_stride, ptr<void>(dx), rows, cols, dtype, kind, gated,
+                               held(codes, scales, pitch, spitch), held(codes_b, scales_b, pitch, spitch),
+                               reinterpret_cast<cudaStream_t>(stream)), "act8_backward");
+  });
+  m.def("act8_repitch", [](uintptr_t src, long long stride, uintptr_t dst, long long rows, int cols, uintptr_t stream) {
+    check(launch_act8_repitch(ptr<const void>(src), stride, ptr<void>(dst), rows, cols, reinterpret_cast<cudaStream_t>(stream)),
+          "act8_repitch");
+  });
+  m.def("act8_wgrad", [](uintptr_t grad, long long grad_stride, uintptr_t codes, uintptr_t scales, int pitch, int spitch,
+                         long long tokens, int outs, int ins, int dtype, int out_f32, uintptr_t out, uintptr_t bias, int sms,
+                         uintptr_t stream) {
+    check(launch_act8_wgrad(ptr<const void>(grad), grad_stride, held(codes, scales, pitch, spitch), tokens, outs, ins, dtype,
+                            out_f32, ptr<void>(out), ptr<void>(bias), sms, reinterpret_cast<cudaStream_t>(stream)), "act8_wgrad");
+  });
+  m.def("act8_wgrad_status", []() {
+    std::vector<unsigned> words(16);
+    py::gil_scoped_release release;
+    check(act8_wgrad_status(words.data()), "act8_wgrad_status");
+    return words;
   });
 
   // ---- host engine of the exchange protocol (CPU ranks over POSIX shared memory) ----

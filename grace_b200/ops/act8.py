@@ -1,0 +1,399 @@
+"""8-bit activation checkpoints: what the forward pass keeps for the backward pass, at a byte an element.
+
+The exchange kernels shrink what ranks send to each other; these shrink what a rank keeps to itself between forward
+and backward, which is what bounds its batch.  A checkpoint holds groups of 32 neighbours of the last axis as int8
+codes with one power-of-two scale (the MXINT8 format of the OCP Microscaling specification, see ``csrc/act8.cuh``): 33
+bytes for 32 values.  The forward pass computes with the full-precision tensors; only the backward pass sees the
+rounded ones, so outputs are untouched and gradients carry an error of at most half a code step (2^-7 of the leading
+power of two of a value's group) in the values they are made of.
+
+* ``pack(x)`` / ``unpack(held)``: write a checkpoint, read it back.
+* ``weight_grad(grad, held)``: the weight (and bias) gradient of a linear layer straight from the checkpoint of its
+  input; the tensor cores' operand tiles are decoded on chip (``csrc/act8_wgrad.cu``).
+* ``activation_forward`` / ``activation_backward``: GELU (erf or tanh form) and SiLU, plain or gated, with the checkpoint of their
+  input (and, for the layer after them, of their output) written in the same pass.
+* ``linear`` and ``activation``: the same with autograd.
+
+CUDA tensors run the kernels, CPU tensors the same arithmetic in torch ops.  Every call allocates what it returns and
+what it needs from torch's allocator on the current stream of the tensor's device, and keeps nothing between calls.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn.functional as F
+
+from . import native
+from .exchange import GRAD_DTYPE, GraceCommError
+
+GROUP = 32
+KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
+MAX_COLS = 1 << 30     # columns of a row: the kernels index within a row in 32 bits
+MAX_TOKENS = (1 << 31) - 64
+
+
+def pitch_of(cols: int) -> Tuple[int, int]:
+    """Bytes of a row of codes (whole groups) and of a row of scales (whole eights of groups)."""
+    groups = -(-cols // GROUP)
+    return groups * GROUP, -(-groups // 8) * 8
+
+
+class Act8:
+    """A checkpoint of a tensor of ``shape`` and ``dtype``: ``codes`` int8 ``[rows, pitch]`` and ``scales`` uint8
+    ``[rows, spitch]`` (``pitch_of``), rows being the product of all axes but the last."""
+
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype):
+        shape = tuple(shape)
+        if not shape:
+            raise ValueError("Act8: a checkpoint has at least one axis")
+        if dtype not in GRAD_DTYPE:
+            raise TypeError("Act8: fp32, bf16 or fp16, not %s" % dtype)
+        pitch, spitch = pitch_of(shape[-1])
+        rows = math.prod(shape[:-1])
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise TypeError("Act8: int8 codes and uint8 scales")
+        if codes.shape != (rows, pitch) or scales.shape != (rows, spitch):
+            raise ValueError("Act8: a checkpoint of %s has codes %s and scales %s, not %s and %s"
+                             % (shape, (rows, pitch), (rows, spitch), tuple(codes.shape), tuple(scales.shape)))
+        if codes.device != scales.device:
+            raise ValueError("Act8: codes and scales are on different devices")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
+            raise ValueError("Act8: codes and scales are contiguous, and start on 16- and 8-byte boundaries")
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return "Act8(shape=%s, dtype=%s, device=%s, nbytes=%d)" % (self.shape, self.dtype, self.device, self.nbytes)
+
+
+def empty_like(shape, dtype: torch.dtype, device) -> Act8:
+    """An Act8 for a tensor of ``shape`` whose contents are yet to be written."""
+    shape = tuple(shape)
+    rows, (pitch, spitch) = math.prod(shape[:-1]), pitch_of(shape[-1])
+    held = Act8.__new__(Act8)     # (its arrays are made to measure: nothing to check)
+    held.codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+    held.scales = torch.empty((rows, spitch), dtype=torch.uint8, device=device)
+    held.shape, held.dtype = shape, dtype
+    return held
+
+
+# ---------------------------------------------------------------------------------------------------- shared checks
+def _on(device: torch.device):
+    """The device to launch on, made current for the launch if it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check_tensor(x, what: str) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("%s: a tensor, not %s" % (what, type(x).__name__))
+    if x.dtype not in GRAD_DTYPE:
+        raise TypeError("%s: fp32, bf16 or fp16, not %s" % (what, x.dtype))
+    if x.layout != torch.strided:
+        raise TypeError("%s: a dense tensor, not %s" % (what, x.layout))
+    if x.dim() == 0:
+        raise ValueError("%s: at least one axis" % what)
+    if x.shape[-1] > MAX_COLS:
+        raise ValueError("%s: at most 2^30 columns" % what)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as ``[rows, cols]`` with neighbouring columns; a copy only where its strides leave no other way."""
+    cols = x.shape[-1]
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(math.prod(x.shape[:-1]), cols)
+    if cols > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x
+
+
+def _ptrs(held: Optional[Act8]) -> Tuple[int, int]:
+    return (held.codes.data_ptr(), held.scales.data_ptr()) if held is not None else (0, 0)
+
+
+# -------------------------------------------------------------------------------------------- the arithmetic on CPU
+def _encode_cpu(x: torch.Tensor, held: Act8) -> None:
+    rows, pitch = held.codes.shape
+    groups = pitch // GROUP
+    v = F.pad(_rows(x).float(), (0, pitch - x.shape[-1])).view(rows, groups, GROUP)
+    finite = torch.isfinite(v).all(-1)
+    top = v.abs().amax(-1) if v.numel() else v.new_zeros(rows, groups)
+    e = torch.frexp(torch.where(finite, top, torch.zeros_like(top))).exponent.clamp(-119, 126)
+    q = torch.ldexp(v, (7 - e).unsqueeze(-1)).round().clamp(-127, 127)
+    held.codes.copy_(torch.where(finite.unsqueeze(-1), q, torch.zeros_like(q)).view(rows, pitch))
+    held.scales.zero_()
+    held.scales[:, :groups] = torch.where(finite, e + 120, torch.full_like(e, 255)).to(torch.uint8)
+
+
+def _decode_cpu(held: Act8) -> torch.Tensor:
+    rows, pitch = held.codes.shape
+    groups = pitch // GROUP
+    s = held.scales[:, :groups].int()
+    v = torch.ldexp(held.codes.float().view(rows, groups, GROUP), (s - 127).unsqueeze(-1))
+    v = torch.where((s == 255).unsqueeze(-1), torch.full_like(v, math.nan), v)
+    return v.view(rows, pitch)[:, : held.shape[-1]].reshape(held.shape)
+
+
+def _function_cpu(x: torch.Tensor, kind: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    if kind == "gelu":
+        p = 0.5 * torch.erfc(-x * math.sqrt(0.5))
+        return x * p, p + x * torch.exp(-0.5 * x * x) / math.sqrt(2 * math.pi)
+    if kind == "gelu_tanh":
+        c, a = math.sqrt(2 / math.pi), 0.044715
+        xx = (x * x).clamp_max(1e4)
+        p = torch.sigmoid(2 * c * x * (1 + a * xx))
+        return x * p, p + 2 * c * x * p * (1 - p) * (1 + 3 * a * xx)
+    p = torch.sigmoid(x)
+    return x * p, p * (1 + x * (1 - p))
+
+
+# ------------------------------------------------------------------------------------------------------- checkpoints
+def pack(x: torch.Tensor) -> Act8:
+    """The checkpoint of ``x`` (fp32, bf16 or fp16, any shape and strides)."""
+    _check_tensor(x, "act8.pack")
+    held = empty_like(x.shape, x.dtype, x.device)
+    if x.is_cuda:
+        v, cols = _rows(x), x.shape[-1]
+        with _on(x.device):
+            native().act8_pack(v.data_ptr(), v.stride(0), held.rows, cols, GRAD_DTYPE[x.dtype], *_ptrs(held), held.codes.shape[1],
+                               held.scales.shape[1], _stream(x.device))
+    else:
+        _encode_cpu(x, held)
+    return held
+
+
+def unpack(held: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values that ``held`` stands for, contiguous, as its own or another of the three types."""
+    dtype = held.dtype if dtype is None else dtype
+    if dtype not in GRAD_DTYPE:
+        raise TypeError("act8.unpack: fp32, bf16 or fp16, not %s" % dtype)
+    if held.codes.is_cuda:
+        out, cols = torch.empty(held.shape, dtype=dtype, device=held.device), held.shape[-1]
+        with _on(held.device):
+            native().act8_unpack(*_ptrs(held), held.codes.shape[1], held.scales.shape[1], out.data_ptr(), cols, held.rows, cols,
+                                 GRAD_DTYPE[dtype], _stream(held.device))
+        return out
+    return _decode_cpu(held).to(dtype)
+
+
+# --------------------------------------------------------------------------------------------------- weight gradient
+_sm_count = {}
+
+
+def _sms(device: torch.device) -> int:
+    n = _sm_count.get(device.index)
+    if n is None:
+        n = _sm_count[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
+
+
+def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optional[torch.dtype] = None
+                ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(dW, db)`` of ``y = x W^T + b``: ``dW [outs, ins] = sum over rows of grad^T x~`` with ``x~`` the values of ``held``, and with
+    ``bias`` the column sums of ``grad`` (else None).  ``grad`` is ``[..., outs]`` with ``held``'s leading axes and, on the GPU,
+    bf16 or fp16 like it; the results are of ``grad``'s type or, with ``dtype=torch.float32``, not rounded below fp32."""
+    _check_tensor(grad, "act8.weight_grad: grad")
+    outs, ins, rows = grad.shape[-1], held.shape[-1], held.rows
+    if grad.shape[:-1] != held.shape[:-1]:
+        raise ValueError("act8.weight_grad: grad %s and the checkpoint %s differ in their leading axes"
+                         % (tuple(grad.shape), held.shape))
+    if grad.device != held.device:
+        raise ValueError("act8.weight_grad: grad is on %s, the checkpoint on %s" % (grad.device, held.device))
+    dtype = grad.dtype if dtype is None else dtype
+    if dtype not in (grad.dtype, torch.float32):
+        raise TypeError("act8.weight_grad: results in grad's type or fp32, not %s" % dtype)
+    if not grad.is_cuda:
+        g = _rows(grad).float()
+        return (g.t() @ _decode_cpu(held).reshape(rows, ins)).to(dtype), g.sum(0).to(dtype) if bias else None
+    if grad.dtype == torch.float32:
+        raise TypeError("act8.weight_grad: the tensor cores take bf16 or fp16 gradients; run the layer in one of them")
+    if rows > MAX_TOKENS or outs * 2 > 1 << 31:
+        raise ValueError("act8.weight_grad: at most 2^31 - 64 rows and 2^30 output features")
+    if rows == 0 or outs == 0 or ins == 0:
+        return (torch.zeros((outs, ins), dtype=dtype, device=grad.device),
+                torch.zeros(outs, dtype=dtype, device=grad.device) if bias else None)
+    C, g = native(), _rows(grad)
+    with _on(grad.device):
+        stream = _stream(grad.device)
+        if g.data_ptr() % 16 or g.stride(0) % 8 or g.stride(0) < outs:   # not what a TMA load takes
+            wide = torch.empty((rows, -(-outs // 8) * 8), dtype=g.dtype, device=g.device)
+            C.act8_repitch(g.data_ptr(), g.stride(0), wide.data_ptr(), rows, outs, stream)
+            g = wide
+        out = torch.empty((outs, ins), dtype=dtype, device=grad.device)
+        db = torch.empty(outs, dtype=dtype, device=grad.device) if bias else None
+        C.act8_wgrad(g.data_ptr(), g.stride(0), *_ptrs(held), held.codes.shape[1], held.scales.shape[1], rows, outs, ins,
+                     GRAD_DTYPE[g.dtype], int(dtype == torch.float32), out.data_ptr(), db.data_ptr() if bias else 0,
+                     _sms(grad.device), stream)
+    return out, db
+
+
+def check(device=None) -> None:
+    """Waits for the device and raises ``GraceCommError`` if a bounded wait of a ``weight_grad`` kernel ran out since the last
+    check (its results are NaN)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with _on(device):
+        words = native().act8_wgrad_status()
+    if words[0]:
+        raise GraceCommError(words[0], words[1], words[2], 0)
+
+
+# ----------------------------------------------------------------------------------------------- activation functions
+Held = Union[Act8, Tuple[Act8, Act8]]
+
+
+def _kind(kind: str) -> int:
+    if kind not in KINDS:
+        raise ValueError("act8: unknown function %r (one of %s)" % (kind, ", ".join(KINDS)))
+    return KINDS[kind]
+
+
+def activation_forward(x: torch.Tensor, kind: str = "gelu", gated: bool = False, checkpoint_output: bool = False,
+                       checkpoint: bool = True) -> Tuple[torch.Tensor, Optional[Held], Optional[Act8]]:
+    """``(y, held, held_y)``: ``y = f(x)``, or for a gated function ``x = [a | b]`` and ``y = f(a) * b``; ``held`` is the checkpoint of
+    ``x`` (a pair of them, of ``a`` and of ``b``; None with ``checkpoint=False``, where no backward pass follows), ``held_y`` with
+    ``checkpoint_output`` that of ``y`` (what ``pack(y)`` gives), else None."""
+    k = _kind(kind)
+    _check_tensor(x, "act8.activation")
+    if gated and x.shape[-1] % 2:
+        raise ValueError("act8.activation: a gated function takes two halves, not %d columns" % x.shape[-1])
+    cols = x.shape[-1] // 2 if gated else x.shape[-1]
+    shape = x.shape[:-1] + (cols,)
+    a = empty_like(shape, x.dtype, x.device) if checkpoint else None
+    b = empty_like(shape, x.dtype, x.device) if checkpoint and gated else None
+    out = empty_like(shape, x.dtype, x.device) if checkpoint_output else None
+    if x.is_cuda:
+        y, v = torch.empty(shape, dtype=x.dtype, device=x.device), _rows(x)
+        with _on(x.device):
+            native().act8_forward(v.data_ptr(), v.stride(0), y.data_ptr(), v.shape[0], cols, GRAD_DTYPE[x.dtype], k, int(gated), *_ptrs(a),
+                                  *_ptrs(b), *_ptrs(out), *pitch_of(cols), _stream(x.device))
+    else:
+        v = x.detach()
+        y = _function_cpu(v[..., :cols].float(), kind)[0]
+        if gated:
+            y = y * v[..., cols:].float()
+        y = y.to(x.dtype)
+        for part, into in ((v[..., :cols], a), (v[..., cols:], b), (y, out)):
+            if into is not None:
+                _encode_cpu(part, into)
+    return y, (a, b) if b is not None else a, out
+
+
+def activation_backward(grad: torch.Tensor, held: Held, kind: str = "gelu", gated: bool = False) -> torch.Tensor:
+    """The gradient of ``activation_forward``'s ``x`` from that of ``y``, at the values that ``held`` stands for."""
+    k = _kind(kind)
+    _check_tensor(grad, "act8.activation: grad")
+    if gated != isinstance(held, tuple):
+        raise ValueError("act8.activation: a gated function has a pair of checkpoints, another one of them")
+    a, b = held if gated else (held, None)
+    if tuple(grad.shape) != a.shape or (gated and b.shape != a.shape):
+        raise ValueError("act8.activation: grad %s for a checkpoint of %s" % (tuple(grad.shape), a.shape))
+    if grad.device != a.device or (gated and b.device != a.device):
+        raise ValueError("act8.activation: grad is on %s, the checkpoint on %s" % (grad.device, a.device))
+    cols = a.shape[-1]
+    if grad.is_cuda:
+        dx = torch.empty(grad.shape[:-1] + (cols * (2 if gated else 1),), dtype=grad.dtype, device=grad.device)
+        g = _rows(grad)
+        with _on(grad.device):
+            native().act8_backward(g.data_ptr(), g.stride(0), dx.data_ptr(), a.rows, cols, GRAD_DTYPE[grad.dtype], k, int(gated),
+                                   *_ptrs(a), *_ptrs(b), a.codes.shape[1], a.scales.shape[1], _stream(grad.device))
+        return dx
+    g = grad.detach().float()
+    f, d = _function_cpu(_decode_cpu(a), kind)
+    return (torch.cat([g * _decode_cpu(b) * d, g * f], -1) if gated else g * d).to(grad.dtype)
+
+
+# ------------------------------------------------------------------------------------------------------ with autograd
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, codes, scales):
+        ctx.save_for_backward(codes, scales, weight)
+        ctx.x_shape, ctx.has_bias = x.shape, bias is not None
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, scales, weight = ctx.saved_tensors
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = grad @ weight
+        want_bias = ctx.has_bias and ctx.needs_input_grad[2]
+        if ctx.needs_input_grad[1]:
+            dw, db = weight_grad(grad, Act8(codes, scales, ctx.x_shape, grad.dtype), bias=want_bias)
+        elif want_bias:
+            db = grad.reshape(-1, grad.shape[-1]).sum(0)
+        return dx, dw, db, None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, checkpoint: Optional[Act8] = None
+           ) -> torch.Tensor:
+    """``x W^T + b`` whose backward pass keeps an 8-bit checkpoint of ``x`` in the place of ``x``.  ``checkpoint``: that of ``x``, where
+    the operation that made ``x`` wrote it already (``activation`` and ``residual_norm`` do on request)."""
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        t = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(t), weight.to(t), None if bias is None else bias.to(t)
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        return F.linear(x, weight, bias)       # nothing reads x again
+    _check_tensor(x, "act8.linear")
+    if x.is_cuda and x.dtype == torch.float32:
+        raise TypeError("act8.linear: bf16 or fp16 on the GPU (or fp32 under autocast): the weight gradient runs on the tensor cores")
+    if checkpoint is None:
+        checkpoint = pack(x)
+    elif checkpoint.shape != tuple(x.shape) or checkpoint.device != x.device:
+        raise ValueError("act8.linear: a checkpoint of %s on %s for x %s on %s"
+                         % (checkpoint.shape, checkpoint.device, tuple(x.shape), x.device))
+    return _Linear.apply(x, weight, bias, checkpoint.codes, checkpoint.scales)
+
+
+class _Activation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kind, gated, checkpoint_output):
+        y, held, out = activation_forward(x, kind, gated, checkpoint_output)
+        parts = held if gated else (held,)
+        ctx.save_for_backward(*(t for h in parts for t in (h.codes, h.scales)))
+        ctx.kind, ctx.gated, ctx.shape, ctx.dtype = kind, gated, parts[0].shape, x.dtype
+        if out is None:
+            return y
+        ctx.mark_non_differentiable(out.codes, out.scales)
+        return y, out.codes, out.scales
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        t = ctx.saved_tensors
+        held = tuple(Act8(t[i], t[i + 1], ctx.shape, ctx.dtype) for i in range(0, len(t), 2))
+        return activation_backward(grad, held if ctx.gated else held[0], ctx.kind, ctx.gated), None, None, None
+
+
+def activation(x: torch.Tensor, kind: str = "gelu", gated: bool = False, checkpoint_output: bool = False):
+    """``activation_forward`` with autograd: ``y``, or with ``checkpoint_output`` the pair ``(y, Act8 of y)`` for the ``linear`` after it."""
+    if not (torch.is_grad_enabled() and x.requires_grad):
+        y, _, held_y = activation_forward(x, kind, gated, checkpoint_output, checkpoint=False)
+        return (y, held_y) if checkpoint_output else y
+    got = _Activation.apply(x, kind, gated, checkpoint_output)
+    if not checkpoint_output:
+        return got
+    y, codes, scales = got
+    return y, Act8(codes, scales, y.shape, y.dtype)

@@ -1,0 +1,289 @@
+"""The kernels of 8-bit activation checkpoints against 64-bit arithmetic."""
+import math
+
+import pytest
+import torch
+
+from _act8_oracle import close, function, half_step, held_value
+from grace_b200.ops import act8
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def rand(*shape, seed=0, dtype=FP32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+# ---------------------------------------------------------------------------------------------------------- checkpoints
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 32), (1, 33), (3, 7), (5, 64), (2, 3, 100), (37, 1003), (300, 256), (1, 8200), (2049, 40)])
+def test_round_trip(shape, dtype):
+    x = rand(*shape, dtype=dtype, scale=3.0)
+    held = act8.pack(x)
+    host = act8.pack(x.cpu())
+    groups = -(-shape[-1] // 32)
+    assert torch.equal(held.codes.cpu(), host.codes) and torch.equal(held.scales[:, :groups].cpu(), host.scales[:, :groups])
+    close(act8.unpack(held).cpu(), held_value(x.cpu()), 2.0 ** -25 if dtype == FP16 else 0.0, "unpack")
+    assert torch.equal(act8.unpack(held, FP32).cpu().double(), held_value(x.cpu()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_strides_and_offsets(dtype):
+    wide = rand(40, 210, dtype=dtype, seed=1)
+    for x in (wide[:, 3:103], wide[::2, :96], wide.t(), wide[:, 5], wide[0].expand(6, 210), wide.view(8, 5, 210)[:, 1:3, 8:40],
+              wide[:, ::2]):
+        assert torch.equal(act8.unpack(act8.pack(x)), act8.unpack(act8.pack(x.contiguous())))
+        assert torch.equal(act8.unpack(act8.pack(x), FP32).cpu().double(), held_value(x.cpu()))
+
+
+def test_empty():
+    for shape in ((0, 64), (4, 0), (0,), (0, 0)):
+        x = torch.empty(shape, device="cuda", dtype=BF16)
+        assert act8.unpack(act8.pack(x)).shape == shape
+        assert act8.activation(x, "silu").shape == shape
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_extremes(dtype):
+    top = float(torch.finfo(dtype).max)
+    x = torch.zeros(8, 64)
+    x[0, 3], x[1, 40], x[2, 5], x[3, 6] = math.inf, math.nan, -math.inf, top
+    x[4, :2] = torch.tensor([float(torch.finfo(dtype).tiny), -float(torch.finfo(dtype).tiny) / 4])
+    x[5, 32:] = 1.0
+    x[6, :8] = torch.tensor([64.0, 0.5, 1.5, 2.5, -0.5, -1.5, 127.5, -126.5])
+    x = x.to(dtype)
+    got = act8.unpack(act8.pack(x.cuda()), FP32).cpu()
+    assert got[0, :32].isnan().all() and got[1, 32:].isnan().all() and got[2, :32].isnan().all() and not got[:3].isnan().all(-1).any()
+    close(got, held_value(x), 0.0)
+
+
+def test_more_chunks_than_31_bits_count_as_slabs():
+    """Offsets in a tensor of more than 2^32 elements (the last rows are compared)."""
+    rows, cols = (1 << 32) // 4096 + 3, 4096
+    x = torch.zeros(rows, cols, dtype=FP16, device="cuda")
+    x[-3:] = rand(3, cols, dtype=FP16, seed=2)
+    held = act8.pack(x)
+    assert torch.equal(act8.unpack(act8.Act8(held.codes[-3:], held.scales[-3:], (3, cols), FP16)), act8.unpack(act8.pack(x[-3:])))
+    del x
+    assert torch.equal(act8.unpack(held)[-3:], act8.unpack(act8.Act8(held.codes[-3:], held.scales[-3:], (3, cols), FP16)))
+
+
+# ------------------------------------------------------------------------------------------------- activation functions
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", [(1, 32), (3, 45), (65, 264)])
+def test_activation(shape, kind, gated, dtype):
+    rows, f = shape
+    x = rand(rows, f * (2 if gated else 1), dtype=dtype, seed=3, scale=2.5)
+    g = rand(rows, f, dtype=dtype, seed=4)
+    y, held, out = act8.activation_forward(x, kind, gated=gated, checkpoint_output=True)
+    dx = act8.activation_backward(g, held, kind, gated=gated)
+    v, gd = x.cpu().double(), g.cpu().double()
+    a, b = v[:, :f], v[:, f:]
+    # the functions: 1.5e-7 / 2 of the error function's approximation and a few fp32 roundings, times |x|; then one rounding
+    eps, least = half_step(dtype), 2.0 ** -25 if dtype == FP16 else 0.0
+    want = function(a, kind)[0] * (b if gated else 1)
+    f_err = 1e-6 * (1 + a.abs())
+    close(y, want, eps * want.abs() + f_err * (b.abs() if gated else 1) + least, "y")
+    assert torch.equal(act8.unpack(out, FP32).cpu().double(), held_value(y.cpu()))
+    assert torch.equal(out.codes, act8.pack(y).codes)
+    ha, hb = held_value(x[:, :f].cpu()), held_value(x[:, f:].cpu())
+    fa, da = function(ha, kind)
+    f_err = 1e-6 * (1 + ha.abs())
+    if gated:
+        want = torch.cat([gd * hb * da, gd * fa], -1)
+        tol = torch.cat([gd.abs() * hb.abs() * f_err, gd.abs() * f_err], -1)
+    else:
+        want, tol = gd * da, gd.abs() * f_err
+    close(dx, want, eps * want.abs() + tol + 3 * 2.0 ** -24 * want.abs() + least, "dx")
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+def test_activation_far_out(kind):
+    x = torch.tensor([-3e38, -1e30, -200.0, -90.0, -13.0, -8.0, 0.0, 8.0, 13.0, 90.0, 200.0, 1e30]).view(-1, 1).to(BF16)
+    y, held, _ = act8.activation_forward(x.cuda(), kind)
+    dx = act8.activation_backward(torch.ones_like(x).cuda(), held, kind)
+    f, _ = function(x, kind)
+    d = torch.where(x.double() > 9, 1.0, torch.where(x.double() < -20, 0.0, function(held_value(x).clamp(-20, 20), kind)[1]))
+    close(y, f, half_step(BF16) * f.abs() + 2e-5, "y")
+    close(dx, d, half_step(BF16) * d.abs() + 2e-5, "dx")
+
+
+def test_activation_strided_and_autograd():
+    wide = rand(6, 5, 200, dtype=BF16, seed=5)
+    x = wide[:, :, 4:132].requires_grad_()
+    y, held = act8.activation(x, "silu", gated=True, checkpoint_output=True)
+    g = rand(6, 64, 5, dtype=BF16, seed=6).transpose(1, 2)
+    dx, = torch.autograd.grad(y, x, g)
+    y2, held2, _ = act8.activation_forward(x.detach().contiguous(), "silu", gated=True)
+    assert torch.equal(y, y2) and torch.equal(dx, act8.activation_backward(g.contiguous(), held2, "silu", gated=True))
+    with torch.no_grad():
+        assert torch.equal(act8.activation(x, "silu", gated=True), y)
+
+
+# ------------------------------------------------------------------------------------------------------ weight gradient
+def check_weight_grad(tokens, outs, ins, dtype, out, bias=True, seed=7, x=None, g=None):
+    x = rand(tokens, ins, dtype=dtype, seed=seed) if x is None else x
+    g = rand(tokens, outs, dtype=dtype, seed=seed + 1, scale=0.1) if g is None else g
+    dw, db = act8.weight_grad(g, act8.pack(x), bias=bias, dtype=out)
+    assert dw.dtype == out and dw.shape == (outs, ins)
+    gd, xd = g.cpu().double(), held_value(x.cpu())
+    want, size = gd.t() @ xd, gd.abs().t() @ xd.abs()
+    # one truncated fp32 addition for 16 tokens and the joins of up to 8 partial sums, then one rounding to the type
+    least = 2.0 ** -25 if out == FP16 else 0.0
+    tail = 2.0 ** -25 * gd.abs().sum(0).view(-1, 1) if dtype == FP16 else 0.0     # fp16 operands: subnormal values are rounded
+    close(dw, want, half_step(out) * want.abs() + (tokens / 16 + 24) * 2.0 ** -23 * size + least + tail, "dW")
+    if bias:
+        want, size = gd.sum(0), gd.abs().sum(0)
+        close(db, want, half_step(out) * want.abs() + (tokens + 8) * 2.0 ** -24 * size + least, "db")
+    else:
+        assert db is None
+    return dw, db
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 63, 64, 65, 200, 513, 1100])
+@pytest.mark.parametrize("outs,ins", [(64, 32), (8, 128), (256, 128), (264, 160), (1000, 96)])
+def test_weight_grad(tokens, outs, ins):
+    check_weight_grad(tokens, outs, ins, BF16, BF16)
+
+
+@pytest.mark.parametrize("dtype,out", [(BF16, FP32), (FP16, FP16), (FP16, FP32)])
+@pytest.mark.parametrize("tokens,outs,ins", [(1, 1, 1), (100, 72, 40), (777, 101, 1003), (2000, 600, 257)])
+def test_weight_grad_types_and_odd_sizes(tokens, outs, ins, dtype, out):
+    check_weight_grad(tokens, outs, ins, dtype, out)
+
+
+@pytest.mark.parametrize("tokens,outs,ins", [(4096, 1024, 1024), (16384, 512, 640), (300, 4096, 2500)])
+def test_weight_grad_larger(tokens, outs, ins):
+    check_weight_grad(tokens, outs, ins, BF16, FP32, bias=True)
+    check_weight_grad(tokens, outs, ins, BF16, BF16, bias=False)
+
+
+def test_weight_grad_one_column_of_tiles_has_every_bias_column():
+    check_weight_grad(130, 700, 20, BF16, FP32)          # one tile along the inputs: a CTA adds up all 256 columns
+    check_weight_grad(130, 30, 128 * 130, BF16, FP32)    # 130 of them: two columns each, most CTAs none
+
+
+def test_weight_grad_strides():
+    g, x = rand(3, 70, 200, dtype=BF16, seed=8), rand(3, 70, 64, dtype=BF16, seed=9)
+    held = act8.pack(x)
+    for part in (g[..., 8:136], g[..., 1:130], g.transpose(0, 1).contiguous().transpose(0, 1)[..., :64], g[:, :1].expand(3, 70, 200)):
+        a, b = act8.weight_grad(part, held, bias=True), act8.weight_grad(part.contiguous(), held, bias=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_weight_grad_scales_differ_by_group_and_token():
+    x = torch.zeros(96, 96)
+    x[:, :32] = torch.exp2(torch.arange(96) % 60 - 30.0).view(-1, 1) * torch.randn(96, 32, generator=torch.Generator().manual_seed(1))
+    x[:, 64:] = torch.randn(96, 32, generator=torch.Generator().manual_seed(2)) * 1e-3
+    check_weight_grad(96, 64, 96, BF16, FP32, x=x.to(BF16).cuda())
+
+
+def test_weight_grad_non_finite_values_reach_their_rows_and_columns_only():
+    x, g = rand(100, 96, dtype=BF16, seed=10), rand(100, 64, dtype=BF16, seed=11)
+    x[7, 40] = math.inf
+    dw, db = act8.weight_grad(g, act8.pack(x), bias=True)
+    assert dw[:, 32:64].isnan().all() and dw[:, :32].isfinite().all() and dw[:, 64:].isfinite().all() and db.isfinite().all()
+    g[3, 5] = math.nan
+    dw, db = act8.weight_grad(g, act8.pack(rand(100, 96, dtype=BF16)), bias=True)
+    assert dw[5].isnan().all() and dw[:5].isfinite().all() and dw[6:].isfinite().all() and db.isnan().sum() == 1
+
+
+def test_weight_grad_same_bits_twice_and_no_failure():
+    x, g = rand(2500, 300, dtype=BF16, seed=12), rand(2500, 280, dtype=BF16, seed=13)
+    held = act8.pack(x)
+    a, b = act8.weight_grad(g, held, bias=True), act8.weight_grad(g, held, bias=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    act8.check()
+
+
+def test_weight_grad_refusals():
+    held = act8.pack(rand(8, 64, dtype=BF16))
+    with pytest.raises(TypeError):
+        act8.weight_grad(rand(8, 64), held)
+    with pytest.raises(TypeError):
+        act8.weight_grad(rand(8, 64, dtype=BF16), held, dtype=FP16)
+    with pytest.raises(ValueError):
+        act8.weight_grad(rand(9, 64, dtype=BF16), held)
+    with pytest.raises(ValueError):
+        act8.weight_grad(rand(8, 64, dtype=BF16).cpu(), held)
+    with pytest.raises(TypeError):
+        act8.linear(rand(8, 64).requires_grad_(), rand(4, 64).requires_grad_())
+    dw, db = act8.weight_grad(torch.empty(0, 16, dtype=BF16, device="cuda"), act8.pack(torch.empty(0, 64, dtype=BF16, device="cuda")), bias=True)
+    assert dw.shape == (16, 64) and not dw.any() and not db.any()
+
+
+# ----------------------------------------------------------------------------------------------------------- as a layer
+def test_linear_and_activation_together():
+    x, w1, b1, w2 = (rand(50, 64, dtype=BF16, seed=14), rand(128, 64, dtype=BF16, seed=15, scale=0.2), rand(128, dtype=BF16, seed=16),
+                     rand(64, 128, dtype=BF16, seed=17, scale=0.2))
+    leaves = [t.requires_grad_() for t in (x, w1, b1, w2)]
+    h = act8.linear(x, w1, b1)
+    a, held = act8.activation(h, "gelu", checkpoint_output=True)
+    y = act8.linear(a, w2, checkpoint=held)
+    g = rand(50, 64, dtype=BF16, seed=18)
+    y.backward(g)
+    da = g @ w2
+    dh = act8.activation_backward(da, act8.pack(h), "gelu")
+    dw1, db1 = act8.weight_grad(dh, act8.pack(x), bias=True)
+    assert torch.equal(w2.grad, act8.weight_grad(g, act8.pack(a))[0])
+    assert torch.equal(w1.grad, dw1) and torch.equal(b1.grad, db1) and torch.equal(x.grad, dh @ w1)
+    ref = [t.detach().clone().requires_grad_() for t in leaves]
+    full = torch.nn.functional.gelu(torch.nn.functional.linear(ref[0], ref[1], ref[2])) @ ref[3].t()
+    full.backward(g)
+    for p, q in zip(leaves, ref):     # against the layer that keeps everything: the codes' steps, 2^-7 of their group's leading power at most
+        assert (p.grad - q.grad).float().norm() < 0.05 * q.grad.float().norm()
+
+
+def test_autocast():
+    x, w, b = rand(40, 64, seed=19).requires_grad_(), rand(32, 64, seed=20).requires_grad_(), rand(32, seed=21).requires_grad_()
+    with torch.autocast("cuda", dtype=BF16):
+        y = act8.linear(x, w, b)
+    assert y.dtype == BF16
+    y.float().sum().backward()
+    assert w.grad.dtype == FP32 and x.grad.dtype == FP32 and torch.equal(b.grad, torch.full_like(b, 40.0))
+
+
+def test_graph_replay_and_two_graphs():
+    """Captured calls replay on new values; two graphs and eager calls in between do not share anything."""
+    x, g = rand(700, 256, dtype=BF16, seed=22), rand(700, 520, dtype=BF16, seed=23)
+
+    def step():
+        a, held, out = act8.activation_forward(x, "gelu", checkpoint_output=True)
+        dw, db = act8.weight_grad(g, out, bias=True)
+        return a, dw, db, act8.activation_backward(a, held, "gelu")
+
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for seed in (24, 25):
+        x.copy_(rand(700, 256, dtype=BF16, seed=seed))
+        g.copy_(rand(700, 520, dtype=BF16, seed=seed + 10))
+        graphs[0].replay()
+        want = step()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for got in outs:
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_side_stream():
+    x, g = rand(3000, 512, dtype=BF16, seed=26), rand(3000, 512, dtype=BF16, seed=27)
+    want = act8.weight_grad(g, act8.pack(x))[0]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        big = torch.zeros(1 << 28, device="cuda")      # the side stream is busy when the calls are made
+        big.add_(1)
+        y = x * 1
+        got = act8.weight_grad(g, act8.pack(y))[0]
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
