@@ -4,6 +4,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <array>
 #include <cerrno>
 #include <cstring>
 #include <stdexcept>
@@ -40,6 +41,19 @@ PeerTable make_peers(int rank, int world, unsigned long long seq, unsigned long 
 
 Held held(uintptr_t codes, uintptr_t scales, int pitch, int spitch) {
   return {ptr<signed char>(codes), ptr<unsigned char>(scales), pitch, spitch};
+}
+
+BlockNormArgs block_norm_args(long long rows, int cols, int pre, int post, int params_f32, float alpha, float eps, long long gate_rows,
+                              const std::array<uintptr_t, 5>& params, uintptr_t stats) {
+  if (pre < kNormRms || pre > kNormLayer || post < kNormNone || post > kNormLayer) throw std::invalid_argument("block_norm: unknown norm");
+  if (gate_rows < 0 || (gate_rows && rows % gate_rows)) throw std::invalid_argument("block_norm: rows are not whole sequences");
+  BlockNormArgs a{};
+  a.rows = rows; a.cols = cols; a.pre = pre; a.post = post; a.params_f32 = params_f32; a.alpha = alpha; a.eps = eps;
+  a.gate_rows = gate_rows;
+  a.pre_weight = ptr<const void>(params[0]); a.pre_bias = ptr<const void>(params[1]); a.post_weight = ptr<const void>(params[2]);
+  a.post_bias = ptr<const void>(params[3]); a.gate = ptr<const void>(params[4]);
+  a.stats = ptr<float>(stats);
+  return a;
 }
 
 }  // namespace
@@ -324,6 +338,44 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
     check(act8_wgrad_status(words.data()), "act8_wgrad_status");
     return words;
   });
+
+  // ---- residual and norm step between two blocks ----
+  m.attr("BLOCK_NORM_MAX_COLS") = (int)kBlockNormMaxCols;
+  m.def("block_norm_sum_rows", [](long long rows, int cols, long long gate_rows, int sms) {
+    const BlockNormShape s = block_norm_shape(rows, cols, gate_rows, sms);
+    return (long long)s.runs * s.rpb;
+  });
+  // params: pre_weight, pre_bias, post_weight, post_bias, gate; held: codes and scales of y, block and h
+  m.def("block_norm_forward",
+        [](uintptr_t x, long long x_stride, uintptr_t block, long long block_stride, uintptr_t h, uintptr_t y, uintptr_t stats,
+           long long rows, int cols, int dtype, int pre, int post, int params_f32, float alpha, float eps, long long gate_rows,
+           const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 6>& helds, int pitch, int spitch, uintptr_t stream) {
+          BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, eps, gate_rows, params, stats);
+          a.held_y = held(helds[0], helds[1], pitch, spitch);
+          a.held_b = held(helds[2], helds[3], pitch, spitch);
+          a.held_h = held(helds[4], helds[5], pitch, spitch);
+          a.x = ptr<const void>(x); a.x_stride = x_stride; a.block = ptr<const void>(block); a.block_stride = block_stride;
+          a.h = ptr<void>(h); a.y = ptr<void>(y);
+          check(launch_block_norm_forward(a, dtype, reinterpret_cast<cudaStream_t>(stream)), "block_norm_forward");
+        });
+  // grads: of params, in their order
+  m.def("block_norm_backward",
+        [](uintptr_t grad_h, long long grad_h_stride, uintptr_t grad_y, long long grad_y_stride, uintptr_t dx, uintptr_t dblock,
+           uintptr_t stats, uintptr_t sums, long long rows, int cols, int dtype, int pre, int post, int params_f32, float alpha,
+           long long gate_rows, const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 5>& grads,
+           const std::array<uintptr_t, 4>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
+          BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, 0.f, gate_rows, params, stats);
+          a.held_y = held(helds[0], helds[1], pitch, spitch);
+          a.held_b = held(helds[2], helds[3], pitch, spitch);
+          if (!a.held_y.codes || !stats || ((post || params[4]) && !a.held_b.codes))
+            throw std::invalid_argument("block_norm_backward: a checkpoint is missing");
+          a.grad_h = ptr<const void>(grad_h); a.grad_h_stride = grad_h_stride;
+          a.grad_y = ptr<const void>(grad_y); a.grad_y_stride = grad_y_stride;
+          a.dx = ptr<void>(dx); a.dblock = ptr<void>(dblock); a.sums = ptr<float>(sums);
+          a.pre_weight_grad = ptr<void>(grads[0]); a.pre_bias_grad = ptr<void>(grads[1]); a.post_weight_grad = ptr<void>(grads[2]);
+          a.post_bias_grad = ptr<void>(grads[3]); a.gate_grad = ptr<void>(grads[4]);
+          check(launch_block_norm_backward(a, dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_backward");
+        });
 
   // ---- host engine of the exchange protocol (CPU ranks over POSIX shared memory) ----
   m.attr("HOST_MAX_WORLD") = host::kMaxWorld;

@@ -1,0 +1,279 @@
+"""The step between two blocks of a transformer as one kernel each way: the norm after a block, its gate, the scaled
+residual, and the norm before the next block, with 8-bit checkpoints (``ops/act8.py``) for the backward pass.
+
+    n = N_post(block)                          (post=None: block)
+    y = residual_scale * x + gate * n          the residual stream, rounded to its type
+    h = N_pre(y)                               the next block's input
+
+``pre`` and ``post`` are ``"rms"`` (``v / sqrt(mean v^2 + eps) * weight``) or ``"layer"`` (``(v - mean) / sqrt(var + eps) * weight +
+bias``); a missing weight is ones.  ``gate`` is ``[cols]`` or, for ``x`` of three axes and more, ``[x.shape[0], cols]``: a row for
+each sequence.  "Add and norm" of a post-norm layer is ``pre="layer"`` with nothing else and ``return_stream=False``; DeepNorm's is the same with
+``residual_scale``; a sandwich norm has both.
+
+What the forward pass keeps: a checkpoint of ``y``, with ``post`` or a gate one of ``block``, and four fp32 statistics a row.
+Gradients are those of the formulas above at the checkpoints' values of ``y`` and ``block`` with the statistics of the full-precision
+ones; parameter gradients are fp32 sums in a fixed order, rounded once to the parameter's type.
+"""
+from __future__ import annotations
+
+import math
+from typing import Dict, NamedTuple, Optional, Tuple
+
+import torch
+
+from . import native
+from .act8 import Act8, _check_tensor, _decode_cpu, _encode_cpu, _on, _ptrs, _rows, _sms, _stream, empty_like, pitch_of
+from .exchange import GRAD_DTYPE
+
+NORMS = {None: 0, "rms": 1, "layer": 2}
+MAX_COLS = 8192      # a row is held in the registers of one CTA (block_norm.cu: kBlockNormMaxCols)
+MAX_ROWS = (1 << 31) - 1
+MAX_SEQUENCES = 65534
+PARAMS = ("pre_weight", "pre_bias", "post_weight", "post_bias", "gate")
+
+
+class Saved(NamedTuple):
+    """What the backward pass takes from the forward pass."""
+
+    held_y: Act8
+    held_block: Optional[Act8]
+    stats: torch.Tensor                  # fp32 [rows, 4]: mean and 1 / deviation of y, then of block
+    params: Tuple[Optional[torch.Tensor], ...]    # as PARAMS
+    pre: str
+    post: Optional[str]
+    residual_scale: float
+    return_stream: bool
+    held_h: Optional[Act8] = None        # checkpoint of h for the layer that reads it, on request
+
+
+def _check(x, block, pre, post, params, residual_scale, eps) -> int:
+    """Rows of a sequence (0: the gate, if any, is the same for all rows)."""
+    _check_tensor(x, "residual_norm: x")
+    _check_tensor(block, "residual_norm: block")
+    if x.shape != block.shape or x.dtype != block.dtype or x.device != block.device:
+        raise ValueError("residual_norm: x %s %s on %s and block %s %s on %s have to be alike"
+                         % (tuple(x.shape), x.dtype, x.device, tuple(block.shape), block.dtype, block.device))
+    if pre not in ("rms", "layer") or post not in NORMS:
+        raise ValueError("residual_norm: pre is 'rms' or 'layer', post one of them or None, not %r and %r" % (pre, post))
+    cols, rows = x.shape[-1], math.prod(x.shape[:-1])
+    if cols > MAX_COLS or rows > MAX_ROWS:
+        raise ValueError("residual_norm: at most %d columns and 2^31 - 1 rows, not %d and %d" % (MAX_COLS, cols, rows))
+    if not (math.isfinite(residual_scale) and math.isfinite(eps) and eps >= 0):
+        raise ValueError("residual_norm: a finite residual_scale and eps >= 0, not %r and %r" % (residual_scale, eps))
+    if post is None and (params[2] is not None or params[3] is not None):
+        raise ValueError("residual_norm: post_weight or post_bias without a norm after the block")
+    if (pre == "rms" and params[1] is not None) or (post == "rms" and params[3] is not None):
+        raise ValueError("residual_norm: an RMS norm has no bias")
+    kinds = {p.dtype for p in params if p is not None}
+    if kinds - {x.dtype, torch.float32} or len(kinds) > 1:
+        raise TypeError("residual_norm: parameters are all %s or all fp32, not %s" % (x.dtype, sorted(map(str, kinds))))
+    gate_rows = 0
+    for name, p in zip(PARAMS, params):
+        if p is None:
+            continue
+        if p.device != x.device:
+            raise ValueError("residual_norm: %s is on %s, x on %s" % (name, p.device, x.device))
+        if name == "gate" and p.dim() == 2:
+            if x.dim() < 3 or tuple(p.shape) != (x.shape[0], cols):
+                raise ValueError("residual_norm: a gate of two axes has a row for each entry of the first of x's three or more axes, "
+                                 "not %s for x %s" % (tuple(p.shape), tuple(x.shape)))
+            if p.shape[0] > MAX_SEQUENCES:
+                raise ValueError("residual_norm: a gate has at most %d rows" % MAX_SEQUENCES)
+            gate_rows = rows // max(1, p.shape[0])
+        elif tuple(p.shape) != (cols,):
+            raise ValueError("residual_norm: %s is %s for %d columns" % (name, tuple(p.shape), cols))
+    return gate_rows
+
+
+def _param_ptrs(params):
+    """The parameters' addresses, and the tensors that have to live until the launch."""
+    kept = [None if p is None else p.detach().contiguous() for p in params]
+    return [0 if p is None else p.data_ptr() for p in kept], kept
+
+
+def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", pre_weight: Optional[torch.Tensor] = None,
+                          pre_bias: Optional[torch.Tensor] = None, post: Optional[str] = None, post_weight: Optional[torch.Tensor] = None,
+                          post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+                          eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False
+                          ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Saved]:
+    """``(h, y, saved)`` (``y`` None without ``return_stream``); with ``checkpoint_output`` ``saved.held_h`` is what ``act8.pack(h)`` gives."""
+    params = (pre_weight, pre_bias, post_weight, post_bias, gate)
+    gate_rows = _check(x, block, pre, post, params, residual_scale, eps)
+    cols, rows, two = x.shape[-1], math.prod(x.shape[:-1]), post is not None or gate is not None
+    held_y = empty_like(x.shape, x.dtype, x.device)
+    held_b = empty_like(x.shape, x.dtype, x.device) if two else None
+    held_h = empty_like(x.shape, x.dtype, x.device) if checkpoint_output else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device)
+    saved = Saved(held_y, held_b, stats, params, pre, post, float(residual_scale), return_stream, held_h)
+    if not x.is_cuda:
+        return _forward_cpu(x, block, saved, float(eps)) + (saved,)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_stream else None
+    vx, vb = _rows(x), _rows(block)
+    ptrs, kept = _param_ptrs(params)
+    with _on(x.device):
+        native().block_norm_forward(vx.data_ptr(), vx.stride(0), vb.data_ptr(), vb.stride(0), h.data_ptr(), 0 if y is None else y.data_ptr(),
+                                    stats.data_ptr(), rows, cols, GRAD_DTYPE[x.dtype], NORMS[pre], NORMS[post], _f32(params),
+                                    float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(held_y) + _ptrs(held_b) + _ptrs(held_h),
+                                    *pitch_of(cols), _stream(x.device))
+    del kept
+    return h, y, saved
+
+
+def _f32(params) -> int:
+    return int(any(p is not None and p.dtype == torch.float32 for p in params))
+
+
+def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor], saved: Saved, needs=(True,) * 5
+                           ) -> Dict[str, Optional[torch.Tensor]]:
+    """The gradients of ``x``, ``block`` and the parameters (``PARAMS``), by name; None where there is no such parameter or ``needs`` (as
+    ``PARAMS``) does not ask for it.  ``grad_y`` is that of the stream, None where nothing reads it.  Without ``post`` and gate and with a
+    ``residual_scale`` of 1, ``x`` and ``block`` have one gradient: both names give the same tensor."""
+    held_y, held_b, params = saved.held_y, saved.held_block, saved.params
+    shape, dtype, device = held_y.shape, held_y.dtype, held_y.device
+    for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
+        if g is None and name == "grad_y":
+            continue
+        _check_tensor(g, "residual_norm: " + name)
+        if tuple(g.shape) != shape or g.dtype != dtype or g.device != device:
+            raise ValueError("residual_norm: %s %s %s on %s for %s %s on %s" % (name, tuple(g.shape), g.dtype, g.device, shape, dtype, device))
+    gate = params[4]
+    want = [p is not None and n for p, n in zip(params, needs)]
+    cols, rows = shape[-1], math.prod(shape[:-1])
+    if device.type != "cuda":
+        return _backward_cpu(grad_h, grad_y, saved, want)
+    if rows == 0 or cols == 0:
+        empty = torch.empty(shape, dtype=dtype, device=device)
+        return dict(zip(("x", "block") + PARAMS, [empty, empty] + [torch.zeros_like(p) if w else None for p, w in zip(params, want)]))
+    one = saved.post is None and gate is None and saved.residual_scale == 1.0
+    block = torch.empty(shape, dtype=dtype, device=device)
+    dx = None if one else torch.empty(shape, dtype=dtype, device=device)
+    grads = [torch.empty(p.shape, dtype=p.dtype, device=device) if w else None for p, w in zip(params, want)]
+    gate_rows = rows // gate.shape[0] if gate is not None and gate.dim() == 2 else 0
+    C, sms = native(), _sms(device)
+    pitch, spitch = pitch_of(cols)
+    g, gy = _rows(grad_h), None if grad_y is None else _rows(grad_y)
+    ptrs, kept = _param_ptrs(params)
+    with _on(device):
+        sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * pitch, dtype=torch.float32, device=device) if any(want) else None
+        C.block_norm_backward(g.data_ptr(), g.stride(0), 0 if gy is None else gy.data_ptr(), 0 if gy is None else gy.stride(0),
+                              0 if dx is None else dx.data_ptr(), block.data_ptr(), saved.stats.data_ptr(),
+                              0 if sums is None else sums.data_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post],
+                              _f32(params), saved.residual_scale, gate_rows, ptrs, [0 if t is None else t.data_ptr() for t in grads],
+                              _ptrs(held_y) + _ptrs(held_b), pitch, spitch, sms, _stream(device))
+    del kept
+    got = dict(zip(PARAMS, grads))
+    got["x"], got["block"] = block if dx is None else dx, block
+    return got
+
+
+# ------------------------------------------------------------------------------------------------------------- on CPU
+def _wide(p: Optional[torch.Tensor], shape, none: float) -> torch.Tensor:
+    if p is None:
+        return torch.full((), none)
+    p = p.detach().float()
+    return p if p.dim() == 1 else p.view((p.shape[0],) + (1,) * (len(shape) - 2) + (p.shape[1],))
+
+
+def _stats_cpu(v, kind, eps):
+    mean = v.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(v[..., :1])
+    if kind is None:
+        return mean, torch.ones_like(mean)
+    return mean, ((v - mean).square().mean(-1, keepdim=True) + eps).rsqrt()
+
+
+def _forward_cpu(x, block, saved: Saved, eps: float):
+    pre_w, pre_b, post_w, post_b, gate = saved.params
+    b = block.detach().float()
+    mb, rb = _stats_cpu(b, saved.post, eps)
+    n = b if saved.post is None else (b - mb) * rb * _wide(post_w, x.shape, 1.0) + _wide(post_b, x.shape, 0.0)
+    if gate is not None:
+        n = n * _wide(gate, x.shape, 1.0)
+    y = (saved.residual_scale * x.detach().float() + n).to(x.dtype)
+    v = y.float()
+    m, r = _stats_cpu(v, saved.pre, eps)
+    h = ((v - m) * r * _wide(pre_w, x.shape, 1.0) + _wide(pre_b, x.shape, 0.0)).to(x.dtype)
+    saved.stats.copy_(torch.stack([t.reshape(-1) for t in (m, r, mb, rb)], -1))
+    for part, into in ((y, saved.held_y), (block.detach(), saved.held_block), (h, saved.held_h)):
+        if into is not None:
+            _encode_cpu(part, into)
+    return h, y if saved.return_stream else None
+
+
+def _norm_grad_cpu(c, hat, r, kind):
+    return r * (c - (c.mean(-1, keepdim=True) if kind == "layer" else 0.0) - hat * (c * hat).mean(-1, keepdim=True))
+
+
+def _backward_cpu(grad_h, grad_y, saved: Saved, want):
+    shape, dtype = saved.held_y.shape, saved.held_y.dtype
+    pre_w, _, post_w, post_b, gate = saved.params
+    m, r, mb, rb = (t.reshape(shape[:-1] + (1,)) for t in saved.stats.unbind(-1))
+    leading = tuple(range(len(shape) - 1))
+    got = dict.fromkeys(PARAMS)
+    dh = grad_h.detach().float()
+    hat = (_decode_cpu(saved.held_y) - m) * r
+    got["pre_weight"], got["pre_bias"] = (dh * hat).sum(leading), dh.sum(leading)
+    g = _norm_grad_cpu(dh * _wide(pre_w, shape, 1.0), hat, r, saved.pre)
+    if grad_y is not None:
+        g = g + grad_y.detach().float()
+    e = g if gate is None else g * _wide(gate, shape, 1.0)
+    if saved.held_block is not None:
+        b = _decode_cpu(saved.held_block)
+        bh = b if saved.post is None else (b - mb) * rb
+        if gate is not None:
+            n = bh * _wide(post_w, shape, 1.0) + _wide(post_b, shape, 0.0)
+            got["gate"] = (g * n).sum(leading if gate.dim() == 1 else leading[1:])
+        if saved.post is not None:
+            got["post_weight"], got["post_bias"] = (e * bh).sum(leading), e.sum(leading)
+            e = _norm_grad_cpu(e * _wide(post_w, shape, 1.0), bh, rb, saved.post)
+    got = {k: got[k].to(p.dtype) if w else None for k, p, w in zip(PARAMS, saved.params, want)}
+    got["x"], got["block"] = (saved.residual_scale * g).to(dtype), e.to(dtype)
+    return got
+
+
+# ------------------------------------------------------------------------------------------------------ with autograd
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, residual_scale, eps, return_stream,
+                checkpoint_output):
+        ctx.set_materialize_grads(False)
+        h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
+                                            post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps,
+                                            return_stream=return_stream, checkpoint_output=checkpoint_output)
+        held = [t for a in (saved.held_y, saved.held_block) if a is not None for t in (a.codes, a.scales)]
+        ctx.save_for_backward(*saved.params, saved.stats, *held)
+        ctx.kinds, ctx.shape, ctx.dtype = (pre, post, saved.residual_scale, return_stream), tuple(x.shape), x.dtype
+        out = (h,) + ((y,) if return_stream else ())
+        if checkpoint_output:
+            ctx.mark_non_differentiable(saved.held_h.codes, saved.held_h.scales)
+            out += (saved.held_h.codes, saved.held_h.scales)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_h, grad_y=None, *_):
+        t = ctx.saved_tensors
+        held = [Act8(t[i], t[i + 1], ctx.shape, ctx.dtype) for i in range(6, len(t), 2)]
+        pre, post, scale, stream = ctx.kinds
+        saved = Saved(held[0], held[1] if len(held) > 1 else None, t[5], tuple(t[:5]), pre, post, scale, stream)
+        if not stream:
+            grad_y = None
+        if grad_h is None and grad_y is None:
+            return (None,) * 13
+        if grad_h is None:
+            grad_h = torch.zeros(ctx.shape, dtype=ctx.dtype, device=t[5].device)
+        got = residual_norm_backward(grad_h, grad_y, saved, ctx.needs_input_grad[2:7])
+        return (got["x"], got["block"]) + tuple(got[k] for k in PARAMS) + (None,) * 6
+
+
+def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", pre_weight: Optional[torch.Tensor] = None,
+                  pre_bias: Optional[torch.Tensor] = None, post: Optional[str] = None, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+                  eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False):
+    """The step with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
+    alone comes as it is, several as a tuple."""
+    out = _ResidualNorm.apply(x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, float(residual_scale), float(eps),
+                              return_stream, checkpoint_output)
+    if checkpoint_output:
+        out = out[:-2] + (Act8(out[-2], out[-1], x.shape, x.dtype),)
+    return out[0] if len(out) == 1 else out

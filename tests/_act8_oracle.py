@@ -47,3 +47,70 @@ def close(got, want, tol, what=""):
         i = int(off.argmax())
         raise AssertionError("%s: element %d is %r, want %r within %r (%d of %d off)" % (
             what, i, got.flatten()[i].item(), want.flatten()[i].item(), tol.flatten()[i].item(), int((off > 0).sum()), off.numel()))
+
+
+# ------------------------------------------------------------------------------------- the residual-and-norm step
+def wide(p, dims, none):
+    """A parameter [cols], or a gate [sequences, cols], against [sequences, ..., cols]."""
+    if p is None:
+        return torch.full((), none, dtype=torch.float64)
+    p = p.double()
+    return p if p.dim() == 1 else p.view((p.shape[0],) + (1,) * (dims - 2) + (p.shape[1],))
+
+
+def norm_stats(v, kind, eps):
+    mean = v.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(v[..., :1])
+    rstd = 1 / torch.sqrt(((v - mean) ** 2).mean(-1, keepdim=True) + eps) if kind is not None else torch.ones_like(mean)
+    return mean, rstd
+
+
+def stream(x, block, post, post_weight, post_bias, gate, alpha, eps):
+    """y before its rounding, and the size of the terms it is made of."""
+    b = block.double()
+    m, r = norm_stats(b, post, eps)
+    n = (b - m) * r * wide(post_weight, b.dim(), 1.0) + wide(post_bias, b.dim(), 0.0)
+    size = (b.abs() + m.abs()) * r * wide(post_weight, b.dim(), 1.0).abs() + wide(post_bias, b.dim(), 0.0).abs()
+    g = wide(gate, b.dim(), 1.0)
+    return alpha * x.double() + g * n, abs(alpha) * x.double().abs() + g.abs() * size
+
+
+def normed(y, kind, weight, bias, eps):
+    """h and the size of its terms."""
+    v = y.double()
+    m, r = norm_stats(v, kind, eps)
+    w, b = wide(weight, v.dim(), 1.0), wide(bias, v.dim(), 0.0)
+    return (v - m) * r * w + b, (v.abs() + m.abs()) * r * w.abs() + b.abs()
+
+
+def _norm_back(c, size, hat, r, kind):
+    mean = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
+    out = r * (c - (mean(c) if kind == "layer" else 0.0) - hat * mean(c * hat))
+    return out, r * (size + (mean(size) if kind == "layer" else 0.0) + hat.abs() * mean(size * hat.abs()))
+
+
+def block_norm_gradients(dh, dy, y, y_stats, b, b_stats, pre, post, pre_weight, post_weight, post_bias, gate, alpha):
+    """{name: (gradient, size of its terms)} at the values y and b (b None: not kept) with the given (mean, rstd) of both."""
+    dims, lead = dh.dim(), tuple(range(dh.dim() - 1))
+    dh = dh.double()
+    (m, r), got = y_stats, {}
+    hat = (y - m) * r
+    got["pre_weight"], got["pre_bias"] = ((dh * hat).sum(lead), (dh * hat).abs().sum(lead)), (dh.sum(lead), dh.abs().sum(lead))
+    c = dh * wide(pre_weight, dims, 1.0)
+    g, size = _norm_back(c, c.abs(), hat, r, pre)
+    if dy is not None:
+        g, size = g + dy.double(), size + dy.double().abs()
+    got["x"] = (alpha * g, abs(alpha) * size)
+    gw = wide(gate, dims, 1.0)
+    e, e_size = g * gw, size * gw.abs()
+    if b is not None:
+        bm, br = b_stats
+        bh = b if post is None else (b - bm) * br
+        pw, pb = wide(post_weight, dims, 1.0), wide(post_bias, dims, 0.0)
+        if gate is not None:
+            over = lead if gate.dim() == 1 else lead[1:]
+            got["gate"] = ((g * (bh * pw + pb)).sum(over), (size * ((bh * pw).abs() + pb.abs())).sum(over))
+        if post is not None:
+            got["post_weight"], got["post_bias"] = ((e * bh).sum(lead), (e_size * bh.abs()).sum(lead)), (e.sum(lead), e_size.sum(lead))
+            e, e_size = _norm_back(e * pw, e_size * pw.abs(), bh, br, post)
+    got["block"] = (e, e_size)
+    return got

@@ -1,0 +1,141 @@
+"""The kernels of the residual-and-norm step against the 64-bit formulas."""
+import math
+
+import pytest
+import torch
+
+from _block_norm_cases import check, make
+from grace_b200.ops import act8, block_norm
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+FORMS = [("layer", None, None, 1.0, False), ("rms", None, None, 2.63, True), ("rms", "rms", "sequence", 1.0, True),
+         ("layer", "layer", "channel", 0.5, True), ("layer", "rms", None, 1.0, True), ("rms", None, "sequence", 1.0, False)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("pre,post,gate,alpha,with_stream", FORMS)
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 70), (3, 37, 256), (2, 5, 1000), (1, 33, 1003), (5, 7, 4096), (2, 9, 5001), (1, 3, 8192)])
+def test_against_formulas(shape, pre, post, gate, alpha, with_stream, dtype):
+    d, p = make(shape, dtype, pre, post, gate, seed=2, device="cuda")
+    check(d, p, alpha=alpha, with_stream=with_stream)
+
+
+@pytest.mark.parametrize("pre,post,gate,alpha,with_stream", FORMS)
+def test_fp32_parameters(pre, post, gate, alpha, with_stream):
+    for dtype in (BF16, FP16):
+        d, p = make((2, 11, 136), dtype, pre, post, gate, param_dtype=FP32, seed=3, device="cuda", bias=False)
+        check(d, p, alpha=alpha, with_stream=with_stream)
+
+
+@pytest.mark.parametrize("shape", [(1, 3000, 64), (40, 100, 96), (700, 2, 40), (1, 1200, 1024)])
+@pytest.mark.parametrize("gate", [None, "sequence"])
+def test_many_rows(shape, gate):
+    d, p = make(shape, BF16, "layer", "rms", gate, param_dtype=FP32, seed=4, device="cuda")
+    check(d, p)
+
+
+def test_no_parameters_at_all():
+    d, p = make((2, 5, 72), BF16, "rms", "layer", None, seed=5, device="cuda")
+    check(d, dict(pre="rms", post="layer"))
+
+
+def test_strides():
+    d, p = make((4, 6, 96), BF16, "rms", "rms", "sequence", seed=6, device="cuda")
+    want = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+    back = block_norm.residual_norm_backward(d["dh"], d["dy"], want[2])
+    wide = {}
+    for k, off in (("x", 3), ("block", 8), ("dh", 1), ("dy", 16)):     # rows off their boundaries, and transposed
+        t = torch.zeros(4, 6, 130, dtype=BF16, device="cuda")
+        t[..., off:off + 96] = d[k]
+        wide[k] = t[..., off:off + 96]
+    turned = {k: d[k].transpose(0, 2).contiguous().transpose(0, 2) for k in d}
+    q = dict(p, gate=torch.stack([p["gate"], p["gate"]], 1)[:, 0], pre_weight=torch.stack([p["pre_weight"]] * 2, 1)[:, 0])
+    for e in (wide, turned):
+        got = block_norm.residual_norm_forward(e["x"], e["block"], **q)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        grads = block_norm.residual_norm_backward(e["dh"], e["dy"], got[2])
+        assert all(torch.equal(grads[k], back[k]) for k in back if back[k] is not None)
+
+
+def test_parameters_off_their_boundaries():
+    d, p = make((2, 3, 64), BF16, "layer", "layer", "channel", seed=7, device="cuda")
+    q = {k: torch.cat([v[:1], v])[1:] if isinstance(v, torch.Tensor) else v for k, v in p.items()}
+    a, b = block_norm.residual_norm_forward(d["x"], d["block"], **p), block_norm.residual_norm_forward(d["x"], d["block"], **q)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    check(d, q)
+
+
+def test_non_finite_rows_stay_by_themselves():
+    d, p = make((1, 6, 64), BF16, "rms", "rms", None, seed=8, device="cuda")
+    d["x"][0, 2, 5], d["block"][0, 4, 7] = math.inf, math.nan
+    h, y, saved = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+    rows = [0, 1, 3, 5]
+    assert h[0, rows].isfinite().all() and h[0, 4].isnan().all() and not h[0, 2].isfinite().all()
+    got = block_norm.residual_norm_backward(d["dh"], d["dy"], saved)
+    for k in ("x", "block"):
+        assert got[k][0, rows].isfinite().all() and got[k][0, 2].isnan().any()
+    assert got["pre_weight"].isnan().any()
+
+
+def test_constant_rows():
+    """A row without variance: 1 / sqrt(eps) times nothing."""
+    x, b = torch.full((3, 40), 2.0, dtype=BF16, device="cuda"), torch.full((3, 40), -0.5, dtype=BF16, device="cuda")
+    h, y, saved = block_norm.residual_norm_forward(x, b, pre="layer", post="layer", eps=1e-6)
+    assert not h.any() and torch.equal(y, x)
+    got = block_norm.residual_norm_backward(torch.ones_like(x), None, saved)
+    assert got["x"].isfinite().all() and got["block"].isfinite().all()
+
+
+def test_empty():
+    for shape in ((0, 64), (2, 0, 32), (3, 0)):
+        x = torch.empty(shape, dtype=BF16, device="cuda")
+        w = torch.ones(shape[-1], dtype=BF16, device="cuda")
+        h, y, saved = block_norm.residual_norm_forward(x, x, pre="rms", pre_weight=w)
+        got = block_norm.residual_norm_backward(x, x, saved)
+        assert h.shape == y.shape == got["x"].shape == shape and not got["pre_weight"].any()
+
+
+def test_same_bits_twice():
+    d, p = make((8, 300, 520), BF16, "layer", "layer", "sequence", seed=9, device="cuda")
+    _, _, saved = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+    a, b = (block_norm.residual_norm_backward(d["dh"], d["dy"], saved) for _ in range(2))
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+def test_only_what_is_asked_for():
+    d, p = make((2, 50, 64), BF16, "layer", "layer", "channel", seed=10, device="cuda")
+    _, _, saved = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+    full = block_norm.residual_norm_backward(d["dh"], d["dy"], saved)
+    for needs in ((True, False, False, False, False), (False, False, False, False, True), (False,) * 5, (False, True, False, True, False)):
+        got = block_norm.residual_norm_backward(d["dh"], d["dy"], saved, needs)
+        for n, k in zip(needs, block_norm.PARAMS):
+            assert (got[k] is not None) == n and (not n or torch.equal(got[k], full[k]))
+        assert torch.equal(got["x"], full["x"]) and torch.equal(got["block"], full["block"])
+
+
+def test_graph_replay():
+    d, p = make((2, 64, 256), BF16, "rms", "rms", "sequence", seed=11, device="cuda")
+
+    def step():
+        h, y, saved = block_norm.residual_norm_forward(d["x"], d["block"], checkpoint_output=True, **p)
+        dw, _ = act8.weight_grad(d["dy"], saved.held_h)
+        got = block_norm.residual_norm_backward(d["dh"], d["dy"], saved)
+        return [h, y, dw] + [v for v in got.values() if v is not None]
+
+    step()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    d2, _ = make((2, 64, 256), BF16, "rms", "rms", "sequence", seed=12, device="cuda")
+    for k in d:
+        d[k].copy_(d2[k])
+    graphs[0].replay()
+    want = step()
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    for got in outs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
