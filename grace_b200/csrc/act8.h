@@ -28,9 +28,10 @@ cudaError_t launch_act8_backward(const void* grad, long long grad_stride, void* 
 
 // dW [outs, ins] = dY^T x~ and (bias not null) db [outs] = column sums of dY, both of grad's type or, with out_f32, fp32.
 // grad: 16-bit, rows `grad_stride` elements apart, base and rows on 16-byte boundaries (launch_act8_repitch makes
-// such a copy: [rows, ceil(cols / 8) * 8]).
+// such a copy: [rows, ceil(cols / 8) * 8]).  work: act8_wgrad_work_bytes of scratch, often none.
 cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held, long long tokens, int outs, int ins, int dtype,
-                              int out_f32, void* out, void* bias, int sms, cudaStream_t stream);
+                              int out_f32, void* out, void* bias, void* work, int sms, cudaStream_t stream);
+size_t act8_wgrad_work_bytes(long long tokens, int outs, int ins, int out_f32, int sms);
 // The current device's status block of the bounded waits (16 words, the first 0 if none ran out), cleared if one did.
 cudaError_t act8_wgrad_status(unsigned* words);
 cudaError_t launch_act8_repitch(const void* src, long long stride, void* dst, long long rows, int cols, cudaStream_t stream);

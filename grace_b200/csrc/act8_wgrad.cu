@@ -2,25 +2,34 @@
 //   dW[n, k] = sum_m dY[m, n] x~[m, k]      db[n] = sum_m dY[m, n]
 // without ever writing x~ to memory: its tiles are decoded on the way into the tensor core.
 //
-// The kernel computes dW^T tiles of 128 input features by 256 output features, D[k, n] += A[k, m] B[m, n], over steps of
-// 64 tokens.  Both operands have the tokens as their contracted axis and lie in memory with the OTHER axis
-// contiguous, which the tensor core takes as it is (MN-major operands, 128-byte rows of 64 elements in the 128-byte
-// swizzle), so nothing is transposed:
+// A pair of CTAs computes a dW^T tile of 256 input features by 256 output features, D[k, n] += A[k, m] B[m, n], in steps of
+// 64 tokens (tcgen05.mma with cta_group::2: each CTA holds 128 rows of A, 128 columns of B, and the accumulator rows
+// that belong to its part of A).  Both operands have the tokens as their contracted axis and lie in memory with the
+// OTHER axis contiguous, which the tensor core takes as it is (MN-major operands, 128-byte rows of 64 elements in the
+// 128-byte swizzle), so nothing is transposed:
 //   B = dY     TMA boxes of 64 tokens x 64 output features land in the operand layout
-//   A = x~     TMA brings the codes (64 tokens x 128 bytes); eight warps decode them and store the operand tile
-// The checkpoint is the operand with the SHORT side (128 against 256) because its elements cost issue slots: 2.5
-// instructions each, 64 * 128 * 2.5 / 128 lanes = 160 of the 512 cycles that the tensor core needs for the step.  For
-// bf16 a code's sign bit and seven others are placed under a significand whose exponent already holds the scale, so
-// decoding and scaling are one subtraction of two bf16 pairs; the result is exact.
+//   A = x~     TMA brings the codes (64 tokens x 128 bytes), the decoders fetch their scale bytes; three groups of four warps take the steps in turn, decode them
+//              and store the operand tile
+// For bf16 a code's low seven bits are placed under an exponent that already holds the scale, its sign bit under
+// another, so decoding and scaling are one subtraction of two bf16 pairs; the result is exact.  (fp16: see decode8.)
 //
-// Roles: warp 0 loads (TMA; the four scale bytes a token by cp.async), warp 1 issues the MMAs, warps 2 - 3 add up the
-// bias gradient (each CTA of a row of tiles takes its share of the 256 columns), warps 4 - 11 decode and, at the end,
-// write the result from TMEM.  Few output tiles would leave SMs idle: then the tokens are split over a cluster of up
-// to 8 CTAs, which add their partial tiles in rank order through distributed shared memory (no atomics: the same
-// bits on every run).  Sums are fp32 throughout, rounded once to the output's type.
+// Roles: warp 0 loads dY, warp 2 the codes (both by TMA), warp 1 of the pair's first CTA issues the MMAs, warp 3 adds up
+// the bias gradient (the CTAs of a row of tiles share its columns), warps 4 - 15 decode, warps 16 - 19 write results
+// from one of two accumulators while the MMAs fill the other.  dY waits in seven stages, the codes in five, the decoded
+// operand in four: a step is on its way for about seven steps' time (load 950 cycles, decode 1100, MMA 512, barriers
+// between), but only its dY is needed all that long.
+//
+// A pair takes whole tiles, one from each full wave of them, so that neighbouring pairs read the same rows at the same
+// time.  The tiles of the last, partial wave are laid end to end and cut into equal runs of steps, one for each pair
+// (where that saves more than it costs: see make_plan); a run that is not a whole tile leaves fp32 partial sums
+// in a workspace, and a second kernel adds a tile's runs in order (no atomics: the same bits on every run).
+//
+// The tensor core truncates where it adds to an fp32 accumulator, which over thousands of tokens adds up to a bias
+// (2.3e-6 of the result after 4096 tokens).  Where the result itself is fp32 the accumulator is therefore emptied every
+// 1536 tokens into the output, rounding to nearest (0.2e-6).  Sums are fp32 throughout, rounded once to the output's type.
 //
 // Every wait is bounded; when one runs out the status block says which and the outputs are NaN.
-#include <cooperative_groups.h>
+#include <type_traits>
 
 #include "act8.cuh"
 #include "act8.h"
@@ -30,62 +39,112 @@
 namespace grace {
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int kThreads = 384;
-constexpr int kTileK = 128;            // input features of a tile: MMA M
-constexpr int kTileN = 256;            // output features of a tile: MMA N
+constexpr int kThreads = 640;
+constexpr int kTileK = 128;            // input features of a CTA's half of the tile
+constexpr int kTileN = 256;            // output features of a tile
+constexpr int kHalfN = 128;            // of them in one CTA's shared memory
 constexpr int kStep = 64;              // tokens of a step
 constexpr int kBoxBytes = kStep * 128; // 64 tokens x 64 features of 16 bits
-constexpr int kBBytes = 4 * kBoxBytes;
-constexpr int kCodeBytes = kStep * kTileK;
-constexpr int kABytes = 2 * kBoxBytes;
-constexpr int kStages = 4, kAStages = 3;
-constexpr int kDecodeWarp0 = 4, kDecodeWarps = 8;
+constexpr int kBStages = 7, kCodeStages = 5, kAStages = 4;
+constexpr int kDecodeWarp0 = 4, kGroups = 3, kGroupWarps = 4, kEpilogueWarp0 = kDecodeWarp0 + kGroups * kGroupWarps;
+constexpr int kMinSavedSteps = 24;
+constexpr int kChunkSteps = 24;        // steps between two emptyings of the accumulator for an fp32 result
 constexpr unsigned long long kTimeoutNs = 2000000000ull;
-constexpr unsigned kTmemCols = 256;
+constexpr unsigned kTmemCols = 512;
 
 struct __align__(1024) WgradSmem {
-  unsigned char b[kStages][kBBytes];        // reused at the end: [256][128] fp32 partial tile for the cluster's other CTAs
-  unsigned char a[kAStages][kABytes];
-  unsigned char codes[kStages][kCodeBytes];
-  unsigned scales[kStages][kStep];          // four scale bytes of a token: the tile's 128 features
-  float bias[kTileN];
-  unsigned long long full[kStages], empty[kStages], a_full[kAStages], a_empty[kAStages], done;
+  unsigned char b[kBStages][2 * kBoxBytes];
+  unsigned char a[kAStages][2 * kBoxBytes];
+  unsigned char codes[kCodeStages][kStep * kTileK];
+  unsigned long long b_full[kBStages];                             // dY has landed
+  unsigned long long b_used[kBStages], b_summed[kBStages];         // the MMAs, the bias warp are done with it
+  unsigned long long c_full[kCodeStages], c_empty[kCodeStages];    // the codes have landed, are in registers
+  unsigned long long ready[kAStages];                              // first CTA of the pair: both CTAs' operands are in place
+  unsigned long long acc_full[2], acc_empty[2];                    // (acc_empty: first CTA)
+  unsigned long long done;
   unsigned tmem_base;
-  unsigned ok;
+  unsigned failed;                                                 // a wait of this CTA ran out
+  int rest[2][4];                                                  // this pair's pieces of the last wave (a Piece each; st1 = 0: none)
 };
-static_assert(kStages * kBBytes >= kTileN * kTileK * 4, "the partial tile reuses the operand ring");
+static_assert(sizeof(WgradSmem) + 1024 <= 227 * 1024, "shared memory");
+static_assert(kAStages <= kCodeStages && kAStages <= kBStages, "see the decoders' waits");
+
+constexpr int kPartFloats = 2 * kTileN * kTileK;    // partial sums of a tile: [2 CTAs][256][128]
+constexpr int kSlotFloats = kPartFloats + 2 * kHalfN;   // and of its CTAs' bias columns
 
 struct WgradArgs {
   const unsigned char* scales;
   int spitch;
   long long tokens;
   int outs, ins;        // N, K
+  int tiles_k;          // pair tiles along the input features
+  int pairs;            // of CTAs
+  int whole;            // whole tiles a pair takes: tiles pair, pair + pairs, ...
+  int rest, rest_pairs; // tiles after them, and the pairs that share their steps equally
   int steps;            // of 64 tokens, over all tokens
-  int bias_cols;        // columns of the 256 that a CTA adds up (a power of two), 0: no bias gradient
+  int chunk;            // steps between two emptyings of the accumulator
+  int bias_cols;        // columns of its 128 that a CTA adds up (a power of two, 8 to 128), 0: no bias gradient
   void* out;
   void* bias;
+  float* work;          // [2 * rest_pairs][kSlotFloats]: runs that are not whole tiles
 };
+
+// A piece of work of a pair: steps [st0, st1) of a tile.
+struct Piece {
+  int tile, st0, st1;
+  int slot;             // of the workspace; -1: a whole tile, straight to the output
+};
+// A pair's run of the last wave is no longer than a tile, so it touches two tiles at most: j = 0 or 1.
+__device__ __forceinline__ Piece rest_piece(const WgradArgs& a, int pair, int j) {
+  Piece p{0, 0, 0, -1};
+  if (pair >= a.rest_pairs) return p;
+  const long long total = (long long)a.rest * a.steps;
+  const long long lo = pair * total / a.rest_pairs, hi = (pair + 1) * total / a.rest_pairs;
+  const int r = (int)(lo / a.steps) + j;
+  p.st0 = j ? 0 : (int)(lo - (long long)r * a.steps);
+  p.st1 = (int)max(0ll, min((long long)a.steps, hi - (long long)r * a.steps));
+  p.tile = a.whole * a.pairs + r;
+  p.slot = p.st0 == 0 && p.st1 == a.steps ? -1 : pair * 2 + j;
+  return p;
+}
+__device__ __forceinline__ bool piece_at(const WgradArgs& a, const WgradSmem& sm, int pair, int i, Piece& p) {
+  if (i < a.whole) {
+    p = {pair + i * a.pairs, 0, a.steps, -1};
+    return true;
+  }
+  i -= a.whole;   // (whole warps call this: what it reads is made uniform)
+  if (i > 1 || __shfl_sync(0xffffffffu, sm.rest[i][2], 0) == 0) return false;
+  p = {__shfl_sync(0xffffffffu, sm.rest[i][0], 0), __shfl_sync(0xffffffffu, sm.rest[i][1], 0), __shfl_sync(0xffffffffu, sm.rest[i][2], 0),
+       __shfl_sync(0xffffffffu, sm.rest[i][3], 0)};
+  return true;
+}
 
 // The status block of the bounded waits (common.cuh), one for each device, sticky until act8_wgrad_status clears it.  A
 // symbol and not an allocation, so that the first call may be made while a graph is being captured.
 __device__ unsigned wgrad_status[16];
 
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accum) {
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accum) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"((unsigned)accum) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
+// Arrives at the barrier of the same name in both CTAs of the pair when the MMAs issued so far are done.
+__device__ __forceinline__ void umma_commit_pair(void* bar, unsigned ctas) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+               "h"((unsigned short)ctas)
+               : "memory");
 }
-__device__ __forceinline__ void cp_async_arrive(void* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// Arrives at the barrier of the same name in another CTA (`cta`: rank in the cluster).  What the barrier announces is
+// this CTA's own operand tile, which its threads have handed to the async proxy by a fence of their own; nothing is
+// read from here through the generic proxy.  The arrival therefore needs no cluster-wide release, which (with the
+// acquire on the other side) took 1300 cycles each, more than two steps of the tensor core.
+__device__ __forceinline__ void mbar_arrive_at(void* bar, unsigned cta) {
+  uint32_t addr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(bar)), "r"(cta));
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-
 // Eight codes as a 16-byte operand chunk.
 __device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __nv_bfloat16) {
   // exponent field s + 7: 2^(s - 127) * 128 * (1 + m / 128) = (128 + m) steps
@@ -101,239 +160,421 @@ __device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __nv_bfloat16) {
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
-__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __half) {   // (fp16's exponent range is too short for that)
-  float v[8];
-  act8_decode(c, s, v);
-  Chunk8<__half> h;
-  h.set(v);
-  return h.w;
+// fp16 has the significand to take a code whole (1024 + byte), but not the exponents: the scale goes on in two factors,
+// 2^-6 and 2^(s - 121), so that its range reaches from 2^-30 to 2^9, that of groups of fp16 values; the first product is
+// exact and the second rounds once, into the subnormals.  A group beyond fp16's range reads as NaN.
+__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __half) {
+  // 2^(s - 121): normal, subnormal, or below 2^-24, where every value rounds to zero
+  const unsigned f = s > 136u ? 0x7e00u : (s >= 107u ? (s - 106u) << 10 : (s >= 97u ? 1u << (s - 97u) : 0u));
+  const __half2 scale = __half2half2(__ushort_as_half((unsigned short)f));
+  const __half2 sixth = __half2half2(__ushort_as_half(0x2400)), offset = __half2half2(__ushort_as_half(0xcc80));   // 2^-6, -18 = -1152 * 2^-6
+  c.x ^= 0x80808080u;
+  c.y ^= 0x80808080u;
+  unsigned r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned v = __byte_perm(j < 2 ? c.x : c.y, 0x64006400u, (j & 1) ? 0x5352 : 0x5150);   // 1024 + code + 128
+    const __half2 d = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&v), sixth, offset), scale);
+    r[j] = *reinterpret_cast<const unsigned*>(&d);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// fp32 accumulator, both operands T and MN-major, M = 256; N is added at run time
 template <class T> constexpr uint32_t instruction_desc() {
-  constexpr uint32_t f = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
-  return (1u << 4) | (f << 7) | (f << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(kTileK >> 4) << 24);   // N is added at run time
+  constexpr uint32_t f = __is_same(T, __nv_bfloat16) ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(2 * kTileK >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// A tile as one of the pair's CTAs sees it.
+struct Tile {
+  int k0;        // its first input feature
+  int n0;        // the tile's first output feature
+  int boxes;     // 64-feature boxes of B in each of the two CTAs
+  int share;     // which share of the bias columns this row of tiles' CTA adds up
+};
+__device__ __forceinline__ Tile tile_at(const WgradArgs& a, int tile, int half) {
+  const int tk = tile % a.tiles_k, tn = tile / a.tiles_k;
+  return {(tk * 2 + half) * kTileK, tn * kTileN, a.outs - tn * kTileN > 2 * 64 ? 2 : 1, tk};
+}
+
+// One lane of a converged warp.  The roles that issue TMA loads and MMAs run as whole warps and elect a lane only around
+// the instruction: descriptors and coordinates then stay in uniform registers, where the instruction wants them.  As a
+// single diverged lane, issuing a step took longer than the tensor core took to compute it.
+__device__ __forceinline__ bool elect_one() {
+  unsigned one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+// A ring position and the parity of its use.
+template <int N> struct Ring {
+  unsigned slot = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) { slot = 0; parity ^= 1; }
+  }
+};
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <class T, class O>
-__global__ void __launch_bounds__(kThreads, 1) wgrad_kernel(const __grid_constant__ CUtensorMap map_dy,
-                                                            const __grid_constant__ CUtensorMap map_codes, const WgradArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    wgrad_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_codes, const WgradArgs a) {
   extern __shared__ unsigned char raw[];
   WgradSmem& sm = *reinterpret_cast<WgradSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const Status status{wgrad_status};
-  const int splits = gridDim.z, split = blockIdx.z;      // the cluster: (1, 1, splits)
-  const int k0 = blockIdx.x * kTileK, n0 = blockIdx.y * kTileN;
-  const int step0 = (int)((long long)a.steps * split / splits);
-  const int nsteps = (int)((long long)a.steps * (split + 1) / splits) - step0;
-  const int boxes = min(4, (a.outs - n0 + 63) / 64);     // 64-feature blocks of this tile that exist
+  const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
   const bool has_bias = a.bias_cols != 0;
+  Piece p;
 
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full[s], 1 + 32);
-      mbar_init(&sm.empty[s], 1 + kDecodeWarps + (has_bias ? 2 : 0));
-    }
-    for (int s = 0; s < kAStages; ++s) { mbar_init(&sm.a_full[s], kDecodeWarps); mbar_init(&sm.a_empty[s], 1); }
+    for (int s = 0; s < kBStages; ++s) { mbar_init(&sm.b_full[s], 1); mbar_init(&sm.b_used[s], 1); mbar_init(&sm.b_summed[s], 1); }
+    for (int s = 0; s < kCodeStages; ++s) { mbar_init(&sm.c_full[s], 1); mbar_init(&sm.c_empty[s], kGroupWarps); }
+    for (int s = 0; s < kAStages; ++s) mbar_init(&sm.ready[s], 2 * kGroupWarps);
+    for (int b = 0; b < 2; ++b) { mbar_init(&sm.acc_full[b], 1); mbar_init(&sm.acc_empty[b], 2 * 4); }
     mbar_init(&sm.done, 1);
-    sm.ok = 1;
+    sm.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 2 && lane < 2) {
+    p = rest_piece(a, pair, lane);
+    sm.rest[lane][0] = p.tile;
+    sm.rest[lane][1] = p.st0;
+    sm.rest[lane][2] = p.st1;
+    sm.rest[lane][3] = p.slot;
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
 
   if (warp == 0) {
-    // ---- loads ----
+    // ---- dY ----
     bool ok = true;
-    int st = 0;
-    for (; st < nsteps; ++st) {
-      const int slot = st % kStages;
-      if (st >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[slot], (st / kStages - 1) & 1, kTimeoutNs, status, 100 + slot));
-      if (!ok) break;
-      const int m = (step0 + st) * kStep;
-      if (lane == 0) {
-        mbar_expect_tx(&sm.full[slot], boxes * kBoxBytes + kCodeBytes);
-        for (int j = 0; j < boxes; ++j) tma_load_2d(&sm.b[slot][j * kBoxBytes], &map_dy, n0 + j * 64, m, &sm.full[slot]);
-        tma_load_2d(&sm.codes[slot][0], &map_codes, k0, m, &sm.full[slot]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const long long row = m + lane + 32 * i;
-        const bool in = row < a.tokens;
-        cp_async4(&sm.scales[slot][lane + 32 * i], a.scales + (in ? row : 0) * a.spitch + (k0 >> 5), in);   // past the end: zeros
-      }
-      cp_async_arrive(&sm.full[slot]);
-    }
-    if (!ok)   // a consumer gave up: the loads that were issued must land before the shared memory is let go
-      for (int s = st > kStages ? st - kStages : 0; s < st; ++s) mbar_wait(&sm.full[s % kStages], (s / kStages) & 1, kTimeoutNs, status, 400);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 1) {
-    // ---- MMAs ----
-    if (lane == 0) {
-      const uint32_t idesc = instruction_desc<T>() | ((uint32_t)(boxes * 8) << 17);
-      for (int st = 0; st < nsteps; ++st) {
-        const int slot = st % kStages, as = st % kAStages;
-        if (!mbar_wait(&sm.full[slot], (st / kStages) & 1, kTimeoutNs, status, 200 + slot) ||
-            !mbar_wait(&sm.a_full[as], (st / kAStages) & 1, kTimeoutNs, status, 300 + as)) {
-          sm.ok = 0;
-          break;
+    unsigned it = 0;
+    Ring<kBStages> r;
+    for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+      const Tile t = tile_at(a, p.tile, half);
+      for (int st = p.st0; st < p.st1; ++st, ++it, r.next()) {
+        if (it >= kBStages) {
+          ok = mbar_wait(&sm.b_used[r.slot], r.parity ^ 1, kTimeoutNs, status, 100 + r.slot) &&
+               (!has_bias || mbar_wait(&sm.b_summed[r.slot], r.parity ^ 1, kTimeoutNs, status, 150 + r.slot));
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
         }
-        tc_fence_after();
-        const uint32_t a_addr = smem_u32(sm.a[as]), b_addr = smem_u32(sm.b[slot]);
-#pragma unroll
-        for (int kk = 0; kk < kStep / 16; ++kk)   // 16 tokens: two groups of eight 128-byte rows; the next 64 features one box further
-          umma_f16(tmem, smem_desc(a_addr + kk * 2048, kBoxBytes, 1024, 2), smem_desc(b_addr + kk * 2048, kBoxBytes, 1024, 2), idesc,
-                   st > 0 || kk > 0);
-        umma_commit(&sm.a_empty[as]);
-        umma_commit(&sm.empty[slot]);
-      }
-      umma_commit(&sm.done);
-    }
-  } else if (warp < kDecodeWarp0) {
-    // ---- bias gradient: this CTA's share of the tile's columns, two a thread, rows dealt to `groups` threads ----
-    if (has_bias) {
-      const int t = tid - 64, pairs = a.bias_cols >> 1;
-      const int groups = min(32, 64 / min(64, pairs)), own = t / groups, sub = t % groups;
-      const int c0 = blockIdx.x * a.bias_cols;             // first column; CTAs past the 256th column have none
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      bool ok = true;
-      for (int st = 0; st < nsteps; ++st) {
-        const int slot = st % kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[slot], (st / kStages) & 1, kTimeoutNs, status, 500 + slot));
-        if (!ok) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int pair = own + 64 * h, col = c0 + pair * 2;
-          if (pair < pairs && col < boxes * 64) {
-            const unsigned char* p = &sm.b[slot][(col >> 6) * kBoxBytes + (col & 7) * 2];
-            for (int m = sub; m < kStep; m += groups) {
-              const unsigned v = *reinterpret_cast<const unsigned*>(p + m * 128 + ((((col >> 3) & 7) ^ (m & 7)) << 4));
-              const unsigned short lo = (unsigned short)v, hi = (unsigned short)(v >> 16);
-              acc[2 * h] += to_f32<T>(*reinterpret_cast<const T*>(&lo));
-              acc[2 * h + 1] += to_f32<T>(*reinterpret_cast<const T*>(&hi));
-            }
-          }
+        if (elect_one()) {
+          mbar_expect_tx(&sm.b_full[r.slot], t.boxes * kBoxBytes);
+          for (int j = 0; j < t.boxes; ++j)
+            tma_load_2d(sm.b[r.slot] + j * kBoxBytes, &map_dy, t.n0 + (half * t.boxes + j) * 64, st * kStep, &sm.b_full[r.slot]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[slot]);
       }
+    }
+    // At the end the last arrivals of the pair's MMAs must have landed here (see the MMAs); where a consumer gave up, the
+    // loads that were issued, before the shared memory is let go.
+    bool landed = true;
+    for (unsigned s = it > kBStages ? it - kBStages : 0; s < it; ++s)
+      landed = mbar_wait(ok ? &sm.b_used[s % kBStages] : &sm.b_full[s % kBStages], (s / kBStages) & 1, 2 * kTimeoutNs, status, 400) && landed;
+    landed = mbar_wait(&sm.done, 0, 2 * kTimeoutNs, status, 800) && landed;
+    if (!ok || !landed) sm.failed = 1;
+  } else if (warp == 1) {
+    // ---- MMAs, by one thread of the pair ----
+    if (half == 0) {
+      // (addresses in a descriptor are in units of 16 bytes, in its low bits)
+      const uint64_t a_desc = smem_desc(smem_u32(sm.a), kBoxBytes, 1024, 2), b_desc = smem_desc(smem_u32(sm.b), kBoxBytes, 1024, 2);
+      unsigned item = 0;
+      Ring<kAStages> ra;
+      Ring<kBStages> rb;
+      bool ok = true;
+      for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+        const Tile t = tile_at(a, p.tile, 0);
+        const uint32_t idesc = instruction_desc<T>() | ((uint32_t)(t.boxes * 128 >> 3) << 17);
+        for (int st = p.st0; ok && st < p.st1; ++item) {
+          const unsigned buf = item & 1;
+          if (item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[buf], ((item >> 1) - 1) & 1, kTimeoutNs, status, 300 + buf));
+          if (!ok) break;
+          tc_fence_after();
+          const int end = min(st + a.chunk, p.st1);
+          for (bool fresh = true; st < end; ++st, ra.next(), rb.next(), fresh = false) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sm.ready[ra.slot], ra.parity, kTimeoutNs, status, 200 + ra.slot));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t ad = a_desc + ra.slot * (2 * kBoxBytes >> 4), bd = b_desc + rb.slot * (2 * kBoxBytes >> 4);
+            if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        for (int o = groups >> 1; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-      if (sub == 0) {
+              for (int kk = 0; kk < kStep / 16; ++kk)   // 16 tokens: two groups of eight 128-byte rows; the next 64 features one box further
+                umma_f16_pair(tmem + buf * kTileN, ad + kk * (2048 >> 4), bd + kk * (2048 >> 4), idesc, kk > 0 || !fresh);
+              umma_commit_pair(&sm.b_used[rb.slot], 3u);
+            }
+            __syncwarp();
+          }
+          if (ok && elect_one()) umma_commit_pair(&sm.acc_full[buf], 3u);
+          __syncwarp();
+        }
+      }
+      if (elect_one()) umma_commit_pair(&sm.done, 3u);
+      __syncwarp();
+      // The other CTA's last arrivals here are on their way without being waited for by anything else, and a barrier
+      // between the CTAs does not order them: this CTA has to be there when they land.
+      for (unsigned n = item > 2 ? item - 2 : 0; ok && n < item; ++n) ok = mbar_wait(&sm.acc_empty[n & 1], (n >> 1) & 1, 2 * kTimeoutNs, status, 350);
+      if (!ok) sm.failed = 1;
+    }
+  } else if (warp == 2) {
+    // ---- codes ----
+    bool ok = true;
+    unsigned it = 0;
+    Ring<kCodeStages> r;
+    for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+      const Tile t = tile_at(a, p.tile, half);
+      for (int st = p.st0; st < p.st1; ++st, ++it, r.next()) {
+        if (it >= kCodeStages) ok = __all_sync(0xffffffffu, mbar_wait(&sm.c_empty[r.slot], r.parity ^ 1, kTimeoutNs, status, 500 + r.slot));
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&sm.c_full[r.slot], kStep * kTileK);
+          tma_load_2d(sm.codes[r.slot], &map_codes, t.k0, st * kStep, &sm.c_full[r.slot]);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok)
+      for (unsigned s = it > kCodeStages ? it - kCodeStages : 0; s < it; ++s) mbar_wait(&sm.c_full[s % kCodeStages], (s / kCodeStages) & 1, kTimeoutNs, status, 450);
+  } else if (warp == 3) {
+    // ---- bias gradient: this CTA's share of its columns, eight a thread, the step's tokens dealt to the threads ----
+    if (has_bias) {
+      const int chunks = a.bias_cols >> 3;                     // 1 .. 16 chunks of eight columns
+      const int sub = lane / chunks, rows = 32 / chunks;       // a thread takes the tokens sub, sub + rows, ...
+      unsigned it = 0;
+      bool ok = true;
+      for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+        const Tile t = tile_at(a, p.tile, half);
+        const int col = t.share * a.bias_cols + (lane % chunks) * 8;      // (tiles past the last share have none)
+        const bool mine = col < t.boxes * 64;
+        float acc[8] = {};
+        for (int st = p.st0; st < p.st1; ++st, ++it) {
+          const unsigned slot = it % kBStages;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[slot], (it / kBStages) & 1, kTimeoutNs, status, 550 + slot));
+          if (!ok) break;
+          if (mine) {
+            const unsigned char* q = sm.b[slot] + (col >> 6) * kBoxBytes;
+            const int c = (col >> 3) & 7;
+#pragma unroll 4
+            for (int m = sub; m < kStep; m += rows) {
+              Chunk8<T> x;
+              x.w = *reinterpret_cast<const uint4*>(q + m * 128 + ((c ^ (m & 7)) << 4));
+              float v[8];
+              x.get(v);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int pair = own + 64 * h, col = c0 + pair * 2;
-          if (pair < pairs && col < kTileN) {
-            sm.bias[col] = acc[2 * h];
-            sm.bias[col + 1] = acc[2 * h + 1];
+              for (int j = 0; j < 8; ++j) acc[j] += v[j];
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.b_summed[slot]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          for (int o = chunks; o < 32; o <<= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+        if (lane < chunks && mine) {
+          const int n = t.n0 + half * t.boxes * 64 + col;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float x = ok ? acc[j] : __uint_as_float(0x7fffffffu);
+            if (p.slot >= 0) a.work[(size_t)p.slot * kSlotFloats + kPartFloats + half * kHalfN + col + j] = x;
+            else if (n + j < a.outs) static_cast<O*>(a.bias)[n + j] = from_f32<O>(x);
           }
         }
       }
     }
-  } else {
-    // ---- decode: a thread takes eight codes (a 16-byte operand chunk) of four tokens a step ----
-    const int t = tid - kDecodeWarp0 * 32, chunk = t & 15, row0 = t >> 4;
-    for (int st = 0; st < nsteps; ++st) {
-      const int slot = st % kStages, as = st % kAStages;
-      bool ok = mbar_wait(&sm.full[slot], (st / kStages) & 1, kTimeoutNs, status, 600 + slot);
-      if (ok && st >= kAStages) ok = mbar_wait(&sm.a_empty[as], (st / kAStages - 1) & 1, kTimeoutNs, status, 700 + as);
-      if (!__all_sync(0xffffffffu, ok)) break;
+  } else if (warp < kEpilogueWarp0) {
+    // ---- decode: a thread takes sixteen codes (two 16-byte operand chunks) of four tokens a step ----
+    const unsigned group = (warp - kDecodeWarp0) / kGroupWarps;
+    const int t = (tid - kDecodeWarp0 * 32) & (kGroupWarps * 32 - 1);
+    const int c = t & 7, row0 = t >> 3, swap = c >> 2;      // eight threads of a row hit eight different 16-byte banks each time
+    const int j0 = (c & 3) * 2 + swap, j1 = (c & 3) * 2 + 1 - swap;
+    unsigned it = 0, sc[4];
+    // the scale bytes of a step's four tokens, asked for one of the group's steps (three in all) ahead
+    auto scales_of = [&](const Tile& tile, int st) {
+      const int at = (tile.k0 >> 5) + (c >> 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int m = row0 + 16 * i;
-        const uint2 c = *reinterpret_cast<const uint2*>(&sm.codes[slot][m * kTileK + chunk * 8]);
-        const unsigned s = (sm.scales[slot][m] >> ((chunk >> 2) * 8)) & 0xffu;
-        *reinterpret_cast<uint4*>(&sm.a[as][(chunk >> 3) * kBoxBytes + m * 128 + (((chunk & 7) ^ (m & 7)) << 4)]) = decode8(c, s, T{});
+      for (int j = 0; j < 4; ++j) {
+        const long long row = (long long)st * kStep + row0 + 16 * j;
+        sc[j] = row < a.tokens && at < a.spitch ? __ldg(a.scales + row * a.spitch + at) : 0u;    // past the end: zeros
       }
-      fence_async_all();   // the tensor core reads the tile through the async proxy
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.empty[slot]);
-        mbar_arrive(&sm.a_full[as]);
+    };
+    bool ok = true;
+    for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+      const Tile tile = tile_at(a, p.tile, half);
+      int st = p.st0 + (int)((group + kGroups - it % kGroups) % kGroups);     // the group's first step of this piece
+      const unsigned it0 = it - p.st0;
+      if (st < p.st1) scales_of(tile, st);
+      for (; st < p.st1; st += kGroups) {
+        const unsigned n = it0 + st, cs = n % kCodeStages, as = n % kAStages;      // n: steps before this one
+        // The operand slot is free when the MMAs of the step that had it are done.  This wait comes before the one for the
+        // codes, and not only for that: a parity tells a phase from its neighbours alone, loads may land out of order, and a
+        // group does not look at the other groups' steps.  That an MMA is done means that the codes of all steps before it
+        // have been decoded, so that the codes' barrier is in this step's phase or past it.
+        if (n >= kAStages) ok = mbar_wait(&sm.b_used[(n - kAStages) % kBStages], ((n - kAStages) / kBStages) & 1, kTimeoutNs, status, 620 + as);
+        if (ok) ok = mbar_wait(&sm.c_full[cs], (n / kCodeStages) & 1, kTimeoutNs, status, 600 + cs);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        uint4 q[4];
+        unsigned s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          q[j] = *reinterpret_cast<const uint4*>(&sm.codes[cs][(row0 + 16 * j) * kTileK + c * 16]);
+          s[j] = sc[j];
+        }
+        if (st + kGroups < p.st1) scales_of(tile, st + kGroups);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.c_empty[cs]);   // (the warp's codes are in registers)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int m = row0 + 16 * j;
+          unsigned char* const row = sm.a[as] + swap * kBoxBytes + m * 128;
+          const uint2 u = swap ? make_uint2(q[j].z, q[j].w) : make_uint2(q[j].x, q[j].y);
+          const uint2 v = swap ? make_uint2(q[j].x, q[j].y) : make_uint2(q[j].z, q[j].w);
+          *reinterpret_cast<uint4*>(row + ((j0 ^ (m & 7)) << 4)) = decode8(u, s[j], T{});
+          *reinterpret_cast<uint4*>(row + ((j1 ^ (m & 7)) << 4)) = decode8(v, s[j], T{});
+        }
+        fence_async_shared();   // the tensor core reads the tile through the async proxy
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[n % kBStages], (n / kBStages) & 1, kTimeoutNs, status, 640));   // the step's dY is here too
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_at(&sm.ready[as], 0);
+      }
+      it += p.st1 - p.st0;
+    }
+    if (!ok) sm.failed = 1;
+  } else {
+    // ---- results: TMEM lane = input feature, column = output feature ----
+    const int kl = (warp - kEpilogueWarp0) * 32 + lane;
+    unsigned item = 0;
+    bool ok = true;
+    for (int i = 0; piece_at(a, sm, pair, i, p); ++i) {
+      const Tile t = tile_at(a, p.tile, half);
+      const int k = t.k0 + kl, cols = t.boxes * 128;
+      for (int st = p.st0; st < p.st1; st += a.chunk, ++item) {
+        const unsigned buf = item & 1;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_full[buf], (item >> 1) & 1, 2 * kTimeoutNs, status, 700 + buf));
+        tc_fence_after();
+        const uint32_t base = tmem + buf * kTileN + ((uint32_t)((warp - kEpilogueWarp0) * 32) << 16);
+        // sums to q, q + stride, ... of `n` columns; an emptying after the first adds to what the one before it left
+        auto put = [&](auto* q, size_t stride, int n, int c) {
+          using Q = std::remove_pointer_t<decltype(q)>;
+          float old[16];
+          if (st > p.st0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) old[j] = j < n ? to_f32<Q>(q[j * stride]) : 0.f;
+          }
+          uint32_t v[16];
+          __syncwarp();
+          tmem_load16(base + c, v);
+          if (!ok) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0x7fffffffu;
+          }
+          if (st > p.st0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + old[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (j < n) q[j * stride] = from_f32<Q>(__uint_as_float(v[j]));
+        };
+        if (p.slot >= 0) {
+          float* const q = a.work + (size_t)p.slot * kSlotFloats + half * (kTileN * kTileK) + kl;
+          for (int c = 0; c < cols; c += 16) put(q + c * kTileK, kTileK, 16, c);
+        } else {
+          O* const q = static_cast<O*>(a.out) + (size_t)t.n0 * a.ins + k;
+          for (int c = 0; c < cols; c += 16) put(q + (size_t)c * a.ins, a.ins, k < a.ins ? min(16, a.outs - t.n0 - c) : 0, c);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_at(&sm.acc_empty[buf], 0);
       }
     }
   }
 
-  // ---- result: TMEM lane = input feature, column = output feature ----
+  // ---- the MMAs are done, in both CTAs: nobody's shared or tensor memory goes before ----
   __syncwarp();
-  const bool done = mbar_wait(&sm.done, 0, 2 * kTimeoutNs, status, 800);   // (also: no MMA reads the rings any more)
-  if (!done) sm.ok = 0;
-  __syncthreads();
-  tc_fence_after();
-  bool good = sm.ok && !status.failed();
-  const float nan = __uint_as_float(0x7fffffffu);
-  O* const out = static_cast<O*>(a.out);
-  if (warp >= kDecodeWarp0) {
-    const int quarter = warp & 3, half = (warp - kDecodeWarp0) >> 2;      // a warp reads its own quarter of the TMEM lanes
-    const int kl = quarter * 32 + lane, k = k0 + kl;
-    float* const part = reinterpret_cast<float*>(sm.b[0]);
-    for (int c = half * 128; c < half * 128 + 128 && c < boxes * 64; c += 32) {
-      uint32_t v[32];
-      asm volatile(
-          "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-          "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-          : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-            "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
-            "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-            "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-          : "r"(tmem + c + ((uint32_t)(quarter * 32) << 16)));
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (splits == 1) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (k < a.ins && n0 + c + j < a.outs)
-            out[(size_t)(n0 + c + j) * a.ins + k] = from_f32<O>(good ? __uint_as_float(v[j]) : nan);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) part[(c + j) * kTileK + kl] = __uint_as_float(v[j]);
-      }
-    }
-  }
-  if (splits == 1) {
-    if (has_bias) {
-      const int c = blockIdx.x * a.bias_cols + tid;
-      if (tid < a.bias_cols && c < kTileN && n0 + c < a.outs) static_cast<O*>(a.bias)[n0 + c] = from_f32<O>(good ? sm.bias[c] : nan);
-    }
-  } else {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    for (int r = 0; r < splits; ++r) good = good && *cluster.map_shared_rank(&sm.ok, r) != 0;
-    const int per = (kTileN + splits - 1) / splits, c_end = min(min((split + 1) * per, kTileN), boxes * 64);
-    for (int i = tid; i < per * (kTileK / 4); i += kThreads) {     // four input features of one column
-      const int c = split * per + i / (kTileK / 4), kl = (i % (kTileK / 4)) * 4;
-      const int n = n0 + c, k = k0 + kl;
-      if (c >= c_end || n >= a.outs || k >= a.ins) continue;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < splits; ++r) {
-        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(reinterpret_cast<float*>(sm.b[0]) + c * kTileK + kl, r));
-        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-      }
-      const float s[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k + j < a.ins) out[(size_t)n * a.ins + k + j] = from_f32<O>(good ? s[j] : nan);
-    }
-    if (has_bias && split == 0) {
-      const int c = blockIdx.x * a.bias_cols + tid;
-      if (tid < a.bias_cols && c < kTileN && n0 + c < a.outs) {
-        float s = 0.f;
-        for (int r = 0; r < splits; ++r) s += *cluster.map_shared_rank(&sm.bias[c], r);
-        static_cast<O*>(a.bias)[n0 + c] = from_f32<O>(good ? s : nan);
-      }
-    }
-    cluster.sync();   // nobody's shared memory goes before its readers are done
-  }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
+  if (sm.failed) {   // arrivals that nobody waited for any more may still be on their way here
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 50000) {
+    }
+  }
+  __syncwarp();
   if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  cluster_sync();   // (the pair gives its tensor memory back together)
+}
+
+// Adds the runs of each tile that more than one pair worked on, in the order of their tokens.  A block takes 8 output
+// features of one of the tile's two halves of input features, a thread four neighbouring input features.
+template <class O>
+__global__ void __launch_bounds__(256) wgrad_runs_kernel(const WgradArgs a) {
+  __shared__ int s_p0, s_p1;
+  const int r = blockIdx.y, half = blockIdx.z;
+  const Tile t = tile_at(a, a.whole * a.pairs + r, half);
+  if (threadIdx.x == 0) {
+    // pairs [p0, p1]: the first whose run ends after the tile begins, the last whose run begins before the tile ends
+    const long long total = (long long)a.rest * a.steps, first = (long long)r * a.steps, last = first + a.steps;
+    int p0 = (int)(first * a.rest_pairs / total);
+    while (p0 > 0 && p0 * total / a.rest_pairs > first) --p0;
+    while ((p0 + 1) * total / a.rest_pairs <= first) ++p0;
+    int p1 = p0;
+    while (p1 + 1 < a.rest_pairs && (p1 + 1) * total / a.rest_pairs < last) ++p1;
+    s_p0 = p0 * 2 + (r - (int)(p0 * total / a.rest_pairs / a.steps));   // its slot: the tile is the first or the second of its run
+    s_p1 = p1 * 2;                                                      // the tile is the first of all later runs
+  }
+  __syncthreads();
+  cudaGridDependencySynchronize();
+  const int p0 = s_p0, p1 = s_p1;
+  if (p1 <= p0) return;    // one pair did it all, straight to the output
+  const int c = blockIdx.x * 8 + (threadIdx.x >> 5), kl = (threadIdx.x & 31) * 4, n = t.n0 + c, k = t.k0 + kl;
+  if (c < t.boxes * 128 && n < a.outs && k < a.ins) {
+    const float* const q = a.work + (half * kTileN + c) * kTileK + kl;
+    float4 s = *reinterpret_cast<const float4*>(q + (size_t)p0 * kSlotFloats);
+    for (int p = (p0 | 1) + 1; p <= p1; p += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(q + (size_t)p * kSlotFloats);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    O* const out = static_cast<O*>(a.out) + (size_t)n * a.ins + k;
+    const float f[4] = {s.x, s.y, s.z, s.w};
+    if (a.ins % 4 == 0) {     // (the output is a fresh allocation: its rows start where four elements do)
+      struct alignas(4 * sizeof(O)) Four { O v[4]; };
+      *reinterpret_cast<Four*>(out) = {{from_f32<O>(f[0]), from_f32<O>(f[1]), from_f32<O>(f[2]), from_f32<O>(f[3])}};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j < a.ins) out[j] = from_f32<O>(f[j]);
+    }
+  }
+  const int col = t.share * a.bias_cols + threadIdx.x, nb = t.n0 + half * t.boxes * 64 + col;
+  if (blockIdx.x == 0 && (int)threadIdx.x < a.bias_cols && col < t.boxes * 64 && nb < a.outs) {
+    const float* const q = a.work + kPartFloats + half * kHalfN + col;
+    float s = q[(size_t)p0 * kSlotFloats];
+    for (int p = (p0 | 1) + 1; p <= p1; p += 2) s += q[(size_t)p * kSlotFloats];
+    static_cast<O*>(a.bias)[nb] = from_f32<O>(s);
+  }
 }
 
 // Rows of 16-bit elements copied to a pitch that TMA accepts (the source's is odd, or it starts off a 16-byte boundary).
@@ -373,24 +614,51 @@ bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How a call is cut up.
+struct Plan {
+  int tiles_k, tiles, steps, pairs, whole, rest, rest_pairs, chunk;
+  size_t work_bytes;
+};
+Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
+  Plan p{};
+  p.tiles_k = (ins + 2 * kTileK - 1) / (2 * kTileK);
+  p.tiles = p.tiles_k * ((outs + kTileN - 1) / kTileN);
+  p.steps = (int)((tokens + kStep - 1) / kStep);
+  p.pairs = sms / 2;
+  p.whole = p.tiles / p.pairs;
+  p.rest = p.tiles % p.pairs;
+  // The last wave's tiles are shared out where that saves more steps than the second kernel and the partial sums cost,
+  // at least four steps for each pair.
+  p.rest_pairs = p.rest;
+  if (p.rest) {
+    const long long total = (long long)p.rest * p.steps;
+    long long n = total / 4 < p.pairs ? total / 4 : p.pairs;
+    if (n > p.rest && p.steps - (total + n - 1) / n >= kMinSavedSteps) p.rest_pairs = (int)n;
+  }
+  p.chunk = out_f32 ? kChunkSteps : p.steps;
+  p.work_bytes = p.rest_pairs > p.rest ? (size_t)p.rest_pairs * 2 * kSlotFloats * 4 : 0;
+  return p;
+}
+
 template <class T, class O>
-cudaError_t launch_typed(const CUtensorMap& dy, const CUtensorMap& codes, const WgradArgs& a, dim3 grid, cudaStream_t stream) {
+cudaError_t launch_typed(const CUtensorMap& dy, const CUtensorMap& codes, const WgradArgs& a, cudaStream_t stream) {
   const int smem = (int)sizeof(WgradSmem) + 1024;
   cudaError_t err = cudaFuncSetAttribute(wgrad_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
+  wgrad_kernel<T, O><<<2 * (a.whole ? a.pairs : a.rest_pairs), kThreads, smem, stream>>>(dy, codes, a);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || a.rest_pairs == a.rest) return err;
+  // (its blocks may be set up while the first kernel still runs; they wait for its end before they read)
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(kTileN / 8, a.rest, 2);
+  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = grid.z;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, wgrad_kernel<T, O>, dy, codes, a);
+  return cudaLaunchKernelEx(&cfg, wgrad_runs_kernel<O>, a);
 }
 
 }  // namespace
@@ -404,6 +672,10 @@ cudaError_t launch_act8_repitch(const void* src, long long stride, void* dst, lo
   return cudaGetLastError();
 }
 
+size_t act8_wgrad_work_bytes(long long tokens, int outs, int ins, int out_f32, int sms) {
+  return tokens > 0 && outs > 0 && ins > 0 ? make_plan(tokens, outs, ins, out_f32 != 0, sms).work_bytes : 0;
+}
+
 cudaError_t act8_wgrad_status(unsigned* words) {
   cudaError_t err = cudaMemcpyFromSymbol(words, wgrad_status, sizeof(wgrad_status));   // waits for the device's work
   if (err != cudaSuccess || words[0] == kOk) return err;
@@ -412,7 +684,7 @@ cudaError_t act8_wgrad_status(unsigned* words) {
 }
 
 cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held, long long tokens, int outs, int ins, int dtype,
-                              int out_f32, void* out, void* bias, int sms, cudaStream_t stream) {
+                              int out_f32, void* out, void* bias, void* work, int sms, cudaStream_t stream) {
   if (tokens <= 0 || outs <= 0 || ins <= 0 || tokens > (1ll << 31) - 64) return cudaErrorInvalidValue;
   if (dtype != kGradBF16 && dtype != kGradF16) return cudaErrorInvalidValue;
   if (reinterpret_cast<uintptr_t>(grad) % 16 || grad_stride % 8 || reinterpret_cast<uintptr_t>(held.codes) % 16 || held.pitch % 32)
@@ -423,22 +695,20 @@ cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held
   if (!encode(&map_dy, type, grad, outs, tokens, grad_stride * 2, 64, kStep, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, held.codes, held.pitch, tokens, held.pitch, kTileK, kStep, CU_TENSOR_MAP_SWIZZLE_NONE))
     return cudaErrorInvalidValue;
-  const int kt = (ins + kTileK - 1) / kTileK, nt = (outs + kTileN - 1) / kTileN;
-  const int steps = (int)((tokens + kStep - 1) / kStep);
-  int splits = 1;
-  while (splits < 8 && (long long)kt * nt * (splits + 1) <= sms && steps / (splits + 1) >= 4) ++splits;
+  const Plan plan = make_plan(tokens, outs, ins, out_f32, sms);
+  if (plan.work_bytes && !work) return cudaErrorInvalidValue;
   int bias_cols = 0;
   if (bias) {
-    bias_cols = 2;
-    while (bias_cols * kt < kTileN) bias_cols *= 2;
+    bias_cols = 8;
+    while (bias_cols * plan.tiles_k < kHalfN) bias_cols *= 2;
   }
-  const WgradArgs a{held.scales, held.spitch, tokens, outs, ins, steps, bias_cols, out, bias};
-  const dim3 grid(kt, nt, splits);
+  const WgradArgs a{held.scales, held.spitch, tokens, outs, ins, plan.tiles_k, plan.pairs, plan.whole, plan.rest, plan.rest_pairs,
+                    plan.steps, plan.chunk, bias_cols, out, bias, static_cast<float*>(work)};
   if (dtype == kGradBF16)
-    return out_f32 ? launch_typed<__nv_bfloat16, float>(map_dy, map_codes, a, grid, stream)
-                   : launch_typed<__nv_bfloat16, __nv_bfloat16>(map_dy, map_codes, a, grid, stream);
-  return out_f32 ? launch_typed<__half, float>(map_dy, map_codes, a, grid, stream)
-                 : launch_typed<__half, __half>(map_dy, map_codes, a, grid, stream);
+    return out_f32 ? launch_typed<__nv_bfloat16, float>(map_dy, map_codes, a, stream)
+                   : launch_typed<__nv_bfloat16, __nv_bfloat16>(map_dy, map_codes, a, stream);
+  return out_f32 ? launch_typed<__half, float>(map_dy, map_codes, a, stream)
+                 : launch_typed<__half, __half>(map_dy, map_codes, a, stream);
 }
 
 }  // namespace grace

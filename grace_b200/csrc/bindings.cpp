@@ -327,11 +327,12 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
           "act8_repitch");
   });
   m.def("act8_wgrad", [](uintptr_t grad, long long grad_stride, uintptr_t codes, uintptr_t scales, int pitch, int spitch,
-                         long long tokens, int outs, int ins, int dtype, int out_f32, uintptr_t out, uintptr_t bias, int sms,
-                         uintptr_t stream) {
+                         long long tokens, int outs, int ins, int dtype, int out_f32, uintptr_t out, uintptr_t bias,
+                         uintptr_t work, int sms, uintptr_t stream) {
     check(launch_act8_wgrad(ptr<const void>(grad), grad_stride, held(codes, scales, pitch, spitch), tokens, outs, ins, dtype,
-                            out_f32, ptr<void>(out), ptr<void>(bias), sms, reinterpret_cast<cudaStream_t>(stream)), "act8_wgrad");
+                            out_f32, ptr<void>(out), ptr<void>(bias), ptr<void>(work), sms, reinterpret_cast<cudaStream_t>(stream)), "act8_wgrad");
   });
+  m.def("act8_wgrad_work_bytes", &act8_wgrad_work_bytes);
   m.def("act8_wgrad_status", []() {
     std::vector<unsigned> words(16);
     py::gil_scoped_release release;

@@ -21,25 +21,29 @@ __device__ __forceinline__ void mbar_expect_tx(void* bar, unsigned bytes) {
 __device__ __forceinline__ void mbar_arrive(void* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity) {
+// One try: the hardware suspends the thread until the phase is over or the hint (nanoseconds) has passed, whichever is
+// first.
+__device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity, unsigned hint_ns) {
   unsigned ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns) : "memory");
   return ok != 0;
 }
-// Bounded wait; returns false (and records the failure) when the limit expires or another role already failed.
+// Bounded wait; returns false (and records the failure) when the limit expires or another role already failed.  The
+// status word and the clock are looked at once in 64 tries that ran out: a global load and a clock read in between
+// would answer the barrier a microsecond late, which is longer than the usual wait.
 __device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, uint64_t timeout_ns, const Status& status,
                                           unsigned detail) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  unsigned spins = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    if ((++spins & 0x3f) == 0) {
+  uint64_t t0 = 0;
+  for (unsigned spins = 1; !mbar_try_wait(bar, parity, 20000); ++spins) {
+    if ((spins & 0x3f) == 0) {
       if (status.failed()) return false;
-      if (globaltimer_ns() - t0 > timeout_ns) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > timeout_ns) {
         status.fail(kTimeoutMbarrier, detail, 0);
         return false;
       }
@@ -53,6 +57,7 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
       ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
 // Shared-memory matrix descriptor: start>>4 [0,14) | LBO>>4 [16,30) | SBO>>4 [32,46) | version 1 [46,48) |

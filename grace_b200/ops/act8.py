@@ -243,9 +243,12 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
             g = wide
         out = torch.empty((outs, ins), dtype=dtype, device=grad.device)
         db = torch.empty(outs, dtype=dtype, device=grad.device) if bias else None
+        f32, sms = int(dtype == torch.float32), _sms(grad.device)
+        nbytes = C.act8_wgrad_work_bytes(rows, outs, ins, f32, sms)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
         C.act8_wgrad(g.data_ptr(), g.stride(0), *_ptrs(held), held.codes.shape[1], held.scales.shape[1], rows, outs, ins,
-                     GRAD_DTYPE[g.dtype], int(dtype == torch.float32), out.data_ptr(), db.data_ptr() if bias else 0,
-                     _sms(grad.device), stream)
+                     GRAD_DTYPE[g.dtype], f32, out.data_ptr(), db.data_ptr() if bias else 0,
+                     0 if work is None else work.data_ptr(), sms, stream)
     return out, db
 
 

@@ -156,7 +156,7 @@ def test_weight_grad_types_and_odd_sizes(tokens, outs, ins, dtype, out):
     check_weight_grad(tokens, outs, ins, dtype, out)
 
 
-@pytest.mark.parametrize("tokens,outs,ins", [(4096, 1024, 1024), (16384, 512, 640), (300, 4096, 2500)])
+@pytest.mark.parametrize("tokens,outs,ins", [(4096, 1024, 1024), (16384, 512, 640), (300, 4096, 2500), (5000, 1000, 99), (9000, 2100, 2700)])
 def test_weight_grad_larger(tokens, outs, ins):
     check_weight_grad(tokens, outs, ins, BF16, FP32, bias=True)
     check_weight_grad(tokens, outs, ins, BF16, BF16, bias=False)
@@ -287,3 +287,21 @@ def test_side_stream():
         got = act8.weight_grad(g, act8.pack(y))[0]
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want)
+
+
+def test_weight_grad_fp16_over_its_whole_range():
+    """Groups from fp16's smallest subnormal to its largest value, each against weights of one: the decoded operand itself."""
+    tokens, cols = 41, 64
+    x = torch.zeros(tokens, cols)
+    g = torch.Generator().manual_seed(28)
+    for t in range(tokens):
+        x[t] = (torch.rand(cols, generator=g) * 2 - 1) * 2.0 ** (t - 24)
+        x[t, 0] = 2.0 ** (t - 24) * (1 if t < 40 else 0.99)
+    x = x.clamp(-65504, 65504).to(FP16)
+    eye = torch.eye(tokens, dtype=FP16)
+    dw, _ = act8.weight_grad(eye.cuda(), act8.pack(x.cuda()), dtype=FP32)
+    close(dw, held_value(x), 2.0 ** -25, "decoded")       # exact but for subnormals, half a step of 2^-24
+    x = torch.zeros(2, 64)
+    x[0, :32], x[1, 32:] = 1e5, 1.0                          # beyond fp16: the group is NaN, the others are not
+    dw, _ = act8.weight_grad(eye[:2, :2].cuda(), act8.Act8(*(lambda h: (h.codes, h.scales))(act8.pack(x.cuda())), (2, 64), FP16))
+    assert dw[0, :32].isnan().all() and (dw[1, 32:] == 1).all()
