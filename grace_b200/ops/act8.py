@@ -19,7 +19,6 @@ what it needs from torch's allocator on the current stream of the tensor's devic
 """
 from __future__ import annotations
 
-import contextlib
 import math
 from typing import Optional, Tuple, Union
 
@@ -27,7 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from . import native
-from .exchange import GRAD_DTYPE, GraceCommError
+from .exchange import GRAD_DTYPE, GraceCommError, _stream_ptr
 
 GROUP = 32
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
@@ -45,7 +44,7 @@ class Act8:
     """A checkpoint of a tensor of ``shape`` and ``dtype``: ``codes`` int8 ``[rows, pitch]`` and ``scales`` uint8
     ``[rows, spitch]`` (``pitch_of``), rows being the product of all axes but the last."""
 
-    __slots__ = ("codes", "scales", "shape", "dtype")
+    __slots__ = ("shape", "dtype", "rows", "pitch", "spitch", "_data", "_at", "_codes", "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype):
         shape = tuple(shape)
@@ -64,45 +63,80 @@ class Act8:
             raise ValueError("Act8: codes and scales are on different devices")
         if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 8:
             raise ValueError("Act8: codes and scales are contiguous, and start on 16- and 8-byte boundaries")
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, shape, dtype
+        self.shape, self.dtype, self.rows, self.pitch, self.spitch = shape, dtype, rows, pitch, spitch
+        self._data, self._at, self._codes, self._scales = None, 0, codes, scales
+
+    @classmethod
+    def _over(cls, data: torch.Tensor, at: int, shape, dtype: torch.dtype) -> "Act8":
+        """A checkpoint in ``data`` (uint8) from byte ``at``, a multiple of 16, on: the codes, then the scales.  One allocation holds it,
+        or several of them, because allocating costs a small call more than computing."""
+        held = cls.__new__(cls)
+        pitch, spitch = pitch_of(shape[-1])
+        held.shape, held.dtype, held.rows, held.pitch, held.spitch = shape, dtype, math.prod(shape[:-1]), pitch, spitch
+        held._data, held._at, held._codes, held._scales = data, at, None, None
+        return held
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            n = self.rows * self.pitch
+            self._codes = self._data[self._at : self._at + n].view(torch.int8).view(self.rows, self.pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            at = self._at + self.rows * self.pitch
+            self._scales = self._data[at : at + self.rows * self.spitch].view(self.rows, self.spitch)
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
-
-    @property
-    def rows(self) -> int:
-        return self.codes.shape[0]
+        return (self._codes if self._data is None else self._data).device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.rows * (self.pitch + self.spitch)
+
+    def _tensors(self) -> Tuple[torch.Tensor, ...]:
+        return (self._data,) if self._data is not None else (self._codes, self._scales)
+
+    def _with(self, tensors) -> "Act8":
+        """This checkpoint over ``_tensors()`` as autograd gives them back."""
+        held = Act8.__new__(Act8)
+        for name in ("shape", "dtype", "rows", "pitch", "spitch", "_at"):
+            setattr(held, name, getattr(self, name))
+        held._data, held._codes, held._scales = (tensors[0], None, None) if len(tensors) == 1 else (None,) + tuple(tensors)
+        return held
+
+    def _shell(self) -> "Act8":
+        """Its description without its tensors, for a context that saves those with autograd's own means."""
+        return self._with((None,))
 
     def __repr__(self):
         return "Act8(shape=%s, dtype=%s, device=%s, nbytes=%d)" % (self.shape, self.dtype, self.device, self.nbytes)
 
 
+def held_bytes(shape) -> int:
+    """Bytes of a checkpoint of a tensor of ``shape``, rounded up to a multiple of 16."""
+    pitch, spitch = pitch_of(shape[-1])
+    return (math.prod(shape[:-1]) * (pitch + spitch) + 15) // 16 * 16
+
+
 def empty_like(shape, dtype: torch.dtype, device) -> Act8:
     """An Act8 for a tensor of ``shape`` whose contents are yet to be written."""
-    shape = tuple(shape)
-    rows, (pitch, spitch) = math.prod(shape[:-1]), pitch_of(shape[-1])
-    held = Act8.__new__(Act8)     # (its arrays are made to measure: nothing to check)
-    held.codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-    held.scales = torch.empty((rows, spitch), dtype=torch.uint8, device=device)
-    held.shape, held.dtype = shape, dtype
-    return held
+    return Act8._over(torch.empty(held_bytes(shape), dtype=torch.uint8, device=device), 0, shape, dtype)
 
 
 # ---------------------------------------------------------------------------------------------------- shared checks
-def _on(device: torch.device):
-    """The device to launch on, made current for the launch if it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _launch(device: torch.device, launch, *args) -> None:
+    """``launch(*args, stream)`` on the current stream of ``device``, which is made current for the call if it is not."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        launch(*args, _stream_ptr(index))
+    else:
+        with torch.cuda.device(index):
+            launch(*args, _stream_ptr(index))
 
 
 def _check_tensor(x, what: str) -> None:
@@ -120,17 +154,21 @@ def _check_tensor(x, what: str) -> None:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as ``[rows, cols]`` with neighbouring columns; a copy only where its strides leave no other way."""
-    cols = x.shape[-1]
-    x = x.detach()
     if x.dim() != 2:
-        x = x.reshape(math.prod(x.shape[:-1]), cols)
-    if cols > 1 and x.stride(1) != 1:
-        x = x.contiguous()
+        x = x.detach().reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.detach().contiguous()
     return x
 
 
 def _ptrs(held: Optional[Act8]) -> Tuple[int, int]:
-    return (held.codes.data_ptr(), held.scales.data_ptr()) if held is not None else (0, 0)
+    """Addresses of a checkpoint's codes and scales."""
+    if held is None:
+        return 0, 0
+    if held._data is None:
+        return held._codes.data_ptr(), held._scales.data_ptr()
+    at = held._data.data_ptr() + held._at
+    return at, at + held.rows * held.pitch
 
 
 # -------------------------------------------------------------------------------------------- the arithmetic on CPU
@@ -173,12 +211,12 @@ def _function_cpu(x: torch.Tensor, kind: str) -> Tuple[torch.Tensor, torch.Tenso
 def pack(x: torch.Tensor) -> Act8:
     """The checkpoint of ``x`` (fp32, bf16 or fp16, any shape and strides)."""
     _check_tensor(x, "act8.pack")
-    held = empty_like(x.shape, x.dtype, x.device)
+    device = x.device
+    held = empty_like(x.shape, x.dtype, device)
     if x.is_cuda:
-        v, cols = _rows(x), x.shape[-1]
-        with _on(x.device):
-            native().act8_pack(v.data_ptr(), v.stride(0), held.rows, cols, GRAD_DTYPE[x.dtype], *_ptrs(held), held.codes.shape[1],
-                               held.scales.shape[1], _stream(x.device))
+        v = _rows(x)
+        _launch(device, native().act8_pack, v.data_ptr(), v.stride(0), held.rows, held.shape[-1], GRAD_DTYPE[x.dtype], *_ptrs(held),
+                held.pitch, held.spitch)
     else:
         _encode_cpu(x, held)
     return held
@@ -189,11 +227,10 @@ def unpack(held: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     dtype = held.dtype if dtype is None else dtype
     if dtype not in GRAD_DTYPE:
         raise TypeError("act8.unpack: fp32, bf16 or fp16, not %s" % dtype)
-    if held.codes.is_cuda:
-        out, cols = torch.empty(held.shape, dtype=dtype, device=held.device), held.shape[-1]
-        with _on(held.device):
-            native().act8_unpack(*_ptrs(held), held.codes.shape[1], held.scales.shape[1], out.data_ptr(), cols, held.rows, cols,
-                                 GRAD_DTYPE[dtype], _stream(held.device))
+    device = held.device
+    if device.type == "cuda":
+        out, cols = torch.empty(held.shape, dtype=dtype, device=device), held.shape[-1]
+        _launch(device, native().act8_unpack, *_ptrs(held), held.pitch, held.spitch, out.data_ptr(), cols, held.rows, cols, GRAD_DTYPE[dtype])
         return out
     return _decode_cpu(held).to(dtype)
 
@@ -234,21 +271,18 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
     if rows == 0 or outs == 0 or ins == 0:
         return (torch.zeros((outs, ins), dtype=dtype, device=grad.device),
                 torch.zeros(outs, dtype=dtype, device=grad.device) if bias else None)
-    C, g = native(), _rows(grad)
-    with _on(grad.device):
-        stream = _stream(grad.device)
-        if g.data_ptr() % 16 or g.stride(0) % 8 or g.stride(0) < outs:   # not what a TMA load takes
-            wide = torch.empty((rows, -(-outs // 8) * 8), dtype=g.dtype, device=g.device)
-            C.act8_repitch(g.data_ptr(), g.stride(0), wide.data_ptr(), rows, outs, stream)
-            g = wide
-        out = torch.empty((outs, ins), dtype=dtype, device=grad.device)
-        db = torch.empty(outs, dtype=dtype, device=grad.device) if bias else None
-        f32, sms = int(dtype == torch.float32), _sms(grad.device)
-        nbytes = C.act8_wgrad_work_bytes(rows, outs, ins, f32, sms)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None
-        C.act8_wgrad(g.data_ptr(), g.stride(0), *_ptrs(held), held.codes.shape[1], held.scales.shape[1], rows, outs, ins,
-                     GRAD_DTYPE[g.dtype], f32, out.data_ptr(), db.data_ptr() if bias else 0,
-                     0 if work is None else work.data_ptr(), sms, stream)
+    C, g, device = native(), _rows(grad), grad.device
+    if g.data_ptr() % 16 or g.stride(0) % 8 or g.stride(0) < outs:   # not what a TMA load takes
+        wide = torch.empty((rows, -(-outs // 8) * 8), dtype=g.dtype, device=device)
+        _launch(device, C.act8_repitch, g.data_ptr(), g.stride(0), wide.data_ptr(), rows, outs)
+        g = wide
+    out = torch.empty((outs, ins), dtype=dtype, device=device)
+    db = torch.empty(outs, dtype=dtype, device=device) if bias else None
+    f32, sms = int(dtype == torch.float32), _sms(device)
+    nbytes = C.act8_wgrad_work_bytes(rows, outs, ins, f32, sms)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch(device, C.act8_wgrad, g.data_ptr(), g.stride(0), *_ptrs(held), held.pitch, held.spitch, rows, outs, ins, GRAD_DTYPE[g.dtype],
+            f32, out.data_ptr(), db.data_ptr() if bias else 0, 0 if work is None else work.data_ptr(), sms)
     return out, db
 
 
@@ -256,7 +290,7 @@ def check(device=None) -> None:
     """Waits for the device and raises ``GraceCommError`` if a bounded wait of a ``weight_grad`` kernel ran out since the last
     check (its results are NaN)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    with _on(device):
+    with torch.cuda.device(device):
         words = native().act8_wgrad_status()
     if words[0]:
         raise GraceCommError(words[0], words[1], words[2], 0)
@@ -281,16 +315,21 @@ def activation_forward(x: torch.Tensor, kind: str = "gelu", gated: bool = False,
     _check_tensor(x, "act8.activation")
     if gated and x.shape[-1] % 2:
         raise ValueError("act8.activation: a gated function takes two halves, not %d columns" % x.shape[-1])
-    cols = x.shape[-1] // 2 if gated else x.shape[-1]
+    cols, device, dtype = x.shape[-1] // 2 if gated else x.shape[-1], x.device, x.dtype
     shape = x.shape[:-1] + (cols,)
-    a = empty_like(shape, x.dtype, x.device) if checkpoint else None
-    b = empty_like(shape, x.dtype, x.device) if checkpoint and gated else None
-    out = empty_like(shape, x.dtype, x.device) if checkpoint_output else None
+    a = b = out = None
+    parts = (2 if gated else 1) if checkpoint else 0
+    if parts:
+        n = held_bytes(shape)
+        data = torch.empty(parts * n, dtype=torch.uint8, device=device)
+        a = Act8._over(data, 0, shape, dtype)
+        b = Act8._over(data, n, shape, dtype) if gated else None
+    if checkpoint_output:
+        out = empty_like(shape, dtype, device)
     if x.is_cuda:
-        y, v = torch.empty(shape, dtype=x.dtype, device=x.device), _rows(x)
-        with _on(x.device):
-            native().act8_forward(v.data_ptr(), v.stride(0), y.data_ptr(), v.shape[0], cols, GRAD_DTYPE[x.dtype], k, int(gated), *_ptrs(a),
-                                  *_ptrs(b), *_ptrs(out), *pitch_of(cols), _stream(x.device))
+        y, v = torch.empty(shape, dtype=dtype, device=device), _rows(x)
+        _launch(device, native().act8_forward, v.data_ptr(), v.stride(0), y.data_ptr(), v.shape[0], cols, GRAD_DTYPE[dtype], k, int(gated),
+                *_ptrs(a), *_ptrs(b), *_ptrs(out), *pitch_of(cols))
     else:
         v = x.detach()
         y = _function_cpu(v[..., :cols].float(), kind)[0]
@@ -314,13 +353,11 @@ def activation_backward(grad: torch.Tensor, held: Held, kind: str = "gelu", gate
         raise ValueError("act8.activation: grad %s for a checkpoint of %s" % (tuple(grad.shape), a.shape))
     if grad.device != a.device or (gated and b.device != a.device):
         raise ValueError("act8.activation: grad is on %s, the checkpoint on %s" % (grad.device, a.device))
-    cols = a.shape[-1]
+    cols, device = a.shape[-1], grad.device
     if grad.is_cuda:
-        dx = torch.empty(grad.shape[:-1] + (cols * (2 if gated else 1),), dtype=grad.dtype, device=grad.device)
-        g = _rows(grad)
-        with _on(grad.device):
-            native().act8_backward(g.data_ptr(), g.stride(0), dx.data_ptr(), a.rows, cols, GRAD_DTYPE[grad.dtype], k, int(gated),
-                                   *_ptrs(a), *_ptrs(b), a.codes.shape[1], a.scales.shape[1], _stream(grad.device))
+        dx, g = torch.empty(grad.shape[:-1] + (cols * (2 if gated else 1),), dtype=grad.dtype, device=device), _rows(grad)
+        _launch(device, native().act8_backward, g.data_ptr(), g.stride(0), dx.data_ptr(), a.rows, cols, GRAD_DTYPE[grad.dtype], k, int(gated),
+                *_ptrs(a), *_ptrs(b), a.pitch, a.spitch)
         return dx
     g = grad.detach().float()
     f, d = _function_cpu(_decode_cpu(a), kind)
@@ -330,24 +367,24 @@ def activation_backward(grad: torch.Tensor, held: Held, kind: str = "gelu", gate
 # ------------------------------------------------------------------------------------------------------ with autograd
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, codes, scales):
-        ctx.save_for_backward(codes, scales, weight)
-        ctx.x_shape, ctx.has_bias = x.shape, bias is not None
+    def forward(ctx, x, weight, bias, held):
+        ctx.save_for_backward(weight, *held._tensors())
+        ctx.held, ctx.has_bias = held._shell(), bias is not None
         return F.linear(x, weight, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        codes, scales, weight = ctx.saved_tensors
+        weight, *tensors = ctx.saved_tensors
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             dx = grad @ weight
         want_bias = ctx.has_bias and ctx.needs_input_grad[2]
         if ctx.needs_input_grad[1]:
-            dw, db = weight_grad(grad, Act8(codes, scales, ctx.x_shape, grad.dtype), bias=want_bias)
+            dw, db = weight_grad(grad, ctx.held._with(tensors), bias=want_bias)
         elif want_bias:
             db = grad.reshape(-1, grad.shape[-1]).sum(0)
-        return dx, dw, db, None, None
+        return dx, dw, db, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, checkpoint: Optional[Act8] = None
@@ -367,36 +404,33 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     elif checkpoint.shape != tuple(x.shape) or checkpoint.device != x.device:
         raise ValueError("act8.linear: a checkpoint of %s on %s for x %s on %s"
                          % (checkpoint.shape, checkpoint.device, tuple(x.shape), x.device))
-    return _Linear.apply(x, weight, bias, checkpoint.codes, checkpoint.scales)
+    return _Linear.apply(x, weight, bias, checkpoint)
 
 
 class _Activation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, kind, gated, checkpoint_output):
+    def forward(ctx, x, kind, gated, checkpoint_output, box):
         y, held, out = activation_forward(x, kind, gated, checkpoint_output)
-        parts = held if gated else (held,)
-        ctx.save_for_backward(*(t for h in parts for t in (h.codes, h.scales)))
-        ctx.kind, ctx.gated, ctx.shape, ctx.dtype = kind, gated, parts[0].shape, x.dtype
-        if out is None:
-            return y
-        ctx.mark_non_differentiable(out.codes, out.scales)
-        return y, out.codes, out.scales
+        box.append(out)
+        a = held[0] if gated else held       # (of a pair, both are in one allocation)
+        ctx.save_for_backward(a._data)
+        ctx.kind, ctx.held = kind, tuple(h._shell() for h in held) if gated else (a._shell(),)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad, *_):
-        t = ctx.saved_tensors
-        held = tuple(Act8(t[i], t[i + 1], ctx.shape, ctx.dtype) for i in range(0, len(t), 2))
-        return activation_backward(grad, held if ctx.gated else held[0], ctx.kind, ctx.gated), None, None, None
+    def backward(ctx, grad):
+        held = tuple(h._with(ctx.saved_tensors) for h in ctx.held)
+        gated = len(held) == 2
+        return activation_backward(grad, held if gated else held[0], ctx.kind, gated), None, None, None, None
 
 
 def activation(x: torch.Tensor, kind: str = "gelu", gated: bool = False, checkpoint_output: bool = False):
     """``activation_forward`` with autograd: ``y``, or with ``checkpoint_output`` the pair ``(y, Act8 of y)`` for the ``linear`` after it."""
-    if not (torch.is_grad_enabled() and x.requires_grad):
+    if torch.is_grad_enabled() and x.requires_grad:
+        box = []
+        y = _Activation.apply(x, kind, gated, checkpoint_output, box)
+        held_y = box[0]
+    else:
         y, _, held_y = activation_forward(x, kind, gated, checkpoint_output, checkpoint=False)
-        return (y, held_y) if checkpoint_output else y
-    got = _Activation.apply(x, kind, gated, checkpoint_output)
-    if not checkpoint_output:
-        return got
-    y, codes, scales = got
-    return y, Act8(codes, scales, y.shape, y.dtype)
+    return (y, held_y) if checkpoint_output else y

@@ -17,12 +17,12 @@ ones; parameter gradients are fp32 sums in a fixed order, rounded once to the pa
 from __future__ import annotations
 
 import math
-from typing import Dict, NamedTuple, Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import native
-from .act8 import Act8, _check_tensor, _decode_cpu, _encode_cpu, _on, _ptrs, _rows, _sms, _stream, empty_like, pitch_of
+from .act8 import Act8, _check_tensor, _decode_cpu, _encode_cpu, _launch, _ptrs, _rows, _sms, empty_like, held_bytes, pitch_of
 from .exchange import GRAD_DTYPE
 
 NORMS = {None: 0, "rms": 1, "layer": 2}
@@ -32,18 +32,29 @@ MAX_SEQUENCES = 65534
 PARAMS = ("pre_weight", "pre_bias", "post_weight", "post_bias", "gate")
 
 
-class Saved(NamedTuple):
-    """What the backward pass takes from the forward pass."""
+class Saved:
+    """What the backward pass takes from the forward pass: one allocation with the checkpoints and the statistics, the parameters, and the
+    forms of the norms."""
 
-    held_y: Act8
-    held_block: Optional[Act8]
-    stats: torch.Tensor                  # fp32 [rows, 4]: mean and 1 / deviation of y, then of block
-    params: Tuple[Optional[torch.Tensor], ...]    # as PARAMS
-    pre: str
-    post: Optional[str]
-    residual_scale: float
-    return_stream: bool
-    held_h: Optional[Act8] = None        # checkpoint of h for the layer that reads it, on request
+    __slots__ = ("data", "shape", "dtype", "params", "pre", "post", "residual_scale", "return_stream", "held_y", "held_block", "held_h", "_at")
+
+    def __init__(self, data: Optional[torch.Tensor], shape, dtype, device, params, pre, post, residual_scale, return_stream, held_h=None):
+        two = post is not None or params[4] is not None
+        n, rows = held_bytes(shape), math.prod(shape[:-1])
+        self._at = n * (2 if two else 1)
+        self.data = torch.empty(self._at + 16 * rows, dtype=torch.uint8, device=device) if data is None else data
+        self.shape, self.dtype, self.params, self.pre, self.post = shape, dtype, params, pre, post
+        self.residual_scale, self.return_stream, self.held_h = residual_scale, return_stream, held_h
+        self.held_y = Act8._over(self.data, 0, shape, dtype)
+        self.held_block = Act8._over(self.data, n, shape, dtype) if two else None
+
+    @property
+    def stats(self) -> torch.Tensor:
+        """fp32 ``[rows, 4]``: mean and 1 / deviation of ``y``, then of ``block`` (0 and 1 without ``post``)."""
+        return self.data[self._at :].view(torch.float32).view(-1, 4)
+
+    def stats_ptr(self) -> int:
+        return self.data.data_ptr() + self._at
 
 
 def _check(x, block, pre, post, params, residual_scale, eps) -> int:
@@ -87,7 +98,7 @@ def _check(x, block, pre, post, params, residual_scale, eps) -> int:
 
 def _param_ptrs(params):
     """The parameters' addresses, and the tensors that have to live until the launch."""
-    kept = [None if p is None else p.detach().contiguous() for p in params]
+    kept = [p if p is None or p.is_contiguous() else p.detach().contiguous() for p in params]
     return [0 if p is None else p.data_ptr() for p in kept], kept
 
 
@@ -99,23 +110,19 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     """``(h, y, saved)`` (``y`` None without ``return_stream``); with ``checkpoint_output`` ``saved.held_h`` is what ``act8.pack(h)`` gives."""
     params = (pre_weight, pre_bias, post_weight, post_bias, gate)
     gate_rows = _check(x, block, pre, post, params, residual_scale, eps)
-    cols, rows, two = x.shape[-1], math.prod(x.shape[:-1]), post is not None or gate is not None
-    held_y = empty_like(x.shape, x.dtype, x.device)
-    held_b = empty_like(x.shape, x.dtype, x.device) if two else None
-    held_h = empty_like(x.shape, x.dtype, x.device) if checkpoint_output else None
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device)
-    saved = Saved(held_y, held_b, stats, params, pre, post, float(residual_scale), return_stream, held_h)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    cols, rows = shape[-1], math.prod(shape[:-1])
+    held_h = empty_like(shape, dtype, device) if checkpoint_output else None
+    saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h)
     if not x.is_cuda:
         return _forward_cpu(x, block, saved, float(eps)) + (saved,)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_stream else None
+    h = torch.empty(shape, dtype=dtype, device=device)
+    y = torch.empty(shape, dtype=dtype, device=device) if return_stream else None
     vx, vb = _rows(x), _rows(block)
     ptrs, kept = _param_ptrs(params)
-    with _on(x.device):
-        native().block_norm_forward(vx.data_ptr(), vx.stride(0), vb.data_ptr(), vb.stride(0), h.data_ptr(), 0 if y is None else y.data_ptr(),
-                                    stats.data_ptr(), rows, cols, GRAD_DTYPE[x.dtype], NORMS[pre], NORMS[post], _f32(params),
-                                    float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(held_y) + _ptrs(held_b) + _ptrs(held_h),
-                                    *pitch_of(cols), _stream(x.device))
+    _launch(device, native().block_norm_forward, vx.data_ptr(), vx.stride(0), vb.data_ptr(), vb.stride(0), h.data_ptr(),
+            0 if y is None else y.data_ptr(), saved.stats_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params),
+            float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(saved.held_y) + _ptrs(saved.held_block) + _ptrs(held_h), *pitch_of(cols))
     del kept
     return h, y, saved
 
@@ -129,8 +136,7 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     """The gradients of ``x``, ``block`` and the parameters (``PARAMS``), by name; None where there is no such parameter or ``needs`` (as
     ``PARAMS``) does not ask for it.  ``grad_y`` is that of the stream, None where nothing reads it.  Without ``post`` and gate and with a
     ``residual_scale`` of 1, ``x`` and ``block`` have one gradient: both names give the same tensor."""
-    held_y, held_b, params = saved.held_y, saved.held_block, saved.params
-    shape, dtype, device = held_y.shape, held_y.dtype, held_y.device
+    params, shape, dtype, device = saved.params, saved.shape, saved.dtype, saved.data.device
     for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
         if g is None and name == "grad_y":
             continue
@@ -154,13 +160,11 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     pitch, spitch = pitch_of(cols)
     g, gy = _rows(grad_h), None if grad_y is None else _rows(grad_y)
     ptrs, kept = _param_ptrs(params)
-    with _on(device):
-        sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * pitch, dtype=torch.float32, device=device) if any(want) else None
-        C.block_norm_backward(g.data_ptr(), g.stride(0), 0 if gy is None else gy.data_ptr(), 0 if gy is None else gy.stride(0),
-                              0 if dx is None else dx.data_ptr(), block.data_ptr(), saved.stats.data_ptr(),
-                              0 if sums is None else sums.data_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post],
-                              _f32(params), saved.residual_scale, gate_rows, ptrs, [0 if t is None else t.data_ptr() for t in grads],
-                              _ptrs(held_y) + _ptrs(held_b), pitch, spitch, sms, _stream(device))
+    sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * pitch, dtype=torch.float32, device=device) if any(want) else None
+    _launch(device, C.block_norm_backward, g.data_ptr(), g.stride(0), 0 if gy is None else gy.data_ptr(), 0 if gy is None else gy.stride(0),
+            0 if dx is None else dx.data_ptr(), block.data_ptr(), saved.stats_ptr(), 0 if sums is None else sums.data_ptr(), rows, cols,
+            GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post], _f32(params), saved.residual_scale, gate_rows, ptrs,
+            [0 if t is None else t.data_ptr() for t in grads], _ptrs(saved.held_y) + _ptrs(saved.held_block), pitch, spitch, sms)
     del kept
     got = dict(zip(PARAMS, grads))
     got["x"], got["block"] = block if dx is None else dx, block
@@ -235,45 +239,40 @@ def _backward_cpu(grad_h, grad_y, saved: Saved, want):
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, residual_scale, eps, return_stream,
-                checkpoint_output):
+                checkpoint_output, box):
         ctx.set_materialize_grads(False)
         h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
                                             post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps,
                                             return_stream=return_stream, checkpoint_output=checkpoint_output)
-        held = [t for a in (saved.held_y, saved.held_block) if a is not None for t in (a.codes, a.scales)]
-        ctx.save_for_backward(*saved.params, saved.stats, *held)
-        ctx.kinds, ctx.shape, ctx.dtype = (pre, post, saved.residual_scale, return_stream), tuple(x.shape), x.dtype
-        out = (h,) + ((y,) if return_stream else ())
-        if checkpoint_output:
-            ctx.mark_non_differentiable(saved.held_h.codes, saved.held_h.scales)
-            out += (saved.held_h.codes, saved.held_h.scales)
-        return out
+        box.append(saved.held_h)
+        ctx.save_for_backward(*saved.params, saved.data)
+        ctx.kinds, ctx.shape, ctx.dtype = (pre, post, saved.residual_scale, return_stream), x.shape, x.dtype
+        return (h, y) if return_stream else h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_h, grad_y=None, *_):
+    def backward(ctx, grad_h, grad_y=None):
         t = ctx.saved_tensors
-        held = [Act8(t[i], t[i + 1], ctx.shape, ctx.dtype) for i in range(6, len(t), 2)]
-        pre, post, scale, stream = ctx.kinds
-        saved = Saved(held[0], held[1] if len(held) > 1 else None, t[5], tuple(t[:5]), pre, post, scale, stream)
-        if not stream:
+        saved = Saved(t[5], ctx.shape, ctx.dtype, t[5].device, tuple(t[:5]), *ctx.kinds)
+        if not saved.return_stream:
             grad_y = None
         if grad_h is None and grad_y is None:
-            return (None,) * 13
+            return (None,) * 14
         if grad_h is None:
             grad_h = torch.zeros(ctx.shape, dtype=ctx.dtype, device=t[5].device)
         got = residual_norm_backward(grad_h, grad_y, saved, ctx.needs_input_grad[2:7])
-        return (got["x"], got["block"]) + tuple(got[k] for k in PARAMS) + (None,) * 6
+        return (got["x"], got["block"]) + tuple(got[k] for k in PARAMS) + (None,) * 7
 
 
 def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", pre_weight: Optional[torch.Tensor] = None,
                   pre_bias: Optional[torch.Tensor] = None, post: Optional[str] = None, post_weight: Optional[torch.Tensor] = None,
                   post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
                   eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False):
-    """The step with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
+    """``residual_norm_forward`` with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
     alone comes as it is, several as a tuple."""
+    box = []
     out = _ResidualNorm.apply(x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, float(residual_scale), float(eps),
-                              return_stream, checkpoint_output)
-    if checkpoint_output:
-        out = out[:-2] + (Act8(out[-2], out[-1], x.shape, x.dtype),)
-    return out[0] if len(out) == 1 else out
+                              return_stream, checkpoint_output, box)
+    if not checkpoint_output:
+        return out
+    return (out if return_stream else (out,)) + (box[0],)

@@ -305,3 +305,17 @@ def test_weight_grad_fp16_over_its_whole_range():
     x[0, :32], x[1, 32:] = 1e5, 1.0                          # beyond fp16: the group is NaN, the others are not
     dw, _ = act8.weight_grad(eye[:2, :2].cuda(), act8.Act8(*(lambda h: (h.codes, h.scales))(act8.pack(x.cuda())), (2, 64), FP16))
     assert dw[0, :32].isnan().all() and (dw[1, 32:] == 1).all()
+
+
+def test_weight_grad_with_a_cold_cache():
+    """Loads that miss L2 land out of order: the stages' barriers have to keep the steps apart, over runs that end inside a tile."""
+    x, g = rand(8192, 1024, dtype=BF16, seed=29), rand(8192, 512, dtype=BF16, seed=30)
+    held = act8.pack(x)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    want, _ = act8.weight_grad(g, held, dtype=FP32)
+    ref = g.double().t() @ held_value(x.cpu()).cuda()
+    assert ((want.double() - ref).norm() / ref.norm()).item() < 2e-6
+    for _ in range(12):
+        flush.zero_()
+        assert torch.equal(act8.weight_grad(g, held, dtype=FP32)[0], want)
+    act8.check()
