@@ -31,12 +31,19 @@ __device__ __forceinline__ unsigned act8_scale_byte(unsigned top_bits) {   // bi
 __device__ __forceinline__ float act8_inverse(unsigned s) { return __uint_as_float(s == 255u ? 0u : (254u - s) << 23); }
 __device__ __forceinline__ float act8_step(unsigned s) { return __uint_as_float(s == 255u ? 0x7fffffffu : s << 23); }
 
+__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN where either is one (its sign bit clear)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Eight values of a group whose other 24 are held by the neighbouring three lanes (lanes 4i .. 4i + 3, all of them
 // active): their codes, and the group's scale byte.
 __device__ __forceinline__ uint2 act8_encode(const float (&v)[8], unsigned& s) {
-  unsigned top = 0;
+  float m = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);   // as integers: a NaN is the largest
+  for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+  unsigned top = __float_as_uint(m);     // from here on as integers: a NaN is the largest
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   s = act8_scale_byte(top);
@@ -73,6 +80,22 @@ template <> __device__ __forceinline__ float from_f32(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
 
+// two neighbours in a register: one or two instructions each way
+template <class T> __device__ __forceinline__ float2 unpack2(unsigned w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <class T> __device__ __forceinline__ unsigned pack2(float lo, float hi);
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+template <> __device__ __forceinline__ unsigned pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+
 template <class T> struct Chunk8 {   // 16-bit types: 16 bytes
   uint4 w;
   __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }
@@ -89,19 +112,13 @@ template <class T> struct Chunk8 {   // 16-bit types: 16 bytes
     const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const unsigned short lo = (unsigned short)(u[j] & 0xffffu), hi = (unsigned short)(u[j] >> 16);
-      v[2 * j] = to_f32<T>(*reinterpret_cast<const T*>(&lo));
-      v[2 * j + 1] = to_f32<T>(*reinterpret_cast<const T*>(&hi));
+      const float2 f = unpack2<T>(u[j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
     }
   }
   __device__ __forceinline__ void set(const float (&v)[8]) {
-    unsigned u[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      T lo = from_f32<T>(v[2 * j]), hi = from_f32<T>(v[2 * j + 1]);
-      u[j] = bits(lo) | bits(hi) << 16;
-    }
-    w = make_uint4(u[0], u[1], u[2], u[3]);
+    w = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
   }
 };
 template <> struct Chunk8<float> {   // 32 bytes

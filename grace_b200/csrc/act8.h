@@ -48,8 +48,8 @@ struct BlockNormArgs {
   float alpha, eps;
   long long gate_rows;       // rows of a sequence with a gate of its own; 0: one gate for all rows, or none
   const void *pre_weight, *pre_bias, *post_weight, *post_bias, *gate;   // null: ones, zeros, ones, zeros, no gate
-  Held held_y, held_b, held_h;   // held_b: with N_post or a gate; held_h: on request; codes null: not kept (pitch still set)
-  float* stats;              // [rows][4]: mean and rstd of y, mean and rstd of block; null: not kept
+  Held held_y, held_b, held_h;   // held_b: with N_post or a gate; held_h: on request; their codes null: not kept
+  float* stats;              // [rows][4]: mean and rstd of y, mean and rstd of block
   // forward
   const void *x, *block;
   long long x_stride, block_stride;
@@ -59,7 +59,7 @@ struct BlockNormArgs {
   long long grad_h_stride, grad_y_stride;
   void *dx, *dblock;         // contiguous; dx null: it equals dblock
   void *pre_weight_grad, *pre_bias_grad, *post_weight_grad, *post_bias_grad, *gate_grad;   // null: not wanted
-  float* sums;               // [runs * rpb][4][pitch] scratch (BlockNormShape)
+  float* sums;               // [runs of the backward pass][4][pitch] scratch (BlockNormShape)
   // filled in by the launchers
   bool x_vec, block_vec, out_vec, grad_h_vec, grad_y_vec, param_vec;
   int parts;
@@ -69,8 +69,8 @@ struct BlockNormShape {
   int vpt, tpr, rpb;         // chunks of eight columns a thread, threads a row, rows a CTA
   int sequences, parts, runs;
 };
-BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms);
-cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, cudaStream_t stream);
+BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward);
+cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
 cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
 
 }  // namespace grace

@@ -343,21 +343,20 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
   // ---- residual and norm step between two blocks ----
   m.attr("BLOCK_NORM_MAX_COLS") = (int)kBlockNormMaxCols;
   m.def("block_norm_sum_rows", [](long long rows, int cols, long long gate_rows, int sms) {
-    const BlockNormShape s = block_norm_shape(rows, cols, gate_rows, sms);
-    return (long long)s.runs * s.rpb;
+    return (long long)block_norm_shape(rows, cols, gate_rows, sms, true).runs;
   });
   // params: pre_weight, pre_bias, post_weight, post_bias, gate; held: codes and scales of y, block and h
   m.def("block_norm_forward",
         [](uintptr_t x, long long x_stride, uintptr_t block, long long block_stride, uintptr_t h, uintptr_t y, uintptr_t stats,
            long long rows, int cols, int dtype, int pre, int post, int params_f32, float alpha, float eps, long long gate_rows,
-           const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 6>& helds, int pitch, int spitch, uintptr_t stream) {
+           const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 6>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
           BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, eps, gate_rows, params, stats);
           a.held_y = held(helds[0], helds[1], pitch, spitch);
           a.held_b = held(helds[2], helds[3], pitch, spitch);
           a.held_h = held(helds[4], helds[5], pitch, spitch);
           a.x = ptr<const void>(x); a.x_stride = x_stride; a.block = ptr<const void>(block); a.block_stride = block_stride;
           a.h = ptr<void>(h); a.y = ptr<void>(y);
-          check(launch_block_norm_forward(a, dtype, reinterpret_cast<cudaStream_t>(stream)), "block_norm_forward");
+          check(launch_block_norm_forward(a, dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_forward");
         });
   // grads: of params, in their order
   m.def("block_norm_backward",

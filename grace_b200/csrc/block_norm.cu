@@ -15,10 +15,12 @@
 //
 // Both passes are bound by memory: forward 4 tensors of the type's width and 1 or 2 checkpoints, 10 bytes an element for
 // bf16 with everything, backward the same; 7 and 5 for "add and norm" alone, whose stream nobody reads.  A row is held
-// in registers, eight columns a thread (16 columns in the backward pass beyond 4096), by one warp or several, so that
-// the mean, the squared deviations from it and the results take one pass over memory; small rows share a CTA.  Sums
-// over tokens: a CTA walks a run of rows of one sequence with its columns' sums in registers and stores them once; a
-// second kernel adds the runs' sums in a fixed order (no atomics: the same bits on every run).
+// in registers, eight columns a thread (16 in the backward pass beyond 4096), by one warp or several, so that statistics
+// and results take one pass over memory; small rows share a CTA.  A CTA walks a run of rows that belong to one
+// sequence: its parameters and its gate stay in shared memory (fetched anew for every row, from L2, they cost three
+// times what the row does), and the next row's loads are under way while this one is reduced and written.
+// Sums over tokens: a CTA keeps its columns' sums in registers over its run and stores them once; a second kernel
+// adds the runs' sums in a fixed order (no atomics: the same bits on every run).
 #include "act8.cuh"
 #include "act8.h"
 #include "common.cuh"
@@ -48,18 +50,58 @@ __device__ __forceinline__ void load_param(const BlockNormArgs& a, const void* p
                                               : (a.params_f32 ? static_cast<const float*>(p)[col + j] : to_f32<T>(static_cast<const T*>(p)[col + j]));
 }
 
+// A row of parameters in shared memory, fp32, for `chunks` chunks of eight columns: the first halves of all chunks, then
+// the second halves, so that a quarter warp's 16-byte accesses are consecutive.
+struct SharedRow {
+  float4* at;
+  int chunks;
+  template <class T>
+  __device__ __forceinline__ void fill(const BlockNormArgs& a, const void* p, float none) const {
+    for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+      float v[8];
+      load_param<T>(a, p, c * 8, none, v);
+      at[c] = make_float4(v[0], v[1], v[2], v[3]);
+      at[chunks + c] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+  __device__ __forceinline__ void get(int chunk, float (&v)[8]) const {
+    const float4 lo = at[chunk], hi = at[chunks + chunk];
+    v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+  }
+};
+
+// The rows of this CTA's run: run = sequence * parts + part, rows [part * L / parts, (part + 1) * L / parts) of the
+// sequence, L = gate_rows (all rows are one sequence where no gate belongs to a sequence).
+struct Run {
+  long long row0, row1, seq;
+};
+__device__ __forceinline__ Run run_of(const BlockNormArgs& a) {
+  const long long run = blockIdx.x, seq = run / a.parts, part = run - seq * a.parts, length = a.gate_rows ? a.gate_rows : a.rows;
+  return {seq * length + part * length / a.parts, seq * length + (part + 1) * length / a.parts, seq};
+}
+template <class T>
+__device__ __forceinline__ const void* gate_of(const BlockNormArgs& a, const Run& run) {
+  if (!a.gate || !a.gate_rows) return a.gate;
+  return static_cast<const char*>(a.gate) + run.seq * a.cols * (a.params_f32 ? 4 : (long long)sizeof(T));
+}
+
 // Sums over the `tpr` threads (whole warps) that share a row, the same value in all of them.  Every thread of the CTA
 // calls it.  The two buffers alternate: a warp cannot be two reductions ahead of another.
 template <int N>
 struct RowSum {
-  float* buf;      // [2][32][N]
+  float* buf;      // [2][64], whatever N is: reductions of one and of two values may alternate
   int parity, tpr;
+  __device__ __forceinline__ float* next() {
+    float* const b = buf + parity * 64;
+    parity ^= 1;
+    return b;
+  }
   __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
     if (tpr == 32) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = tpr >> 5, first = warp / warps * warps;
-    float* const b = buf + parity * 32 * N;
+    float* const b = next();
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) b[warp * N + i] = v[i];
@@ -67,96 +109,188 @@ struct RowSum {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? b[(first + lane) * N + i] : 0.f);
-    parity ^= 1;
   }
 };
+
+// 1 / sqrt(x): the hardware's estimate and one Newton step
+__device__ __forceinline__ float inv_sqrt(float x) {
+  const float r = rsqrtf(x);
+  return r * fmaf(-0.5f * x * r, r, 1.5f);
+}
+
+// (mean, 1 / deviation) of a row, eight columns a thread.  Layer norm: each warp's mean and squared deviations from it,
+// joined over the warps by Chan, Golub and LeVeque's formula, so that one barrier does and nothing cancels.
+template <bool LAYER>
+__device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int cols, float inv_cols, float eps, RowSum<2>& sum) {
+  const int lane = threadIdx.x & 31, warps = sum.tpr >> 5, warp = threadIdx.x >> 5, first = warp / warps * warps;
+  if (!LAYER) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);   // (columns past the end are zeros)
+    s = warp_sum(s);
+    if (warps > 1) {
+      float* const b = sum.next();
+      if (lane == 0) b[warp] = s;
+      __syncthreads();
+      s = warp_sum(lane < warps ? b[first + lane] : 0.f);
+    }
+    return make_float2(0.f, inv_sqrt(fmaf(s, inv_cols, eps)));
+  }
+  const float n = (float)min(256, max(0, cols - (warp - first) * 256));
+  float m = 0.f, d = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m += v[j];
+  m = n > 0.f ? __fdividef(warp_sum(m), n) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = j < valid ? v[j] - m : 0.f;
+    d = fmaf(x, x, d);
+  }
+  d = warp_sum(d);
+  if (warps > 1) {
+    float* const b = sum.next();
+    if (lane == 0) {
+      b[warp * 2] = m;
+      b[warp * 2 + 1] = d;
+    }
+    __syncthreads();
+    const float nl = lane < warps ? (float)min(256, max(0, cols - lane * 256)) : 0.f;
+    const float ml = lane < warps ? b[(first + lane) * 2] : 0.f;
+    m = warp_sum(nl * ml) * inv_cols;
+    d = warp_sum(lane < warps ? fmaf(nl * (ml - m), ml - m, b[(first + lane) * 2 + 1]) : 0.f);
+  }
+  return make_float2(m, inv_sqrt(fmaf(d, inv_cols, eps)));
+}
 
 __device__ __forceinline__ void put_codes(const Held& h, size_t row, int col, uint2 codes, unsigned s) {
   *reinterpret_cast<uint2*>(h.codes + row * h.pitch + col) = codes;
   if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
 }
 
-__device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int kind, float inv_cols, float eps, RowSum<1>& sum) {
-  float s[1] = {0.f};
-  float mean = 0.f;
-  if (kind == kNormLayer) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] += v[j];   // (columns past the end are zeros)
-    sum(s);
-    mean = s[0] * inv_cols;
-  }
-  s[0] = 0.f;
+// alpha x + n as an fp32 number that rounds to T as the exact sum does.  The fp32 sum itself may round onto the middle
+// between two 16-bit values (one in 2^13 for fp16), whence ties go to even whatever was cut off: there the sum is
+// taken in 64 bits, and the fp32 one moved off the middle towards it.
+template <class T> constexpr unsigned tie_mask() { return sizeof(T) == 4 ? 0u : (__is_same(T, __half) ? 0x1fffu : 0xffffu); }
+template <class T>
+__device__ __forceinline__ void scaled_sum(float alpha, const float (&x)[8], float (&v)[8]) {
+  constexpr unsigned mask = tie_mask<T>(), tie = (mask + 1) >> 1;
+  bool any = false;
+  float y[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float d = j < valid ? v[j] - mean : 0.f;
-    s[0] = fmaf(d, d, s[0]);
+    y[j] = fmaf(alpha, x[j], v[j]);
+    if (mask) any = any || (__float_as_uint(y[j]) & mask) == tie;
   }
-  sum(s);
-  return make_float2(mean, rsqrtf(fmaf(s[0], inv_cols, eps)));
+  if (mask && any) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if ((__float_as_uint(y[j]) & mask) != tie) continue;
+      const double exact = (double)alpha * (double)x[j] + (double)v[j], at = (double)y[j];
+      if (exact != at) y[j] = __uint_as_float(__float_as_uint(y[j]) + ((exact > at) == (at > 0.0) ? 1u : ~0u));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = y[j];
 }
 
-template <class T>
+template <class T, bool PRE_LAYER, int POST>
 __global__ void __launch_bounds__(1024) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
-  __shared__ float buf[2 * 32];
+  __shared__ float buf[2 * 64];
+  extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
-  const int col = t * 8, valid = min(8, max(0, a.cols - col));
+  const int col = t * 8, valid = min(8, max(0, a.cols - col)), chunks = a.held_y.pitch / 8;
   const bool owns = col < a.held_y.pitch;      // (threads past the last group of 32 only take part in the sums)
+  const int chunk = owns ? t : 0;
   const float inv_cols = 1.f / (float)a.cols;
-  const long long row = (long long)blockIdx.x * rpb + lane_row;
-  const bool in = row < a.rows;
-  RowSum<1> sum{buf, 0, tpr};
+  const Run run = run_of(a);
+  RowSum<2> sum{buf, 0, tpr};
   Chunk8<T> cb, cx;
-  cb.zero();
-  cx.zero();
-  if (in) {
-    load_chunk(cb, static_cast<const T*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
-    load_chunk(cx, static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols, a.x_vec);
-  }
-  float v[8], w[8], x[8];
-  cb.get(v);
-  unsigned s;
-  if (a.held_b.codes) {
-    const uint2 codes = act8_encode(v, s);
-    if (in && owns) put_codes(a.held_b, row, col, codes, s);
-  }
-  float2 post = make_float2(0.f, 1.f);
-  if (a.post != kNormNone) {
-    post = row_stats(v, valid, a.post, inv_cols, a.eps, sum);
-    load_param<T>(a, a.post_weight, col, 1.f, w);
-    load_param<T>(a, a.post_bias, col, 0.f, x);
+  auto load = [&](long long row) {
+    cb.zero();
+    cx.zero();
+    if (row < run.row1) {
+      load_chunk(cb, static_cast<const T*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
+      load_chunk(cx, static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols, a.x_vec);
+    }
+  };
+  load(run.row0 + lane_row);
+  int used = 0;
+  auto shared_row = [&](const void* p, float none) {
+    const SharedRow r{params + 2 * chunks * used++, chunks};
+    r.template fill<T>(a, p, none);
+    return r;
+  };
+  const SharedRow pre_w = shared_row(a.pre_weight, 1.f);
+  const SharedRow pre_b = PRE_LAYER ? shared_row(a.pre_bias, 0.f) : pre_w;
+  const SharedRow post_w = POST ? shared_row(a.post_weight, 1.f) : pre_w;
+  const SharedRow post_b = POST == kNormLayer ? shared_row(a.post_bias, 0.f) : pre_w;
+  const SharedRow gate = a.gate ? shared_row(gate_of<T>(a, run), 0.f) : pre_w;
+  __syncthreads();
+
+  for (long long base = run.row0; base < run.row1; base += rpb) {
+    const long long row = base + lane_row;
+    const bool in = row < run.row1;
+    float v[8], w[8], x[8];
+    cb.get(v);
+    cx.get(x);
+    load(row + rpb);
+    unsigned s;
+    if (a.held_b.codes) {
+      const uint2 codes = act8_encode(v, s);
+      if (in && owns) put_codes(a.held_b, row, col, codes, s);
+    }
+    float2 post = make_float2(0.f, 1.f);
+    if (POST) {
+      post = row_stats<POST == kNormLayer>(v, valid, a.cols, inv_cols, a.eps, sum);
+      post_w.get(chunk, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fmaf((v[j] - post.x) * post.y, w[j], x[j]);
-  }
-  if (a.gate) {
-    const char* gate = static_cast<const char*>(a.gate);
-    if (in && a.gate_rows) gate += (row / a.gate_rows) * a.cols * (a.params_f32 ? 4 : sizeof(T));
-    load_param<T>(a, gate, col, 0.f, w);
+      for (int j = 0; j < 8; ++j) v[j] = (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y * w[j];
+      if (POST == kNormLayer) {
+        post_b.get(chunk, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= w[j];
-  }
-  cx.get(x);
+        for (int j = 0; j < 8; ++j) v[j] += w[j];
+      }
+    }
+    if (a.gate) {
+      gate.get(chunk, w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < valid ? fmaf(a.alpha, x[j], v[j]) : 0.f;
-  cx.set(v);       // the stream as it is rounded to its type
-  cx.get(v);
-  if (in && a.y) store_chunk(v, static_cast<T*>(a.y) + row * a.cols, col, a.cols, a.out_vec);
-  {
-    const uint2 codes = act8_encode(v, s);
-    if (in && owns && a.held_y.codes) put_codes(a.held_y, row, col, codes, s);
-  }
-  const float2 pre = row_stats(v, valid, a.pre, inv_cols, a.eps, sum);
-  load_param<T>(a, a.pre_weight, col, 1.f, w);
-  load_param<T>(a, a.pre_bias, col, 0.f, x);
+      for (int j = 0; j < 8; ++j) v[j] *= w[j];
+    }
+    scaled_sum<T>(a.alpha, x, v);
+    if (valid < 8) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = j < valid ? fmaf((v[j] - pre.x) * pre.y, w[j], x[j]) : 0.f;
-  if (in) store_chunk(v, static_cast<T*>(a.h) + row * a.cols, col, a.cols, a.out_vec);
-  if (a.held_h.codes) {
-    cx.set(v);
-    cx.get(v);
-    const uint2 codes = act8_encode(v, s);
-    if (in && owns) put_codes(a.held_h, row, col, codes, s);
+      for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] : 0.f;
+    }
+    Chunk8<T> cy;
+    cy.set(v);       // the stream as it is rounded to its type
+    cy.get(v);
+    if (in && a.y) store_chunk(v, static_cast<T*>(a.y) + row * a.cols, col, a.cols, a.out_vec);
+    {
+      const uint2 codes = act8_encode(v, s);
+      if (in && owns) put_codes(a.held_y, row, col, codes, s);
+    }
+    const float2 pre = row_stats<PRE_LAYER>(v, valid, a.cols, inv_cols, a.eps, sum);
+    pre_w.get(chunk, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (PRE_LAYER ? v[j] - pre.x : v[j]) * pre.y * w[j];
+    if (PRE_LAYER) {
+      pre_b.get(chunk, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += w[j];
+    }
+    if (in) store_chunk(v, static_cast<T*>(a.h) + row * a.cols, col, a.cols, a.out_vec);
+    if (a.held_h.codes) {
+      if (valid < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] : 0.f;
+      }
+      cy.set(v);
+      cy.get(v);
+      const uint2 codes = act8_encode(v, s);
+      if (in && owns) put_codes(a.held_h, row, col, codes, s);
+    }
+    if (in && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(pre.x, pre.y, post.x, post.y);
   }
-  if (in && t == 0 && a.stats) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(pre.x, pre.y, post.x, post.y);
 }
 
 // What a thread loads of a row: eight columns.
@@ -184,202 +318,225 @@ struct RowLoads {
   }
 };
 
-// A CTA walks the rows of one run: run = sequence * parts + part, rows [part * L / parts, (part + 1) * L / parts) of the
-// sequence, L = a.gate_rows (all rows are one sequence where no gate belongs to a sequence).  VPT chunks of eight columns
-// a thread, tpr * 8 columns apart.  TWO: N_post or a gate, so that b~ is read.
-template <class T, int VPT, bool TWO>
+// (value - mean) * rstd of eight held values; the difference first: a mean far from zero must not cost digits
+template <bool LAYER>
+__device__ __forceinline__ void decode_normed(uint2 codes, unsigned s, float mean, float rstd, float (&v)[8]) {
+  act8_decode(codes, s, v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (LAYER ? v[j] - mean : v[j]) * rstd;
+}
+
+// VPT chunks of eight columns a thread, tpr * 8 columns apart.  BLOCK: 0 neither a norm after the block nor a gate, so that
+// b~ is not read; 1 either, without sums of g (G0); 2 with them (a layer norm after the block).
+template <class T, int VPT, bool PRE_LAYER, int BLOCK>
 __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNormArgs a, int tpr) {
-  __shared__ float buf[2 * 32 * 2];
+  constexpr bool TWO = BLOCK > 0;
+  constexpr int B = TWO ? VPT : 1, L = PRE_LAYER ? VPT : 1, Z = BLOCK == 2 ? VPT : 1;
+  __shared__ float buf[2 * 64];
+  extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
+  const int chunks = a.held_y.pitch / 8;
   const float inv_cols = 1.f / (float)a.cols;
-  const long long run = blockIdx.x, seq = run / a.parts, part = run - seq * a.parts;
-  const long long length = a.gate_rows ? a.gate_rows : a.rows;
-  const long long row0 = seq * length + part * length / a.parts, row1 = seq * length + (part + 1) * length / a.parts;
-  RowSum<2> sum{buf, 0, tpr};
-  const bool post = TWO && a.post != kNormNone, layer = a.pre == kNormLayer, post_layer = a.post == kNormLayer;
-  float dw[VPT][8] = {}, db[VPT][8] = {}, g1[TWO ? VPT : 1][8] = {}, g0[TWO ? VPT : 1][8] = {};
-  const char* gate = static_cast<const char*>(a.gate);
-  if (gate && a.gate_rows) gate += seq * a.cols * (a.params_f32 ? 4 : (int)sizeof(T));
+  const Run run = run_of(a);
+  RowSum<2> sum2{buf, 0, tpr};
+  RowSum<1> sum1{buf, 0, tpr};
+  const bool post = TWO && a.post != kNormNone;
+  float dw[VPT][8] = {}, db[L][8] = {}, g1[B][8] = {}, g0[Z][8] = {};
 
   RowLoads<T, TWO> r[VPT];
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-  {
-    const long long row = row0 + lane_row;
-    const bool in = row < row1;
+  auto load = [&](long long row) {
+    const bool in = row < run.row1;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) r[i].load(a, row, (i * tpr + t) * 8, in);
-    if (in) st = __ldg(reinterpret_cast<const float4*>(a.stats + row * 4));
-  }
-  for (long long base = row0; base < row1; base += rpb) {
+    st = in ? __ldg(reinterpret_cast<const float4*>(a.stats + row * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(run.row0 + lane_row);
+  int used = 0;
+  auto shared_row = [&](const void* p, float none) {
+    const SharedRow r{params + 2 * chunks * used++, chunks};
+    r.template fill<T>(a, p, none);
+    return r;
+  };
+  const SharedRow pre_w = shared_row(a.pre_weight, 1.f);
+  const SharedRow post_w = post ? shared_row(a.post_weight, 1.f) : pre_w;
+  const SharedRow gate = a.gate ? shared_row(gate_of<T>(a, run), 0.f) : pre_w;
+  __syncthreads();
+
+  for (long long base = run.row0; base < run.row1; base += rpb) {
     const long long row = base + lane_row;
-    const bool in = row < row1;
-    float c[VPT][8], hat[VPT][8], bh[TWO ? VPT : 1][8];
+    const bool in = row < run.row1;
+    float c[VPT][8], hat[VPT][8], bh[B][8];
     Chunk8<T> dy[VPT];
     float s[2] = {0.f, 0.f};
     const float4 stats = st;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int col = (i * tpr + t) * 8;
+      const int k = i * tpr + t, chunk = k < chunks ? k : 0;
       float w[8], d[8];
       r[i].dh.get(d);
-      act8_decode(r[i].qy, r[i].sy, hat[i]);
-      load_param<T>(a, a.pre_weight, col, 1.f, w);
+      decode_normed<PRE_LAYER>(r[i].qy, r[i].sy, stats.x, stats.y, hat[i]);
+      pre_w.get(chunk, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        hat[i][j] = (hat[i][j] - stats.x) * stats.y;
         dw[i][j] = fmaf(d[j], hat[i][j], dw[i][j]);
-        db[i][j] += d[j];
         c[i][j] = d[j] * w[j];
-        s[0] += c[i][j];
-        s[1] = fmaf(c[i][j], hat[i][j], s[1]);
+        s[0] = fmaf(c[i][j], hat[i][j], s[0]);
+        if (PRE_LAYER) {
+          db[PRE_LAYER ? i : 0][j] += d[j];
+          s[1] += c[i][j];
+        }
       }
       dy[i] = r[i].dy;
-      if (TWO) {
-        act8_decode(r[i].qb, r[i].sb, bh[TWO ? i : 0]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bh[TWO ? i : 0][j] = (bh[TWO ? i : 0][j] - stats.z) * stats.w;
+      if (TWO) decode_normed<BLOCK == 2>(r[i].qb, r[i].sb, stats.z, stats.w, bh[TWO ? i : 0]);
+    }
+    load(row + rpb);     // the next row's loads are under way during the sums
+    auto row_sum = [&](bool both) {
+      if (both) {
+        sum2(s);
+      } else {
+        float v[1] = {s[0]};
+        sum1.parity = sum2.parity;   // (the two share their buffers)
+        sum1(v);
+        s[0] = v[0];
+        sum2.parity = sum1.parity;
       }
-    }
-    {   // the next row's loads are under way during the sums
-      const bool next = row + rpb < row1;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) r[i].load(a, row + rpb, (i * tpr + t) * 8, next);
-      st = next ? __ldg(reinterpret_cast<const float4*>(a.stats + (row + rpb) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    sum(s);
-    const float m0 = layer ? s[0] * inv_cols : 0.f, m1 = s[1] * inv_cols;
+    };
+    row_sum(PRE_LAYER);
+    const float m1 = s[0] * inv_cols, m0 = PRE_LAYER ? s[1] * inv_cols : 0.f;
     s[0] = s[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int col = (i * tpr + t) * 8;
+      const int k = i * tpr + t, chunk = k < chunks ? k : 0, col = k * 8;
       float d[8], w[8];
       dy[i].get(d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[i][j] = fmaf(stats.y, c[i][j] - m0 - hat[i][j] * m1, d[j]);   // g
+      for (int j = 0; j < 8; ++j) c[i][j] = fmaf(stats.y, fmaf(-hat[i][j], m1, PRE_LAYER ? c[i][j] - m0 : c[i][j]), d[j]);   // g
       if (in && a.dx) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] = a.alpha * c[i][j];
         store_chunk(d, static_cast<T*>(a.dx) + row * a.cols, col, a.cols, a.out_vec);
       }
       if (TWO) {
-        constexpr int z = TWO ? 1 : 0;
-        const bool some = in;   // a row that does not exist adds nothing
+        if (!in || col + 8 > a.cols) {   // what does not exist adds nothing
+#pragma unroll
+          for (int j = 0; j < 8; ++j) c[i][j] = in && col + j < a.cols ? c[i][j] : 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float g = some && col + j < a.cols ? c[i][j] : 0.f;
-          g1[i * z][j] = fmaf(g, bh[i * z][j], g1[i * z][j]);
-          g0[i * z][j] += g;
-          c[i][j] = g;
+          g1[TWO ? i : 0][j] = fmaf(c[i][j], bh[TWO ? i : 0][j], g1[TWO ? i : 0][j]);
+          if (BLOCK == 2) g0[BLOCK == 2 ? i : 0][j] += c[i][j];
         }
-        if (gate) {
-          load_param<T>(a, gate, col, 0.f, w);
+        if (a.gate) {
+          gate.get(chunk, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) c[i][j] *= w[j];
         }
         if (post) {
-          load_param<T>(a, a.post_weight, col, 1.f, w);
+          post_w.get(chunk, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             c[i][j] *= w[j];
-            s[0] += c[i][j];
-            s[1] = fmaf(c[i][j], bh[i * z][j], s[1]);
+            s[0] = fmaf(c[i][j], bh[TWO ? i : 0][j], s[0]);
+            if (BLOCK == 2) s[1] += c[i][j];
           }
         }
       }
     }
-    float p0 = 0.f, p1 = 0.f;
     if (post) {
-      sum(s);
-      p0 = post_layer ? s[0] * inv_cols : 0.f;
-      p1 = s[1] * inv_cols;
+      row_sum(BLOCK == 2);
+      const float p1 = s[0] * inv_cols, p0 = BLOCK == 2 ? s[1] * inv_cols : 0.f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[i][j] = stats.w * fmaf(-bh[TWO ? i : 0][j], p1, BLOCK == 2 ? c[i][j] - p0 : c[i][j]);
     }
     if (in) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int col = (i * tpr + t) * 8;
-        if (post) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) c[i][j] = stats.w * (c[i][j] - p0 - bh[TWO ? i : 0][j] * p1);
-        }
-        store_chunk(c[i], static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
-      }
+      for (int i = 0; i < VPT; ++i) store_chunk(c[i], static_cast<T*>(a.dblock) + row * a.cols, (i * tpr + t) * 8, a.cols, a.out_vec);
     }
   }
-  // this run's sums: [4][pitch] floats for each row lane of the CTA
-  if (a.sums) {
-    float* const out = a.sums + (run * rpb + lane_row) * 4 * (long long)a.held_y.pitch;
+  if (!a.sums) return;
+  // This run's sums: [4][pitch] floats.  The CTA's row lanes are added in order, each on top of the one before it.
+  const long long pitch = a.held_y.pitch;
+  float4* const out = reinterpret_cast<float4*>(a.sums + (long long)blockIdx.x * 4 * pitch);
+  float4* const part = params;                       // the parameters are not needed any more
+  constexpr int kSums = 1 + (PRE_LAYER ? 1 : 0) + (TWO ? 1 : 0) + (BLOCK == 2 ? 1 : 0);
+  for (int l = 0; l < rpb; ++l) {
+    __syncthreads();
+    if (lane_row != l) continue;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int col = (i * tpr + t) * 8;
-      if (col >= a.held_y.pitch) continue;
-      auto put = [&](int which, const float (&v)[8]) {
-        float4* p = reinterpret_cast<float4*>(out + (long long)which * a.held_y.pitch + col);
-        p[0] = make_float4(v[0], v[1], v[2], v[3]);
-        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+      const int k = i * tpr + t;
+      if (k >= chunks) continue;
+      int n = 0;
+      auto put = [&](int which, float (&v)[8]) {
+        float4* const p = part + (long long)n * 2 * chunks + k;     // first halves, then second halves of the chunks
+        ++n;
+        if (l > 0) {
+          const float4 x = p[0], y = p[chunks];
+          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+        }
+        const float4 x = make_float4(v[0], v[1], v[2], v[3]), y = make_float4(v[4], v[5], v[6], v[7]);
+        if (l + 1 < rpb) {
+          p[0] = x;
+          p[chunks] = y;
+        } else {
+          out[which * (pitch / 4) + k * 2] = x;
+          out[which * (pitch / 4) + k * 2 + 1] = y;
+        }
       };
       put(0, dw[i]);
-      if (layer) put(1, db[i]);
-      if (TWO) {
-        put(2, g1[TWO ? i : 0]);
-        put(3, g0[TWO ? i : 0]);
-      }
+      if (PRE_LAYER) put(1, db[PRE_LAYER ? i : 0]);
+      if (TWO) put(2, g1[TWO ? i : 0]);
+      if (BLOCK == 2) put(3, g0[BLOCK == 2 ? i : 0]);
     }
   }
+  static_assert(kSums <= 4, "see backward_smem");
 }
 
-// Adds the runs' sums.  Block: 32 columns x 8 lanes of runs.  blockIdx.y 0: the norms' parameters, over all runs; 1 + s:
-// the gate of sequence s.
-constexpr int kLanes = 8;
+// Adds the runs' sums.  Block: 32 columns x 32 lanes of runs.  blockIdx.y 0 .. 3: one of the norms' parameters, over all
+// runs; 4 + s: the gate of sequence s.
+constexpr int kLanes = 32;
 template <class T>
-__global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const BlockNormArgs a, int sum_rows, int gates) {
-  __shared__ float part[4][kLanes][33];
+__global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const BlockNormArgs a, int runs, int gates) {
+  __shared__ float part[2][kLanes][33];
   const int col = blockIdx.x * 32 + threadIdx.x, lane = threadIdx.y;
   const long long pitch = a.held_y.pitch;
-  const bool for_gate = blockIdx.y > 0;
-  const long long seq = (long long)blockIdx.y - 1;
-  const long long runs = (long long)sum_rows;                         // rows of sums in all
-  const long long per_gate = runs / gates;
-  const long long first = for_gate ? seq * per_gate : 0, last = for_gate ? first + per_gate : runs;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (long long u = first + lane; u < last; u += kLanes) {
-    const float* p = a.sums + u * 4 * pitch + col;
-    float g = 1.f;
-    if (!for_gate) {
-      if (a.pre_weight_grad) v[0] += p[0];
-      if (a.pre_bias_grad) v[1] += p[pitch];
-      if (a.gate && col < a.cols) {
-        const long long at = a.gate_rows ? u / per_gate * a.cols + col : col;
-        g = a.params_f32 ? static_cast<const float*>(a.gate)[at] : to_f32<T>(static_cast<const T*>(a.gate)[at]);
-      }
-    }
-    if (for_gate || a.post_weight_grad) v[2] = fmaf(g, p[2 * pitch], v[2]);
-    if (for_gate ? a.post_bias != nullptr : a.post_bias_grad != nullptr) v[3] = fmaf(g, p[3 * pitch], v[3]);
+  const bool for_gate = blockIdx.y >= 4;
+  const int seq = (int)blockIdx.y - 4, per_gate = runs / gates, which = for_gate ? 2 : (int)blockIdx.y;
+  void* const grads[4] = {a.pre_weight_grad, a.pre_bias_grad, a.post_weight_grad, a.post_bias_grad};
+  if (!for_gate && grads[which] == nullptr) return;
+  const int first = for_gate ? seq * per_gate : 0, last = for_gate ? first + per_gate : runs;
+  const bool second = for_gate && a.post_bias;
+  auto param = [&](const void* p, long long at) {
+    return a.params_f32 ? static_cast<const float*>(p)[at] : to_f32<T>(static_cast<const T*>(p)[at]);
+  };
+  const bool weigh = !for_gate && which >= 2 && a.gate && col < a.cols;     // sum of gate * G over the sequences
+  cudaGridDependencySynchronize();
+  float v = 0.f, z = 0.f;
+  const float* p = a.sums + (long long)(first + lane) * 4 * pitch + which * pitch + col;
+#pragma unroll 4
+  for (int u = first + lane; u < last; u += kLanes, p += kLanes * 4 * pitch) {
+    float x = *p;
+    if (weigh && a.gate_rows) x *= param(a.gate, (long long)(u / per_gate) * a.cols + col);
+    v += x;
+    if (second) z += p[pitch];
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[i][lane][threadIdx.x] = v[i];
+  part[0][lane][threadIdx.x] = v;
+  part[1][lane][threadIdx.x] = z;
   __syncthreads();
-  if (lane != 0 || col >= a.cols) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = 0.f;
-    for (int l = 0; l < kLanes; ++l) v[i] += part[i][l][threadIdx.x];
-  }
-  auto put = [&](void* p, long long at, float x) {
-    if (!p) return;
-    if (a.params_f32) static_cast<float*>(p)[at] = x;
-    else static_cast<T*>(p)[at] = from_f32<T>(x);
+  // a warp for each of the block's columns
+  const int c = threadIdx.y, at = blockIdx.x * 32 + c;
+  v = warp_sum(part[0][threadIdx.x][c]);
+  z = warp_sum(part[1][threadIdx.x][c]);
+  if (threadIdx.x != 0 || at >= a.cols) return;
+  auto put = [&](void* to, long long i, float x) {
+    if (a.params_f32) static_cast<float*>(to)[i] = x;
+    else static_cast<T*>(to)[i] = from_f32<T>(x);
   };
-  auto get = [&](const void* p, float none) {
-    return p == nullptr ? none : (a.params_f32 ? static_cast<const float*>(p)[col] : to_f32<T>(static_cast<const T*>(p)[col]));
-  };
-  if (for_gate) {
-    put(a.gate_grad, seq * a.cols + col, get(a.post_weight, 1.f) * v[2] + get(a.post_bias, 0.f) * v[3]);
-  } else {
-    put(a.pre_weight_grad, col, v[0]);
-    put(a.pre_bias_grad, col, v[1]);
-    put(a.post_weight_grad, col, v[2]);
-    put(a.post_bias_grad, col, v[3]);
-  }
+  if (for_gate) put(a.gate_grad, (long long)seq * a.cols + at, (a.post_weight ? param(a.post_weight, at) : 1.f) * v + (second ? param(a.post_bias, at) * z : 0.f));
+  else put(grads[which], at, weigh && !a.gate_rows ? v * param(a.gate, at) : v);
 }
 
 bool aligned(const void* p, long long stride, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * es % 16 == 0; }
@@ -391,16 +548,56 @@ bool params_aligned(const BlockNormArgs& a) {
   return a.cols % 8 == 0;
 }
 
+template <class K>
+cudaError_t launch_shared(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const BlockNormArgs& a, int tpr) {
+  if (smem > 40 * 1024) {   // (48 KB with the static part need no leave)
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) return err;
+  }
+  kernel<<<grid, block, smem, stream>>>(a, tpr);
+  return cudaGetLastError();
+}
+
 template <class T>
-cudaError_t forward_typed(BlockNormArgs a, cudaStream_t stream) {
+cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   a.x_vec = aligned(a.x, a.x_stride, sizeof(T));
   a.block_vec = aligned(a.block, a.block_stride, sizeof(T));
   a.out_vec = aligned(a.h, a.cols, sizeof(T)) && aligned(a.y, a.cols, sizeof(T));
   a.param_vec = params_aligned(a);
-  const int tpr = (a.held_y.pitch / 8 + 31) / 32 * 32, rpb = tpr >= 256 ? 1 : 256 / tpr;
-  const long long grid = (a.rows + rpb - 1) / rpb;
-  block_norm_forward_kernel<T><<<(unsigned)grid, tpr * rpb, 0, stream>>>(a, tpr);
-  return cudaGetLastError();
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, false);
+  a.parts = shape.parts;
+  const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
+  const bool layer = a.pre == kNormLayer;
+  const int rows = 1 + (layer ? 1 : 0) + (a.post ? 1 : 0) + (a.post == kNormLayer ? 1 : 0) + (a.gate ? 1 : 0);
+  const size_t smem = (size_t)rows * a.held_y.pitch * 4;
+  switch (a.post * 2 + (layer ? 1 : 0)) {
+    case 0: return launch_shared(block_norm_forward_kernel<T, false, kNormNone>, grid, block, smem, stream, a, shape.tpr);
+    case 1: return launch_shared(block_norm_forward_kernel<T, true, kNormNone>, grid, block, smem, stream, a, shape.tpr);
+    case 2: return launch_shared(block_norm_forward_kernel<T, false, kNormRms>, grid, block, smem, stream, a, shape.tpr);
+    case 3: return launch_shared(block_norm_forward_kernel<T, true, kNormRms>, grid, block, smem, stream, a, shape.tpr);
+    case 4: return launch_shared(block_norm_forward_kernel<T, false, kNormLayer>, grid, block, smem, stream, a, shape.tpr);
+    default: return launch_shared(block_norm_forward_kernel<T, true, kNormLayer>, grid, block, smem, stream, a, shape.tpr);
+  }
+}
+
+template <class T, int VPT>
+cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape, cudaStream_t stream) {
+  const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
+  const int form = a.held_b.codes == nullptr ? 0 : (a.post == kNormLayer ? 2 : 1);
+  const bool layer = a.pre == kNormLayer;
+  // the parameters, or (several row lanes) the sums on their way from lane to lane
+  int rows = 1 + (a.post ? 1 : 0) + (a.gate ? 1 : 0);
+  const int sums = 1 + (layer ? 1 : 0) + form;
+  if (shape.rpb > 1 && sums > rows) rows = sums;
+  const size_t smem = (size_t)rows * a.held_y.pitch * 4;
+  switch (form * 2 + (layer ? 1 : 0)) {
+    case 0: return launch_shared(block_norm_backward_kernel<T, VPT, false, 0>, grid, block, smem, stream, a, shape.tpr);
+    case 1: return launch_shared(block_norm_backward_kernel<T, VPT, true, 0>, grid, block, smem, stream, a, shape.tpr);
+    case 2: return launch_shared(block_norm_backward_kernel<T, VPT, false, 1>, grid, block, smem, stream, a, shape.tpr);
+    case 3: return launch_shared(block_norm_backward_kernel<T, VPT, true, 1>, grid, block, smem, stream, a, shape.tpr);
+    case 4: return launch_shared(block_norm_backward_kernel<T, VPT, false, 2>, grid, block, smem, stream, a, shape.tpr);
+    default: return launch_shared(block_norm_backward_kernel<T, VPT, true, 2>, grid, block, smem, stream, a, shape.tpr);
+  }
 }
 
 template <class T>
@@ -410,32 +607,28 @@ cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, cudaStr
   a.out_vec = aligned(a.dblock, a.cols, sizeof(T)) && aligned(a.dx, a.cols, sizeof(T));
   a.param_vec = params_aligned(a);
   a.parts = shape.parts;
-  const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
-  const bool two = a.held_b.codes != nullptr;
-  if (shape.vpt == 1) {
-    if (two) block_norm_backward_kernel<T, 1, true><<<grid, block, 0, stream>>>(a, shape.tpr);
-    else block_norm_backward_kernel<T, 1, false><<<grid, block, 0, stream>>>(a, shape.tpr);
-  } else {
-    if (two) block_norm_backward_kernel<T, 2, true><<<grid, block, 0, stream>>>(a, shape.tpr);
-    else block_norm_backward_kernel<T, 2, false><<<grid, block, 0, stream>>>(a, shape.tpr);
-  }
-  cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess || !a.sums) return err;
+  const cudaError_t err = shape.vpt == 1 ? backward_launch<T, 1>(a, shape, stream) : backward_launch<T, 2>(a, shape, stream);
   const bool params = a.pre_weight_grad || a.pre_bias_grad || a.post_weight_grad || a.post_bias_grad || a.gate_grad;
-  if (!params) return cudaSuccess;
-  const int gates = a.gate_grad ? shape.sequences : 0;
-  block_norm_sums_kernel<T><<<dim3((a.cols + 31) / 32, 1 + gates), dim3(32, kLanes), 0, stream>>>(a, shape.runs * shape.rpb,
-                                                                                                 shape.sequences);
-  return cudaGetLastError();
+  if (err != cudaSuccess || !a.sums || !params) return err;
+  cudaLaunchConfig_t cfg{};     // (set up while the first kernel still runs; it waits for that one's end before it reads)
+  cfg.gridDim = dim3((a.cols + 31) / 32, 4 + (a.gate_grad ? shape.sequences : 0));
+  cfg.blockDim = dim3(32, kLanes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, block_norm_sums_kernel<T>, a, shape.runs, shape.sequences);
 }
 
 }  // namespace
 
-// How the backward pass covers [rows, cols]: about two CTAs of 512 threads, or four of 256, for each SM.
-BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms) {
+// How a pass covers [rows, cols]: 1024 threads for each SM, a thread eight columns (16 in the backward pass beyond 4096).
+BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward) {
   BlockNormShape s{};
   const int chunks = (cols + 31) / 32 * 4;
-  s.vpt = chunks > 512 ? 2 : 1;
+  s.vpt = backward && chunks > 512 ? 2 : 1;
   s.tpr = ((chunks + s.vpt - 1) / s.vpt + 31) / 32 * 32;
   s.rpb = s.tpr >= 256 ? 1 : 256 / s.tpr;
   const long long length = gate_rows ? gate_rows : rows;
@@ -450,13 +643,13 @@ BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, i
   return s;
 }
 
-cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, cudaStream_t stream) {
+cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
-  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll || !a.stats || !a.held_y.codes) return cudaErrorInvalidValue;
   switch (dtype) {
-    case kGradF32: return forward_typed<float>(a, stream);
-    case kGradBF16: return forward_typed<__nv_bfloat16>(a, stream);
-    case kGradF16: return forward_typed<__half>(a, stream);
+    case kGradF32: return forward_typed<float>(a, sms, stream);
+    case kGradBF16: return forward_typed<__nv_bfloat16>(a, sms, stream);
+    case kGradF16: return forward_typed<__half>(a, sms, stream);
   }
   return cudaErrorInvalidValue;
 }
@@ -464,8 +657,8 @@ cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, cudaStr
 cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
   if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
-  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms);
-  if (shape.sequences > 65534) return cudaErrorInvalidValue;
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, true);
+  if (shape.sequences > 65531) return cudaErrorInvalidValue;
   switch (dtype) {
     case kGradF32: return backward_typed<float>(a, shape, stream);
     case kGradBF16: return backward_typed<__nv_bfloat16>(a, shape, stream);

@@ -28,7 +28,7 @@ from .exchange import GRAD_DTYPE
 NORMS = {None: 0, "rms": 1, "layer": 2}
 MAX_COLS = 8192      # a row is held in the registers of one CTA (block_norm.cu: kBlockNormMaxCols)
 MAX_ROWS = (1 << 31) - 1
-MAX_SEQUENCES = 65534
+MAX_SEQUENCES = 65531
 PARAMS = ("pre_weight", "pre_bias", "post_weight", "post_bias", "gate")
 
 
@@ -122,7 +122,7 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     ptrs, kept = _param_ptrs(params)
     _launch(device, native().block_norm_forward, vx.data_ptr(), vx.stride(0), vb.data_ptr(), vb.stride(0), h.data_ptr(),
             0 if y is None else y.data_ptr(), saved.stats_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params),
-            float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(saved.held_y) + _ptrs(saved.held_block) + _ptrs(held_h), *pitch_of(cols))
+            float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(saved.held_y) + _ptrs(saved.held_block) + _ptrs(held_h), *pitch_of(cols), _sms(device))
     del kept
     return h, y, saved
 
