@@ -7,17 +7,19 @@
 //             gated: x = [a | b], y = f(a) b, checkpoints of a and b      3 es + 2 1/16 (+ 1 1/32), for an element of y
 //   backward  dx = dy f'(x~);  gated: da = dy b~ f'(a~), db = dy f(a~)    2 es + 1 1/32;  3 es + 2 1/16
 //
-// All four are bound by memory: a thread takes chunks of eight neighbouring elements (16 bytes of a 16-bit type in, 8
-// bytes of codes out), four lanes share a group of 32 and agree on its largest magnitude by two shuffles; a thread
+// All four are bound by memory: a thread takes chunks of sixteen neighbouring elements (32 bytes of a 16-bit type in, 16
+// bytes of codes out), two lanes share a group of 32 and agree on its largest magnitude by one shuffle; a thread
 // issues the loads of all its chunks before it computes.  The issue slots are the second limit: at 6.5 TB/s an SM has
-// about 16 of them an element of a bf16 pack and 25 of a forward pass, so the encoder takes one FMA, one clamp and
-// 7/8 of a byte shuffle an element, and the functions take one exponential and one reciprocal.
+// about 16 of them an element of a bf16 pack and 25 of a forward pass, so the encoder takes a maximum, an FMA, a clamp and
+// 3/4 of a byte shuffle an element, and the functions take one exponential and one reciprocal.
 //
 // f is GELU (erf form), GELU (tanh form) or SiLU.  For 16-bit tensors the error function is the rational approximation
 // 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error below 1.5e-7, 2^-22.6: far
 // below half a step of a 16-bit result, 2^-9 or 2^-12 of its value wherever the value is not itself below 2^-10),
 // whose exp(-z^2) is also the density that the derivative needs; the exponential is the hardware's.  For fp32
 // tensors erfc and exp are CUDA's.
+#include <algorithm>
+
 #include "act8.cuh"
 #include "act8.h"
 #include "gradio.cuh"
@@ -44,32 +46,49 @@ __device__ __forceinline__ void divmod(const FastDiv& f, unsigned n, unsigned& q
 }
 
 struct Rows {          // which chunks a launch covers
-  unsigned chunks;     // rows * (pitch / 8), below 2^31; a multiple of 4
-  FastDiv per_row;     // pitch / 8
+  unsigned chunks;     // of sixteen columns: rows * (pitch / 16), below 2^31; a multiple of 2
+  FastDiv per_row;     // pitch / 16
   int cols;
 };
 
-__device__ __forceinline__ void put_held(const Held& h, size_t row, int col, uint2 codes, unsigned s) {
-  *reinterpret_cast<uint2*>(h.codes + row * h.pitch + col) = codes;
+__device__ __forceinline__ void put_held(const Held& h, size_t row, int col, uint4 codes, unsigned s) {
+  *reinterpret_cast<uint4*>(h.codes + row * h.pitch + col) = codes;
   if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
 }
-__device__ __forceinline__ void get_held(const Held& h, size_t row, int col, float (&v)[8]) {
-  const uint2 codes = __ldg(reinterpret_cast<const uint2*>(h.codes + row * h.pitch + col));
-  act8_decode(codes, (unsigned)__ldg(h.scales + row * h.spitch + (col >> 5)), v);
-}
+struct HeldChunk {
+  uint4 codes;
+  unsigned s;
+  __device__ __forceinline__ void load(const Held& h, size_t row, int col) {
+    codes = __ldg(reinterpret_cast<const uint4*>(h.codes + row * h.pitch + col));
+    s = __ldg(h.scales + row * h.spitch + (col >> 5));
+  }
+  __device__ __forceinline__ void get(float (&v)[16]) const { act8_decode(codes, s, v); }
+};
 
 // ---- the functions: f and f' at x ----
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <int KIND, bool FAST>
 __device__ __forceinline__ float2 function(float x) {
-  constexpr float kInvSqrt2Pi = 0.3989422804f;
+  constexpr float kInvSqrt2Pi = 0.3989422804f, kLog2e = 1.4426950409f;
   if (KIND == kActGelu) {
     float p, e;   // p: the normal distribution function, e: exp(-x^2 / 2)
     if (FAST) {
-      const float z = fabsf(x) * 0.70710678f;
-      const float t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-      e = __expf(-z * z);
-      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
-      p = x < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);   // q = erfc(z)
+      const float t = rcp_fast(fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.f));
+      e = exp2_fast(-0.5f * kLog2e * (x * x));
+      const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f),
+                              0.5f * 0.254829592f);
+      const float q = t * poly * e;              // erfc(|x| / sqrt 2) / 2
+      p = x < 0.f ? q : 1.f - q;
     } else {
       e = expf(-0.5f * x * x);
       p = 0.5f * erfcf(-0.70710678f * x);
@@ -80,18 +99,18 @@ __device__ __forceinline__ float2 function(float x) {
     constexpr float c = 0.7978845608f, a = 0.044715f;
     const float xx = fminf(x * x, 1e4f);   // past |x| = 100 the sigmoid is 0 or 1 to the last bit
     const float u = 2.f * c * x * fmaf(a, xx, 1.f);
-    const float p = FAST ? __fdividef(1.f, 1.f + __expf(-u)) : 1.f / (1.f + expf(-u));   // (1 + tanh(u / 2)) / 2
+    const float p = FAST ? rcp_fast(1.f + exp2_fast(-kLog2e * u)) : 1.f / (1.f + expf(-u));   // (1 + tanh(u / 2)) / 2
     return make_float2(x * p, fmaf(2.f * c * x * p * (1.f - p), fmaf(3.f * a, xx, 1.f), p));
   }
-  const float p = FAST ? __fdividef(1.f, 1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+  const float p = FAST ? rcp_fast(1.f + exp2_fast(-kLog2e * x)) : 1.f / (1.f + expf(-x));
   return make_float2(x * p, p * fmaf(x, 1.f - p, 1.f));
 }
 
 // ---- kernels: thread t of a block takes the chunks base + t, base + t + 256, ... (U of them) ----
 template <class T, int U>
-__global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, long long stride, bool vec, Rows r, Held held) {
+__global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, long long stride, int vec, Rows r, Held held) {
   const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
-  Chunk8<T> c[U];
+  Chunk16<T> c[U];
   unsigned row[U], k[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -100,40 +119,47 @@ __global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, l
     c[i].zero();
     if (at < r.chunks) {
       divmod(r.per_row, at, row[i], k[i]);
-      load_chunk(c[i], x + (long long)row[i] * stride, (int)k[i] * 8, r.cols, vec);
+      c[i].load(x + (long long)row[i] * stride, (int)k[i] * 16, r.cols, vec);
     }
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    float v[8];
+    float v[16];
     unsigned s;
     c[i].get(v);
-    const uint2 codes = act8_encode(v, s);
-    if (base + i * kBlock < r.chunks) put_held(held, row[i], (int)k[i] * 8, codes, s);
+    const uint4 codes = act8_encode(v, s);
+    if (base + i * kBlock < r.chunks) put_held(held, row[i], (int)k[i] * 16, codes, s);
   }
 }
 
 template <class T, int U>
-__global__ void __launch_bounds__(kBlock) unpack_kernel(Held held, T* __restrict__ out, long long stride, bool vec, Rows r) {
+__global__ void __launch_bounds__(kBlock) unpack_kernel(Held held, T* __restrict__ out, long long stride, int vec, Rows r) {
   const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
+  HeldChunk c[U];
+  unsigned row[U], k[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const unsigned at = base + i * kBlock;
-    if (at >= r.chunks) return;
-    unsigned row, k;
-    divmod(r.per_row, at, row, k);
-    float v[8];
-    get_held(held, row, (int)k * 8, v);
-    store_chunk(v, out + (long long)row * stride, (int)k * 8, r.cols, vec);
+    if (at < r.chunks) {
+      divmod(r.per_row, at, row[i], k[i]);
+      c[i].load(held, row[i], (int)k[i] * 16);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (base + i * kBlock >= r.chunks) return;
+    float v[16];
+    c[i].get(v);
+    store16(v, out + (long long)row[i] * stride, (int)k[i] * 16, r.cols, vec);
   }
 }
 
 template <class T, int KIND, bool GATED, int U>
-__global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x, long long stride, bool vec_x, T* __restrict__ y,
-                                                        bool vec_y, Rows r, Held held, Held held_b, Held held_y) {
+__global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x, long long stride, int vec_x, T* __restrict__ y,
+                                                        int vec_y, Rows r, Held held, Held held_b, Held held_y) {
   constexpr bool kFast = sizeof(T) == 2;
   const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
-  Chunk8<T> ca[U], cb[GATED ? U : 1];
+  Chunk16<T> ca[U], cb[GATED ? U : 1];
   unsigned row[U], k[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -144,24 +170,24 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x
     if (at < r.chunks) {
       divmod(r.per_row, at, row[i], k[i]);
       const T* p = x + (long long)row[i] * stride;
-      load_chunk(ca[i], p, (int)k[i] * 8, r.cols, vec_x);
-      if (GATED) load_chunk(cb[GATED ? i : 0], p + r.cols, (int)k[i] * 8, r.cols, vec_x);
+      ca[i].load(p, (int)k[i] * 16, r.cols, vec_x);
+      if (GATED) cb[GATED ? i : 0].load(p + r.cols, (int)k[i] * 16, r.cols, vec_x);
     }
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const bool in = base + i * kBlock < r.chunks;
-    const int col = (int)k[i] * 8;
-    float v[8], w[8];
+    const int col = (int)k[i] * 16;
+    float v[16], w[16];
     unsigned s;
-    uint2 codes;
+    uint4 codes;
     ca[i].get(v);
     if (held.codes) {
       codes = act8_encode(v, s);
       if (in) put_held(held, row[i], col, codes, s);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = function<KIND, kFast>(v[j]).x;
+    for (int j = 0; j < 16; ++j) v[j] = function<KIND, kFast>(v[j]).x;
     if (GATED) {
       cb[GATED ? i : 0].get(w);
       if (held_b.codes) {
@@ -169,11 +195,11 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x
         if (in) put_held(held_b, row[i], col, codes, s);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= w[j];
+      for (int j = 0; j < 16; ++j) v[j] *= w[j];
     }
-    if (in) store_chunk(v, y + (size_t)row[i] * r.cols, col, r.cols, vec_y);
+    if (in) store16(v, y + (size_t)row[i] * r.cols, col, r.cols, vec_y);
     if (held_y.codes) {
-      Chunk8<T> cy;   // the checkpoint is of y as the next layer sees it
+      Chunk16<T> cy;   // the checkpoint is of y as the next layer sees it
       cy.set(v);
       cy.get(v);
       codes = act8_encode(v, s);
@@ -183,55 +209,47 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x
 }
 
 template <class T, int KIND, bool GATED, int U>
-__global__ void __launch_bounds__(kBlock) backward_kernel(const T* __restrict__ grad, long long stride, bool vec_g, T* __restrict__ dx,
-                                                         bool vec_x, Rows r, Held held, Held held_b) {
+__global__ void __launch_bounds__(kBlock) backward_kernel(const T* __restrict__ grad, long long stride, int vec_g, T* __restrict__ dx,
+                                                         int vec_x, Rows r, Held held, Held held_b) {
   constexpr bool kFast = sizeof(T) == 2;
   const unsigned base = blockIdx.x * (kBlock * U) + threadIdx.x;
-  Chunk8<T> c[U];
-  uint2 qa[U], qb[GATED ? U : 1];
-  unsigned sa[U], sb[GATED ? U : 1], row[U], k[U];
+  Chunk16<T> c[U];
+  HeldChunk qa[U], qb[GATED ? U : 1];
+  unsigned row[U], k[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const unsigned at = base + i * kBlock;
     if (at < r.chunks) {
       divmod(r.per_row, at, row[i], k[i]);
-      const int col = (int)k[i] * 8;
-      load_chunk(c[i], grad + (long long)row[i] * stride, col, r.cols, vec_g);
-      qa[i] = __ldg(reinterpret_cast<const uint2*>(held.codes + (size_t)row[i] * held.pitch + col));
-      sa[i] = __ldg(held.scales + (size_t)row[i] * held.spitch + (col >> 5));
-      if (GATED) {
-        qb[GATED ? i : 0] = __ldg(reinterpret_cast<const uint2*>(held_b.codes + (size_t)row[i] * held_b.pitch + col));
-        sb[GATED ? i : 0] = __ldg(held_b.scales + (size_t)row[i] * held_b.spitch + (col >> 5));
-      }
+      const int col = (int)k[i] * 16;
+      c[i].load(grad + (long long)row[i] * stride, col, r.cols, vec_g);
+      qa[i].load(held, row[i], col);
+      if (GATED) qb[GATED ? i : 0].load(held_b, row[i], col);
     }
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     if (base + i * kBlock >= r.chunks) return;
-    const int col = (int)k[i] * 8;
-    float g[8], a[8], b[8];
+    const int col = (int)k[i] * 16;
+    float g[16], a[16], b[16];
     c[i].get(g);
-    act8_decode(qa[i], sa[i], a);
+    qa[i].get(a);
     T* const out = dx + (size_t)row[i] * (GATED ? 2 : 1) * r.cols;
     if (GATED) {
-      act8_decode(qb[GATED ? i : 0], sb[GATED ? i : 0], b);
+      qb[GATED ? i : 0].get(b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 16; ++j) {
         const float2 f = function<KIND, kFast>(a[j]);
         a[j] = g[j] * b[j] * f.y;
         b[j] = g[j] * f.x;
       }
-      store_chunk(b, out + r.cols, col, r.cols, vec_x);
+      store16(b, out + r.cols, col, r.cols, vec_x);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = g[j] * function<KIND, kFast>(a[j]).y;
+      for (int j = 0; j < 16; ++j) a[j] = g[j] * function<KIND, kFast>(a[j]).y;
     }
-    store_chunk(a, out, col, r.cols, vec_x);
+    store16(a, out, col, r.cols, vec_x);
   }
-}
-
-bool aligned(const void* p, long long stride_elems, int es) {
-  return (reinterpret_cast<uintptr_t>(p) % 16 == 0) && (stride_elems * es) % 16 == 0;
 }
 
 Held rows_from(Held h, long long row) {
@@ -245,7 +263,7 @@ Held rows_from(Held h, long long row) {
 // Calls f(first row, Rows, grid for `per_thread` chunks a thread) for slabs of rows whose chunk count fits 31 bits.
 template <class F>
 cudaError_t over_slabs(long long rows, int cols, int per_thread, F f) {
-  const long long per_row = ((long long)cols + 31) / 32 * 4;
+  const long long per_row = ((long long)cols + 31) / 32 * 2;
   const long long slab = ((1ll << 31) - 1) / per_row;
   for (long long at = 0; at < rows; at += slab) {
     const long long n = rows - at < slab ? rows - at : slab;
@@ -258,12 +276,12 @@ cudaError_t over_slabs(long long rows, int cols, int per_thread, F f) {
   return cudaSuccess;
 }
 
-constexpr int kUnroll = 2;
+constexpr int kUnroll = 1;
 
 template <class T>
 cudaError_t pack_typed(const void* x, long long stride, long long rows, int cols, Held held, cudaStream_t st) {
   const T* p = static_cast<const T*>(x);
-  const bool vec = aligned(x, stride, sizeof(T));
+  const int vec = row_align(x, stride, sizeof(T));
   return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
     pack_kernel<T, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec, r, rows_from(held, at));
   });
@@ -271,7 +289,7 @@ cudaError_t pack_typed(const void* x, long long stride, long long rows, int cols
 template <class T>
 cudaError_t unpack_typed(Held held, void* out, long long stride, long long rows, int cols, cudaStream_t st) {
   T* p = static_cast<T*>(out);
-  const bool vec = aligned(out, stride, sizeof(T));
+  const int vec = row_align(out, stride, sizeof(T));
   return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
     unpack_kernel<T, kUnroll><<<grid, kBlock, 0, st>>>(rows_from(held, at), p + at * stride, stride, vec, r);
   });
@@ -280,7 +298,8 @@ template <class T, int KIND, bool GATED>
 cudaError_t forward_typed(const void* x, long long stride, void* y, long long rows, int cols, Held a, Held b, Held hy, cudaStream_t st) {
   const T* p = static_cast<const T*>(x);
   T* q = static_cast<T*>(y);
-  const bool vec_x = aligned(x, stride, sizeof(T)) && (!GATED || aligned(x, cols, sizeof(T))), vec_y = aligned(y, cols, sizeof(T));
+  const int vec_y = row_align(y, cols, sizeof(T));
+  const int vec_x = std::min(row_align(x, stride, sizeof(T)), GATED ? row_align(x, cols, sizeof(T)) : (int)kRow32);
   return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
     forward_kernel<T, KIND, GATED, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec_x, q + at * cols, vec_y, r,
                                                                      rows_from(a, at), rows_from(b, at), rows_from(hy, at));
@@ -290,7 +309,7 @@ template <class T, int KIND, bool GATED>
 cudaError_t backward_typed(const void* grad, long long stride, void* dx, long long rows, int cols, Held a, Held b, cudaStream_t st) {
   const T* p = static_cast<const T*>(grad);
   T* q = static_cast<T*>(dx);
-  const bool vec_g = aligned(grad, stride, sizeof(T)), vec_x = aligned(dx, cols, sizeof(T));
+  const int vec_g = row_align(grad, stride, sizeof(T)), vec_x = row_align(dx, cols, sizeof(T));
   return over_slabs(rows, cols, kUnroll, [&](long long at, Rows r, unsigned grid) {
     backward_kernel<T, KIND, GATED, kUnroll><<<grid, kBlock, 0, st>>>(p + at * stride, stride, vec_g, q + at * cols * (GATED ? 2 : 1),
                                                                       vec_x, r, rows_from(a, at), rows_from(b, at));

@@ -37,37 +37,45 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN where ei
   return r;
 }
 
-// Eight values of a group whose other 24 are held by the neighbouring three lanes (lanes 4i .. 4i + 3, all of them
-// active): their codes, and the group's scale byte.
-__device__ __forceinline__ uint2 act8_encode(const float (&v)[8], unsigned& s) {
+// Sixteen values of a group whose other half is held by the neighbouring lane (lanes 2i and 2i + 1, both active): their
+// codes, and the group's scale byte.
+__device__ __forceinline__ uint4 act8_encode(const float (&v)[16], unsigned& s) {
   float m = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+  for (int j = 0; j < 16; ++j) m = max_nan(m, fabsf(v[j]));
   unsigned top = __float_as_uint(m);     // from here on as integers: a NaN is the largest
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   s = act8_scale_byte(top);
   const float inv = act8_inverse(s);
-  unsigned u[8];
   constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: the sum's low byte is the integer nearest to x * inv, ties to even
+  unsigned w[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    u[j] = __float_as_uint(fminf(fmaxf(__fmaf_rn(v[j], inv, kMagic), kMagic - 127.f), kMagic + 127.f));
-  if (s == 255u) return make_uint2(0u, 0u);   // (an infinity times 0 is a NaN, which the clamp above turns into a bound)
-  const unsigned a = __byte_perm(u[0], u[1], 0x0040), b = __byte_perm(u[2], u[3], 0x0040);
-  const unsigned c = __byte_perm(u[4], u[5], 0x0040), d = __byte_perm(u[6], u[7], 0x0040);
-  return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+  for (int i = 0; i < 4; ++i) {
+    unsigned u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      u[j] = __float_as_uint(fminf(fmaxf(__fmaf_rn(v[4 * i + j], inv, kMagic), kMagic - 127.f), kMagic + 127.f));
+    w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+  }
+  // (an infinity times 0 is a NaN, which the clamp above turns into a bound)
+  return s == 255u ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void act8_decode(uint2 codes, unsigned s, float (&v)[8]) {
+// The values of N codes (four in each of N / 4 words).
+template <int N>
+__device__ __forceinline__ void act8_decode(const unsigned (&codes)[N / 4], unsigned s, float (&v)[N]) {
   const float step = act8_step(s);
-  codes.x ^= 0x80808080u;   // code + 128, an unsigned byte
-  codes.y ^= 0x80808080u;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {   // a byte in the low bits of 2^23 is the number 2^23 + byte
-    v[j] = (__uint_as_float(__byte_perm(codes.x, 0x4b000000u, 0x7540 + j)) - 8388736.f) * step;
-    v[j + 4] = (__uint_as_float(__byte_perm(codes.y, 0x4b000000u, 0x7540 + j)) - 8388736.f) * step;
+  for (int i = 0; i < N / 4; ++i) {
+    const unsigned c = codes[i] ^ 0x80808080u;   // code + 128, an unsigned byte
+#pragma unroll
+    for (int j = 0; j < 4; ++j)   // a byte in the low bits of 2^23 is the number 2^23 + byte
+      v[4 * i + j] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7540 + j)) - 8388736.f) * step;
   }
+}
+__device__ __forceinline__ void act8_decode(uint4 codes, unsigned s, float (&v)[16]) {
+  const unsigned w[4] = {codes.x, codes.y, codes.z, codes.w};
+  act8_decode<16>(w, s, v);
 }
 
 // ---- eight neighbouring elements of a row of fp32, bf16 or fp16, as fp32 ----
@@ -147,22 +155,97 @@ template <> struct Chunk8<float> {   // 32 bytes
   }
 };
 
-// Elements col .. col + 7 of a row of `cols` (zeros past its end).  `vec`: the row starts on a 16-byte boundary.
-template <class T>
-__device__ __forceinline__ void load_chunk(Chunk8<T>& c, const T* __restrict__ row, int col, int cols, bool vec) {
-  if (vec && col + 8 <= cols) c.load(row + col);
-  else if (col < cols) c.load_some(row + col, cols - col);
-  else c.zero();
+// How a row may be accessed: its start, and the distance to the next row, on no boundary, on 16 or on 32 bytes.
+enum RowAlign : int { kRowAny = 0, kRow16 = 1, kRow32 = 2 };
+inline int row_align(const void* p, long long stride_elems, int es) {
+  const unsigned long long both = reinterpret_cast<uintptr_t>(p) | (unsigned long long)(stride_elems * es);
+  return both % 32 == 0 ? kRow32 : (both % 16 == 0 ? kRow16 : kRowAny);
 }
+
+// 32 bytes in one access
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y),
+               "r"(b.z), "r"(b.w) : "memory");
+}
+__device__ __forceinline__ uint4 as_u4(float4 v) { return make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)); }
+__device__ __forceinline__ float4 as_f4(uint4 v) { return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)); }
+
+// Sixteen neighbouring elements, as kernels hold and move them: elements col .. col + 15 of a row of `cols` (zeros past
+// its end), col a multiple of 16.
 template <class T>
-__device__ __forceinline__ void store_chunk(const float (&v)[8], T* __restrict__ row, int col, int cols, bool vec) {
-  if (vec && col + 8 <= cols) {
-    Chunk8<T> c;
+struct Chunk16 {
+  Chunk8<T> lo, hi;
+  __device__ __forceinline__ void zero() {
+    lo.zero();
+    hi.zero();
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ row, int col, int cols, int align) {
+    if (align == kRow32 && col + 16 <= cols) {
+      if constexpr (sizeof(T) == 2) {
+        load32(row + col, lo.w, hi.w);
+      } else {
+        uint4 a, b;
+        load32(row + col, a, b);
+        lo.a = as_f4(a);
+        lo.b = as_f4(b);
+        load32(row + col + 8, a, b);
+        hi.a = as_f4(a);
+        hi.b = as_f4(b);
+      }
+    } else if (align == kRow16 && col + 16 <= cols) {
+      lo.load(row + col);
+      hi.load(row + col + 8);
+    } else {
+      zero();
+      if (col < cols) lo.load_some(row + col, cols - col);
+      if (col + 8 < cols) hi.load_some(row + col + 8, cols - col - 8);
+    }
+  }
+  __device__ __forceinline__ void store(T* __restrict__ row, int col, int align) const {
+    if (align == kRow32) {
+      if constexpr (sizeof(T) == 2) {
+        store32(row + col, lo.w, hi.w);
+      } else {
+        store32(row + col, as_u4(lo.a), as_u4(lo.b));
+        store32(row + col + 8, as_u4(hi.a), as_u4(hi.b));
+      }
+    } else {
+      lo.store(row + col);
+      hi.store(row + col + 8);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[16]) const {
+    float x[8];
+    lo.get(x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = x[j];
+    hi.get(x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[8 + j] = x[j];
+  }
+  __device__ __forceinline__ void set(const float (&v)[16]) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[j];
+    lo.set(x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[8 + j];
+    hi.set(x);
+  }
+};
+template <class T>
+__device__ __forceinline__ void store16(const float (&v)[16], T* __restrict__ row, int col, int cols, int align) {
+  if (align != kRowAny && col + 16 <= cols) {
+    Chunk16<T> c;
     c.set(v);
-    c.store(row + col);
+    c.store(row, col, align);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 16; ++j)
       if (col + j < cols) row[col + j] = from_f32<T>(v[j]);
   }
 }

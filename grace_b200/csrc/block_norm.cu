@@ -15,12 +15,14 @@
 //
 // Both passes are bound by memory: forward 4 tensors of the type's width and 1 or 2 checkpoints, 10 bytes an element for
 // bf16 with everything, backward the same; 7 and 5 for "add and norm" alone, whose stream nobody reads.  A row is held
-// in registers, eight columns a thread (16 in the backward pass beyond 4096), by one warp or several, so that statistics
-// and results take one pass over memory; small rows share a CTA.  A CTA walks a run of rows that belong to one
+// in registers, sixteen columns a thread, by one warp or several, so that statistics and results take one pass over
+// memory; small rows share a CTA.  A CTA walks a run of rows that belong to one
 // sequence: its parameters and its gate stay in shared memory (fetched anew for every row, from L2, they cost three
 // times what the row does), and the next row's loads are under way while this one is reduced and written.
 // Sums over tokens: a CTA keeps its columns' sums in registers over its run and stores them once; a second kernel
 // adds the runs' sums in a fixed order (no atomics: the same bits on every run).
+#include <algorithm>
+
 #include "act8.cuh"
 #include "act8.h"
 #include "common.cuh"
@@ -29,44 +31,32 @@
 namespace grace {
 namespace {
 
-// Columns col .. col + 7 of a row of parameters, fp32 or of the activations' type; null, or past the end: `none`.
+// Columns col .. col + 3 of a row of parameters, fp32 or of the activations' type; null, or past the end: `none`.
 template <class T>
-__device__ __forceinline__ void load_param(const BlockNormArgs& a, const void* p, int col, float none, float (&v)[8]) {
-  if (p != nullptr && a.param_vec && col + 8 <= a.cols) {
-    if (a.params_f32) {
-      Chunk8<float> c;
-      c.load(static_cast<const float*>(p) + col);
-      c.get(v);
-    } else {
-      Chunk8<T> c;
-      c.load(static_cast<const T*>(p) + col);
-      c.get(v);
-    }
-    return;
-  }
+__device__ __forceinline__ float4 load_param(const BlockNormArgs& a, const void* p, int col, float none) {
+  float v[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 4; ++j)
     v[j] = p == nullptr || col + j >= a.cols ? none
-                                              : (a.params_f32 ? static_cast<const float*>(p)[col + j] : to_f32<T>(static_cast<const T*>(p)[col + j]));
+                                              : (a.params_f32 ? __ldg(static_cast<const float*>(p) + col + j) : to_f32<T>(static_cast<const T*>(p)[col + j]));
+  return make_float4(v[0], v[1], v[2], v[3]);
 }
 
-// A row of parameters in shared memory, fp32, for `chunks` chunks of eight columns: the first halves of all chunks, then
-// the second halves, so that a quarter warp's 16-byte accesses are consecutive.
+// A row of parameters in shared memory, fp32, for `chunks` chunks of sixteen columns: the first quarters of all chunks,
+// then the second ones, and so on, so that a quarter warp's 16-byte accesses are consecutive.
 struct SharedRow {
   float4* at;
   int chunks;
   template <class T>
   __device__ __forceinline__ void fill(const BlockNormArgs& a, const void* p, float none) const {
-    for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
-      float v[8];
-      load_param<T>(a, p, c * 8, none, v);
-      at[c] = make_float4(v[0], v[1], v[2], v[3]);
-      at[chunks + c] = make_float4(v[4], v[5], v[6], v[7]);
-    }
+    for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) at[(i & 3) * chunks + (i >> 2)] = load_param<T>(a, p, i * 4, none);
   }
-  __device__ __forceinline__ void get(int chunk, float (&v)[8]) const {
-    const float4 lo = at[chunk], hi = at[chunks + chunk];
-    v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+  __device__ __forceinline__ void get(int chunk, float (&v)[16]) const {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 x = at[q * chunks + chunk];
+      v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+    }
   }
 };
 
@@ -118,15 +108,15 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
-// (mean, 1 / deviation) of a row, eight columns a thread.  Layer norm: each warp's mean and squared deviations from it,
-// joined over the warps by Chan, Golub and LeVeque's formula, so that one barrier does and nothing cancels.
+// (mean, 1 / deviation) of a row, sixteen columns a thread.  Layer norm: each warp's mean and squared deviations from
+// it, joined over the warps by Chan, Golub and LeVeque's formula, so that one barrier does and nothing cancels.
 template <bool LAYER>
-__device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int cols, float inv_cols, float eps, RowSum<2>& sum) {
+__device__ __forceinline__ float2 row_stats(const float (&v)[16], int valid, int cols, float inv_cols, float eps, RowSum<2>& sum) {
   const int lane = threadIdx.x & 31, warps = sum.tpr >> 5, warp = threadIdx.x >> 5, first = warp / warps * warps;
   if (!LAYER) {
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);   // (columns past the end are zeros)
+    for (int j = 0; j < 16; ++j) s = fmaf(v[j], v[j], s);   // (columns past the end are zeros)
     s = warp_sum(s);
     if (warps > 1) {
       float* const b = sum.next();
@@ -136,13 +126,13 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int 
     }
     return make_float2(0.f, inv_sqrt(fmaf(s, inv_cols, eps)));
   }
-  const float n = (float)min(256, max(0, cols - (warp - first) * 256));
+  const float n = (float)min(512, max(0, cols - (warp - first) * 512));
   float m = 0.f, d = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m += v[j];
+  for (int j = 0; j < 16; ++j) m += v[j];
   m = n > 0.f ? __fdividef(warp_sum(m), n) : 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 16; ++j) {
     const float x = j < valid ? v[j] - m : 0.f;
     d = fmaf(x, x, d);
   }
@@ -154,7 +144,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int 
       b[warp * 2 + 1] = d;
     }
     __syncthreads();
-    const float nl = lane < warps ? (float)min(256, max(0, cols - lane * 256)) : 0.f;
+    const float nl = lane < warps ? (float)min(512, max(0, cols - lane * 512)) : 0.f;
     const float ml = lane < warps ? b[(first + lane) * 2] : 0.f;
     m = warp_sum(nl * ml) * inv_cols;
     d = warp_sum(lane < warps ? fmaf(nl * (ml - m), ml - m, b[(first + lane) * 2 + 1]) : 0.f);
@@ -162,8 +152,9 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[8], int valid, int 
   return make_float2(m, inv_sqrt(fmaf(d, inv_cols, eps)));
 }
 
-__device__ __forceinline__ void put_codes(const Held& h, size_t row, int col, uint2 codes, unsigned s) {
-  *reinterpret_cast<uint2*>(h.codes + row * h.pitch + col) = codes;
+// The codes at columns col .. col + 15 of a row and, from the lane with a group's first columns, its scale byte.
+__device__ __forceinline__ void put_codes(const Held& h, long long row, int col, uint4 codes, unsigned s) {
+  *reinterpret_cast<uint4*>(h.codes + row * h.pitch + col) = codes;
   if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
 }
 
@@ -172,51 +163,52 @@ __device__ __forceinline__ void put_codes(const Held& h, size_t row, int col, ui
 // taken in 64 bits, and the fp32 one moved off the middle towards it.
 template <class T> constexpr unsigned tie_mask() { return sizeof(T) == 4 ? 0u : (__is_same(T, __half) ? 0x1fffu : 0xffffu); }
 template <class T>
-__device__ __forceinline__ void scaled_sum(float alpha, const float (&x)[8], float (&v)[8]) {
+__device__ __forceinline__ void scaled_sum(float alpha, const float (&x)[16], float (&v)[16]) {
   constexpr unsigned mask = tie_mask<T>(), tie = (mask + 1) >> 1;
-  bool any = false;
-  float y[8];
+  float y[16];
+  unsigned least = ~0u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 16; ++j) {
     y[j] = fmaf(alpha, x[j], v[j]);
-    if (mask) any = any || (__float_as_uint(y[j]) & mask) == tie;
+    if (mask) least = min(least, (__float_as_uint(y[j]) ^ tie) & mask);     // 0: on a middle
   }
-  if (mask && any) {
+  if (mask && least == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 16; ++j) {
       if ((__float_as_uint(y[j]) & mask) != tie) continue;
       const double exact = (double)alpha * (double)x[j] + (double)v[j], at = (double)y[j];
       if (exact != at) y[j] = __uint_as_float(__float_as_uint(y[j]) + ((exact > at) == (at > 0.0) ? 1u : ~0u));
     }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = y[j];
+  for (int j = 0; j < 16; ++j) v[j] = y[j];
 }
 
 template <class T, bool PRE_LAYER, int POST>
-__global__ void __launch_bounds__(1024) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
+__global__ void __launch_bounds__(512) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
   __shared__ float buf[2 * 64];
   extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
-  const int col = t * 8, valid = min(8, max(0, a.cols - col)), chunks = a.held_y.pitch / 8;
+  const int col = t * 16, valid = min(16, max(0, a.cols - col)), chunks = a.held_y.pitch / 16;
   const bool owns = col < a.held_y.pitch;      // (threads past the last group of 32 only take part in the sums)
   const int chunk = owns ? t : 0;
   const float inv_cols = 1.f / (float)a.cols;
   const Run run = run_of(a);
   RowSum<2> sum{buf, 0, tpr};
-  Chunk8<T> cb, cx;
+  Chunk16<T> cb, cx;
   auto load = [&](long long row) {
-    cb.zero();
-    cx.zero();
     if (row < run.row1) {
-      load_chunk(cb, static_cast<const T*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
-      load_chunk(cx, static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols, a.x_vec);
+      cb.load(static_cast<const T*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
+      cx.load(static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols, a.x_vec);
+    } else {
+      cb.zero();
+      cx.zero();
     }
   };
   load(run.row0 + lane_row);
   int used = 0;
   auto shared_row = [&](const void* p, float none) {
-    const SharedRow r{params + 2 * chunks * used++, chunks};
+    const SharedRow r{params + 4 * chunks * used++, chunks};
     r.template fill<T>(a, p, none);
     return r;
   };
@@ -230,13 +222,11 @@ __global__ void __launch_bounds__(1024) block_norm_forward_kernel(const BlockNor
   for (long long base = run.row0; base < run.row1; base += rpb) {
     const long long row = base + lane_row;
     const bool in = row < run.row1;
-    float v[8], w[8], x[8];
+    float v[16], w[16];
     cb.get(v);
-    cx.get(x);
-    load(row + rpb);
     unsigned s;
     if (a.held_b.codes) {
-      const uint2 codes = act8_encode(v, s);
+      const uint4 codes = act8_encode(v, s);
       if (in && owns) put_codes(a.held_b, row, col, codes, s);
     }
     float2 post = make_float2(0.f, 1.f);
@@ -244,117 +234,114 @@ __global__ void __launch_bounds__(1024) block_norm_forward_kernel(const BlockNor
       post = row_stats<POST == kNormLayer>(v, valid, a.cols, inv_cols, a.eps, sum);
       post_w.get(chunk, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y * w[j];
+      for (int j = 0; j < 16; ++j) v[j] = (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y * w[j];
       if (POST == kNormLayer) {
         post_b.get(chunk, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += w[j];
+        for (int j = 0; j < 16; ++j) v[j] += w[j];
       }
     }
     if (a.gate) {
       gate.get(chunk, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= w[j];
+      for (int j = 0; j < 16; ++j) v[j] *= w[j];
     }
-    scaled_sum<T>(a.alpha, x, v);
-    if (valid < 8) {
+    cx.get(w);
+    scaled_sum<T>(a.alpha, w, v);
+    load(row + rpb);       // the next row's loads are under way during the rest of this one
+    if (valid < 16) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] : 0.f;
+      for (int j = 0; j < 16; ++j) v[j] = j < valid ? v[j] : 0.f;
     }
-    Chunk8<T> cy;
+    Chunk16<T> cy;
     cy.set(v);       // the stream as it is rounded to its type
     cy.get(v);
-    if (in && a.y) store_chunk(v, static_cast<T*>(a.y) + row * a.cols, col, a.cols, a.out_vec);
+    if (in && a.y) store16(v, static_cast<T*>(a.y) + row * a.cols, col, a.cols, a.out_vec);
     {
-      const uint2 codes = act8_encode(v, s);
+      const uint4 codes = act8_encode(v, s);
       if (in && owns) put_codes(a.held_y, row, col, codes, s);
     }
     const float2 pre = row_stats<PRE_LAYER>(v, valid, a.cols, inv_cols, a.eps, sum);
     pre_w.get(chunk, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (PRE_LAYER ? v[j] - pre.x : v[j]) * pre.y * w[j];
+    for (int j = 0; j < 16; ++j) v[j] = (PRE_LAYER ? v[j] - pre.x : v[j]) * pre.y * w[j];
     if (PRE_LAYER) {
       pre_b.get(chunk, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += w[j];
+      for (int j = 0; j < 16; ++j) v[j] += w[j];
     }
-    if (in) store_chunk(v, static_cast<T*>(a.h) + row * a.cols, col, a.cols, a.out_vec);
+    if (in) store16(v, static_cast<T*>(a.h) + row * a.cols, col, a.cols, a.out_vec);
     if (a.held_h.codes) {
-      if (valid < 8) {
+      if (valid < 16) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] : 0.f;
+        for (int j = 0; j < 16; ++j) v[j] = j < valid ? v[j] : 0.f;
       }
       cy.set(v);
       cy.get(v);
-      const uint2 codes = act8_encode(v, s);
+      const uint4 codes = act8_encode(v, s);
       if (in && owns) put_codes(a.held_h, row, col, codes, s);
     }
     if (in && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(pre.x, pre.y, post.x, post.y);
   }
 }
 
-// What a thread loads of a row: eight columns.
+// What a thread loads of a row in the backward pass: sixteen columns.
 template <class T, bool TWO>
 struct RowLoads {
-  Chunk8<T> dh, dy;
-  uint2 qy, qb;
+  Chunk16<T> dh, dy;
+  uint4 qy, qb;
   unsigned sy, sb;
+  float4 stats;
   __device__ __forceinline__ void load(const BlockNormArgs& a, long long row, int col, bool in) {
-    qy = qb = make_uint2(0u, 0u);
+    qy = qb = make_uint4(0u, 0u, 0u, 0u);
     sy = sb = 1u;
     dh.zero();
     dy.zero();
+    stats = make_float4(0.f, 0.f, 0.f, 0.f);
     if (!in) return;
-    load_chunk(dh, static_cast<const T*>(a.grad_h) + row * a.grad_h_stride, col, a.cols, a.grad_h_vec);
-    if (a.grad_y) load_chunk(dy, static_cast<const T*>(a.grad_y) + row * a.grad_y_stride, col, a.cols, a.grad_y_vec);
+    dh.load(static_cast<const T*>(a.grad_h) + row * a.grad_h_stride, col, a.cols, a.grad_h_vec);
+    if (a.grad_y) dy.load(static_cast<const T*>(a.grad_y) + row * a.grad_y_stride, col, a.cols, a.grad_y_vec);
+    stats = __ldg(reinterpret_cast<const float4*>(a.stats + row * 4));
     if (col < a.held_y.pitch) {
-      qy = __ldg(reinterpret_cast<const uint2*>(a.held_y.codes + (size_t)row * a.held_y.pitch + col));
-      sy = __ldg(a.held_y.scales + (size_t)row * a.held_y.spitch + (col >> 5));
+      qy = __ldg(reinterpret_cast<const uint4*>(a.held_y.codes + row * a.held_y.pitch + col));
+      sy = __ldg(a.held_y.scales + row * a.held_y.spitch + (col >> 5));
       if (TWO) {
-        qb = __ldg(reinterpret_cast<const uint2*>(a.held_b.codes + (size_t)row * a.held_b.pitch + col));
-        sb = __ldg(a.held_b.scales + (size_t)row * a.held_b.spitch + (col >> 5));
+        qb = __ldg(reinterpret_cast<const uint4*>(a.held_b.codes + row * a.held_b.pitch + col));
+        sb = __ldg(a.held_b.scales + row * a.held_b.spitch + (col >> 5));
       }
     }
   }
 };
 
-// (value - mean) * rstd of eight held values; the difference first: a mean far from zero must not cost digits
+// (value - mean) * rstd of held values; the difference first: a mean far from zero must not cost digits
 template <bool LAYER>
-__device__ __forceinline__ void decode_normed(uint2 codes, unsigned s, float mean, float rstd, float (&v)[8]) {
+__device__ __forceinline__ void decode_normed(uint4 codes, unsigned s, float mean, float rstd, float (&v)[16]) {
   act8_decode(codes, s, v);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = (LAYER ? v[j] - mean : v[j]) * rstd;
+  for (int j = 0; j < 16; ++j) v[j] = (LAYER ? v[j] - mean : v[j]) * rstd;
 }
 
-// VPT chunks of eight columns a thread, tpr * 8 columns apart.  BLOCK: 0 neither a norm after the block nor a gate, so that
-// b~ is not read; 1 either, without sums of g (G0); 2 with them (a layer norm after the block).
-template <class T, int VPT, bool PRE_LAYER, int BLOCK>
+// BLOCK: 0 neither a norm after the block nor a gate, so that b~ is not read; 1 either, without sums of g (G0); 2 with them
+// (a layer norm after the block).
+template <class T, bool PRE_LAYER, int BLOCK>
 __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNormArgs a, int tpr) {
   constexpr bool TWO = BLOCK > 0;
-  constexpr int B = TWO ? VPT : 1, L = PRE_LAYER ? VPT : 1, Z = BLOCK == 2 ? VPT : 1;
+  constexpr int B = TWO ? 16 : 1, L = PRE_LAYER ? 16 : 1, Z = BLOCK == 2 ? 16 : 1;
   __shared__ float buf[2 * 64];
   extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
-  const int chunks = a.held_y.pitch / 8;
+  const int chunks = a.held_y.pitch / 16, chunk = t < chunks ? t : 0, col = t * 16;
   const float inv_cols = 1.f / (float)a.cols;
   const Run run = run_of(a);
   RowSum<2> sum2{buf, 0, tpr};
-  RowSum<1> sum1{buf, 0, tpr};
   const bool post = TWO && a.post != kNormNone;
-  float dw[VPT][8] = {}, db[L][8] = {}, g1[B][8] = {}, g0[Z][8] = {};
+  float dw[16] = {}, db[L] = {}, g1[B] = {}, g0[Z] = {};
 
-  RowLoads<T, TWO> r[VPT];
-  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto load = [&](long long row) {
-    const bool in = row < run.row1;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) r[i].load(a, row, (i * tpr + t) * 8, in);
-    st = in ? __ldg(reinterpret_cast<const float4*>(a.stats + row * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-  };
-  load(run.row0 + lane_row);
+  RowLoads<T, TWO> r;
+  r.load(a, run.row0 + lane_row, col, run.row0 + lane_row < run.row1);
   int used = 0;
   auto shared_row = [&](const void* p, float none) {
-    const SharedRow r{params + 2 * chunks * used++, chunks};
+    const SharedRow r{params + 4 * chunks * used++, chunks};
     r.template fill<T>(a, p, none);
     return r;
   };
@@ -366,133 +353,103 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
   for (long long base = run.row0; base < run.row1; base += rpb) {
     const long long row = base + lane_row;
     const bool in = row < run.row1;
-    float c[VPT][8], hat[VPT][8], bh[B][8];
-    Chunk8<T> dy[VPT];
-    float s[2] = {0.f, 0.f};
-    const float4 stats = st;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int k = i * tpr + t, chunk = k < chunks ? k : 0;
-      float w[8], d[8];
-      r[i].dh.get(d);
-      decode_normed<PRE_LAYER>(r[i].qy, r[i].sy, stats.x, stats.y, hat[i]);
-      pre_w.get(chunk, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dw[i][j] = fmaf(d[j], hat[i][j], dw[i][j]);
-        c[i][j] = d[j] * w[j];
-        s[0] = fmaf(c[i][j], hat[i][j], s[0]);
-        if (PRE_LAYER) {
-          db[PRE_LAYER ? i : 0][j] += d[j];
-          s[1] += c[i][j];
-        }
-      }
-      dy[i] = r[i].dy;
-      if (TWO) decode_normed<BLOCK == 2>(r[i].qb, r[i].sb, stats.z, stats.w, bh[TWO ? i : 0]);
-    }
-    load(row + rpb);     // the next row's loads are under way during the sums
+    float c[16], hat[16], bh[B], w[16], s[2] = {0.f, 0.f};
+    const float4 stats = r.stats;
+    const Chunk16<T> dy = r.dy;
     auto row_sum = [&](bool both) {
       if (both) {
         sum2(s);
       } else {
+        RowSum<1> sum1{buf, sum2.parity, tpr};   // (the two share their buffers)
         float v[1] = {s[0]};
-        sum1.parity = sum2.parity;   // (the two share their buffers)
         sum1(v);
         s[0] = v[0];
         sum2.parity = sum1.parity;
       }
     };
+    r.dh.get(c);
+    decode_normed<PRE_LAYER>(r.qy, r.sy, stats.x, stats.y, hat);
+    pre_w.get(chunk, w);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      dw[j] = fmaf(c[j], hat[j], dw[j]);
+      if (PRE_LAYER) db[PRE_LAYER ? j : 0] += c[j];
+      c[j] *= w[j];
+      s[0] = fmaf(c[j], hat[j], s[0]);
+      if (PRE_LAYER) s[1] += c[j];
+    }
+    if constexpr (TWO) decode_normed<BLOCK == 2>(r.qb, r.sb, stats.z, stats.w, bh);
+    r.load(a, row + rpb, col, row + rpb < run.row1);     // the next row's loads are under way during the sums
     row_sum(PRE_LAYER);
     const float m1 = s[0] * inv_cols, m0 = PRE_LAYER ? s[1] * inv_cols : 0.f;
     s[0] = s[1] = 0.f;
+    dy.get(w);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int k = i * tpr + t, chunk = k < chunks ? k : 0, col = k * 8;
-      float d[8], w[8];
-      dy[i].get(d);
+    for (int j = 0; j < 16; ++j) c[j] = fmaf(stats.y, fmaf(-hat[j], m1, PRE_LAYER ? c[j] - m0 : c[j]), w[j]);   // g
+    if (in && a.dx) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[i][j] = fmaf(stats.y, fmaf(-hat[i][j], m1, PRE_LAYER ? c[i][j] - m0 : c[i][j]), d[j]);   // g
-      if (in && a.dx) {
+      for (int j = 0; j < 16; ++j) w[j] = a.alpha * c[j];
+      store16(w, static_cast<T*>(a.dx) + row * a.cols, col, a.cols, a.out_vec);
+    }
+    if constexpr (TWO) {
+      if (!in || col + 16 > a.cols) {   // what does not exist adds nothing
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = a.alpha * c[i][j];
-        store_chunk(d, static_cast<T*>(a.dx) + row * a.cols, col, a.cols, a.out_vec);
+        for (int j = 0; j < 16; ++j) c[j] = in && col + j < a.cols ? c[j] : 0.f;
       }
-      if (TWO) {
-        if (!in || col + 8 > a.cols) {   // what does not exist adds nothing
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c[i][j] = in && col + j < a.cols ? c[i][j] : 0.f;
-        }
+      for (int j = 0; j < 16; ++j) {
+        g1[j] = fmaf(c[j], bh[j], g1[j]);
+        if (BLOCK == 2) g0[BLOCK == 2 ? j : 0] += c[j];
+      }
+      if (a.gate) {
+        gate.get(chunk, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          g1[TWO ? i : 0][j] = fmaf(c[i][j], bh[TWO ? i : 0][j], g1[TWO ? i : 0][j]);
-          if (BLOCK == 2) g0[BLOCK == 2 ? i : 0][j] += c[i][j];
-        }
-        if (a.gate) {
-          gate.get(chunk, w);
+        for (int j = 0; j < 16; ++j) c[j] *= w[j];
+      }
+      if (post) {
+        post_w.get(chunk, w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c[i][j] *= w[j];
+        for (int j = 0; j < 16; ++j) {
+          c[j] *= w[j];
+          s[0] = fmaf(c[j], bh[j], s[0]);
+          if (BLOCK == 2) s[1] += c[j];
         }
-        if (post) {
-          post_w.get(chunk, w);
+        row_sum(BLOCK == 2);
+        const float p1 = s[0] * inv_cols, p0 = BLOCK == 2 ? s[1] * inv_cols : 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            c[i][j] *= w[j];
-            s[0] = fmaf(c[i][j], bh[TWO ? i : 0][j], s[0]);
-            if (BLOCK == 2) s[1] += c[i][j];
-          }
-        }
+        for (int j = 0; j < 16; ++j) c[j] = stats.w * fmaf(-bh[j], p1, BLOCK == 2 ? c[j] - p0 : c[j]);
       }
     }
-    if (post) {
-      row_sum(BLOCK == 2);
-      const float p1 = s[0] * inv_cols, p0 = BLOCK == 2 ? s[1] * inv_cols : 0.f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[i][j] = stats.w * fmaf(-bh[TWO ? i : 0][j], p1, BLOCK == 2 ? c[i][j] - p0 : c[i][j]);
-    }
-    if (in) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) store_chunk(c[i], static_cast<T*>(a.dblock) + row * a.cols, (i * tpr + t) * 8, a.cols, a.out_vec);
-    }
+    if (in) store16(c, static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
   }
   if (!a.sums) return;
   // This run's sums: [4][pitch] floats.  The CTA's row lanes are added in order, each on top of the one before it.
   const long long pitch = a.held_y.pitch;
   float4* const out = reinterpret_cast<float4*>(a.sums + (long long)blockIdx.x * 4 * pitch);
   float4* const part = params;                       // the parameters are not needed any more
-  constexpr int kSums = 1 + (PRE_LAYER ? 1 : 0) + (TWO ? 1 : 0) + (BLOCK == 2 ? 1 : 0);
   for (int l = 0; l < rpb; ++l) {
     __syncthreads();
-    if (lane_row != l) continue;
+    if (lane_row != l || t >= chunks) continue;
+    int n = 0;
+    auto put = [&](int which, const float (&v)[16]) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int k = i * tpr + t;
-      if (k >= chunks) continue;
-      int n = 0;
-      auto put = [&](int which, float (&v)[8]) {
-        float4* const p = part + (long long)n * 2 * chunks + k;     // first halves, then second halves of the chunks
-        ++n;
+      for (int q = 0; q < 4; ++q) {
+        float4 x = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        float4* const p = part + (n * 4 + q) * chunks + t;
         if (l > 0) {
-          const float4 x = p[0], y = p[chunks];
-          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+          const float4 y = *p;
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
-        const float4 x = make_float4(v[0], v[1], v[2], v[3]), y = make_float4(v[4], v[5], v[6], v[7]);
-        if (l + 1 < rpb) {
-          p[0] = x;
-          p[chunks] = y;
-        } else {
-          out[which * (pitch / 4) + k * 2] = x;
-          out[which * (pitch / 4) + k * 2 + 1] = y;
-        }
-      };
-      put(0, dw[i]);
-      if (PRE_LAYER) put(1, db[PRE_LAYER ? i : 0]);
-      if (TWO) put(2, g1[TWO ? i : 0]);
-      if (BLOCK == 2) put(3, g0[BLOCK == 2 ? i : 0]);
-    }
+        if (l + 1 < rpb) *p = x;
+        else out[which * (pitch / 4) + t * 4 + q] = x;
+      }
+      ++n;
+    };
+    put(0, dw);
+    if constexpr (PRE_LAYER) put(1, db);
+    if constexpr (TWO) put(2, g1);
+    if constexpr (BLOCK == 2) put(3, g0);
   }
-  static_assert(kSums <= 4, "see backward_smem");
 }
 
 // Adds the runs' sums.  Block: 32 columns x 32 lanes of runs.  blockIdx.y 0 .. 3: one of the norms' parameters, over all
@@ -539,15 +496,6 @@ __global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const Bloc
   else put(grads[which], at, weigh && !a.gate_rows ? v * param(a.gate, at) : v);
 }
 
-bool aligned(const void* p, long long stride, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * es % 16 == 0; }
-
-bool params_aligned(const BlockNormArgs& a) {
-  const void* all[] = {a.pre_weight, a.pre_bias, a.post_weight, a.post_bias, a.gate};
-  for (const void* p : all)
-    if (reinterpret_cast<uintptr_t>(p) % 16) return false;
-  return a.cols % 8 == 0;
-}
-
 template <class K>
 cudaError_t launch_shared(K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const BlockNormArgs& a, int tpr) {
   if (smem > 40 * 1024) {   // (48 KB with the static part need no leave)
@@ -560,11 +508,10 @@ cudaError_t launch_shared(K kernel, dim3 grid, dim3 block, size_t smem, cudaStre
 
 template <class T>
 cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
-  a.x_vec = aligned(a.x, a.x_stride, sizeof(T));
-  a.block_vec = aligned(a.block, a.block_stride, sizeof(T));
-  a.out_vec = aligned(a.h, a.cols, sizeof(T)) && aligned(a.y, a.cols, sizeof(T));
-  a.param_vec = params_aligned(a);
-  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, false);
+  a.x_vec = row_align(a.x, a.x_stride, sizeof(T));
+  a.block_vec = row_align(a.block, a.block_stride, sizeof(T));
+  a.out_vec = std::min(row_align(a.h, a.cols, sizeof(T)), row_align(a.y, a.cols, sizeof(T)));
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms);
   a.parts = shape.parts;
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
   const bool layer = a.pre == kNormLayer;
@@ -580,7 +527,7 @@ cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   }
 }
 
-template <class T, int VPT>
+template <class T>
 cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape, cudaStream_t stream) {
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
   const int form = a.held_b.codes == nullptr ? 0 : (a.post == kNormLayer ? 2 : 1);
@@ -591,23 +538,22 @@ cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape,
   if (shape.rpb > 1 && sums > rows) rows = sums;
   const size_t smem = (size_t)rows * a.held_y.pitch * 4;
   switch (form * 2 + (layer ? 1 : 0)) {
-    case 0: return launch_shared(block_norm_backward_kernel<T, VPT, false, 0>, grid, block, smem, stream, a, shape.tpr);
-    case 1: return launch_shared(block_norm_backward_kernel<T, VPT, true, 0>, grid, block, smem, stream, a, shape.tpr);
-    case 2: return launch_shared(block_norm_backward_kernel<T, VPT, false, 1>, grid, block, smem, stream, a, shape.tpr);
-    case 3: return launch_shared(block_norm_backward_kernel<T, VPT, true, 1>, grid, block, smem, stream, a, shape.tpr);
-    case 4: return launch_shared(block_norm_backward_kernel<T, VPT, false, 2>, grid, block, smem, stream, a, shape.tpr);
-    default: return launch_shared(block_norm_backward_kernel<T, VPT, true, 2>, grid, block, smem, stream, a, shape.tpr);
+    case 0: return launch_shared(block_norm_backward_kernel<T, false, 0>, grid, block, smem, stream, a, shape.tpr);
+    case 1: return launch_shared(block_norm_backward_kernel<T, true, 0>, grid, block, smem, stream, a, shape.tpr);
+    case 2: return launch_shared(block_norm_backward_kernel<T, false, 1>, grid, block, smem, stream, a, shape.tpr);
+    case 3: return launch_shared(block_norm_backward_kernel<T, true, 1>, grid, block, smem, stream, a, shape.tpr);
+    case 4: return launch_shared(block_norm_backward_kernel<T, false, 2>, grid, block, smem, stream, a, shape.tpr);
+    default: return launch_shared(block_norm_backward_kernel<T, true, 2>, grid, block, smem, stream, a, shape.tpr);
   }
 }
 
 template <class T>
 cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, cudaStream_t stream) {
-  a.grad_h_vec = aligned(a.grad_h, a.grad_h_stride, sizeof(T));
-  a.grad_y_vec = a.grad_y && aligned(a.grad_y, a.grad_y_stride, sizeof(T));
-  a.out_vec = aligned(a.dblock, a.cols, sizeof(T)) && aligned(a.dx, a.cols, sizeof(T));
-  a.param_vec = params_aligned(a);
+  a.grad_h_vec = row_align(a.grad_h, a.grad_h_stride, sizeof(T));
+  a.grad_y_vec = row_align(a.grad_y, a.grad_y_stride, sizeof(T));
+  a.out_vec = std::min(row_align(a.dblock, a.cols, sizeof(T)), row_align(a.dx, a.cols, sizeof(T)));
   a.parts = shape.parts;
-  const cudaError_t err = shape.vpt == 1 ? backward_launch<T, 1>(a, shape, stream) : backward_launch<T, 2>(a, shape, stream);
+  const cudaError_t err = backward_launch<T>(a, shape, stream);
   const bool params = a.pre_weight_grad || a.pre_bias_grad || a.post_weight_grad || a.post_bias_grad || a.gate_grad;
   if (err != cudaSuccess || !a.sums || !params) return err;
   cudaLaunchConfig_t cfg{};     // (set up while the first kernel still runs; it waits for that one's end before it reads)
@@ -624,16 +570,14 @@ cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, cudaStr
 
 }  // namespace
 
-// How a pass covers [rows, cols]: 1024 threads for each SM, a thread eight columns (16 in the backward pass beyond 4096).
-BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward) {
+// How a pass covers [rows, cols]: a thread takes sixteen columns, an SM as many threads as the pass's registers allow.
+BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms) {
   BlockNormShape s{};
-  const int chunks = (cols + 31) / 32 * 4;
-  s.vpt = backward && chunks > 512 ? 2 : 1;
-  s.tpr = ((chunks + s.vpt - 1) / s.vpt + 31) / 32 * 32;
+  s.tpr = ((cols + 31) / 32 * 2 + 31) / 32 * 32;
   s.rpb = s.tpr >= 256 ? 1 : 256 / s.tpr;
   const long long length = gate_rows ? gate_rows : rows;
   s.sequences = (int)(length ? rows / length : 0);
-  const long long target = (long long)sms * 1024 / (s.tpr * s.rpb);
+  const long long target = (long long)sms * 512 / (s.tpr * s.rpb);
   long long parts = s.sequences ? target / s.sequences : 1;
   const long long most = (length + s.rpb - 1) / s.rpb;
   if (parts > most) parts = most;
@@ -657,7 +601,7 @@ cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms
 cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
   if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
-  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, true);
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms);
   if (shape.sequences > 65531) return cudaErrorInvalidValue;
   switch (dtype) {
     case kGradF32: return backward_typed<float>(a, shape, stream);
