@@ -40,10 +40,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN where ei
 // Sixteen values of a group whose other half is held by the neighbouring lane (lanes 2i and 2i + 1, both active): their
 // codes, and the group's scale byte.
 __device__ __forceinline__ uint4 act8_encode(const float (&v)[16], unsigned& s) {
-  float m = 0.f;
+  float m[4];      // (four chains of maxima: one would be sixteen latencies long)
 #pragma unroll
-  for (int j = 0; j < 16; ++j) m = max_nan(m, fabsf(v[j]));
-  unsigned top = __float_as_uint(m);     // from here on as integers: a NaN is the largest
+  for (int j = 0; j < 4; ++j) m[j] = max_nan(max_nan(fabsf(v[j]), fabsf(v[j + 4])), max_nan(fabsf(v[j + 8]), fabsf(v[j + 12])));
+  unsigned top = __float_as_uint(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])));     // from here on as integers: a NaN is the largest
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   s = act8_scale_byte(top);
   const float inv = act8_inverse(s);

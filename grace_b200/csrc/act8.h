@@ -59,7 +59,7 @@ struct BlockNormArgs {
   long long grad_h_stride, grad_y_stride;
   void *dx, *dblock;         // contiguous; dx null: it equals dblock
   void *pre_weight_grad, *pre_bias_grad, *post_weight_grad, *post_bias_grad, *gate_grad;   // null: not wanted
-  float* sums;               // [runs][4][pitch] scratch (BlockNormShape)
+  float* sums;               // [runs of the backward pass][4][pitch] scratch (BlockNormShape)
   // filled in by the launchers
   int x_vec, block_vec, out_vec, grad_h_vec, grad_y_vec;   // RowAlign (act8.cuh)
   int parts;
@@ -69,7 +69,7 @@ struct BlockNormShape {
   int tpr, rpb;              // threads a row, rows a CTA
   int sequences, parts, runs;
 };
-BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms);
+BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward);
 cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
 cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
 

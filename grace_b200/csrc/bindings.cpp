@@ -343,7 +343,7 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
   // ---- residual and norm step between two blocks ----
   m.attr("BLOCK_NORM_MAX_COLS") = (int)kBlockNormMaxCols;
   m.def("block_norm_sum_rows", [](long long rows, int cols, long long gate_rows, int sms) {
-    return (long long)block_norm_shape(rows, cols, gate_rows, sms).runs;
+    return (long long)block_norm_shape(rows, cols, gate_rows, sms, true).runs;
   });
   // params: pre_weight, pre_bias, post_weight, post_bias, gate; held: codes and scales of y, block and h
   m.def("block_norm_forward",

@@ -51,6 +51,14 @@ struct SharedRow {
   __device__ __forceinline__ void fill(const BlockNormArgs& a, const void* p, float none) const {
     for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) at[(i & 3) * chunks + (i >> 2)] = load_param<T>(a, p, i * 4, none);
   }
+  template <class T>      // p * q, zeros past the end
+  __device__ __forceinline__ void fill_product(const BlockNormArgs& a, const void* p, const void* q) const {
+    for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
+      const float4 x = load_param<T>(a, p, i * 4, 1.f), y = load_param<T>(a, q, i * 4, 1.f);
+      const int n = a.cols - i * 4;
+      at[(i & 3) * chunks + (i >> 2)] = make_float4(n > 0 ? x.x * y.x : 0.f, n > 1 ? x.y * y.y : 0.f, n > 2 ? x.z * y.z : 0.f, n > 3 ? x.w * y.w : 0.f);
+    }
+  }
   __device__ __forceinline__ void get(int chunk, float (&v)[16]) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -75,32 +83,66 @@ __device__ __forceinline__ const void* gate_of(const BlockNormArgs& a, const Run
   return static_cast<const char*>(a.gate) + run.seq * a.cols * (a.params_f32 ? 4 : (long long)sizeof(T));
 }
 
-// Sums over the `tpr` threads (whole warps) that share a row, the same value in all of them.  Every thread of the CTA
-// calls it.  The two buffers alternate: a warp cannot be two reductions ahead of another.
-template <int N>
+constexpr int kMaxSums = 7;                      // values that one reduction may add up
+constexpr int kSumFloats = 2 * kMaxSums * 32;    // shared memory of the reductions
+
+// Sums over the `tpr` threads (whole warps) that share a row, the same value in all of them: shuffles within a warp, then
+// every thread adds the warps' sums from shared memory (a few 16-byte broadcasts take less time than five more
+// shuffles).  Every thread of the CTA calls it.  Two buffers alternate: a warp cannot be two reductions ahead of another.
 struct RowSum {
-  float* buf;      // [2][64], whatever N is: reductions of one and of two values may alternate
-  int parity, tpr;
+  float* buf;
+  int parity, warps, first, warp;   // warps of a row, the first of this row's, this one
+  __device__ __forceinline__ RowSum(float* b, int tpr) : buf(b), parity(0), warps(tpr >> 5), warp(threadIdx.x >> 5) { first = warp / warps * warps; }
   __device__ __forceinline__ float* next() {
-    float* const b = buf + parity * 64;
+    float* const b = buf + parity * (kMaxSums * 32);
     parity ^= 1;
     return b;
   }
+  // w[warp] = x of each of the row's warps, visible after the next barrier; the same for all of the row's threads
+  __device__ __forceinline__ float total(const float* w) const {
+    float s = 0.f;
+    if ((warps & 3) == 0) {
+      for (int i = 0; i < warps; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(w + first + i);
+        s += (x.x + x.y) + (x.z + x.w);
+      }
+    } else {
+      for (int i = 0; i < warps; ++i) s += w[first + i];
+    }
+    return s;
+  }
+  template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N]) {
+    static_assert(N <= kMaxSums, "");
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-    if (tpr == 32) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = tpr >> 5, first = warp / warps * warps;
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (warps == 1) return;
     float* const b = next();
-    if (lane == 0) {
+    if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) b[warp * N + i] = v[i];
+      for (int i = 0; i < N; ++i) b[i * 32 + warp] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? b[(first + lane) * N + i] : 0.f);
+    for (int i = 0; i < N; ++i) v[i] = total(b + i * 32);
   }
 };
+
+// sum of a[j] b[j], in four chains
+__device__ __forceinline__ float dot16(const float (&a)[16], const float (&b)[16]) {
+  float s[4] = {};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s[j & 3] = fmaf(a[j], b[j], s[j & 3]);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+__device__ __forceinline__ float sum16(const float (&a)[16]) {
+  float s[4] = {};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s[j & 3] += a[j];
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
 
 // 1 / sqrt(x): the hardware's estimate and one Newton step
 __device__ __forceinline__ float inv_sqrt(float x) {
@@ -111,43 +153,34 @@ __device__ __forceinline__ float inv_sqrt(float x) {
 // (mean, 1 / deviation) of a row, sixteen columns a thread.  Layer norm: each warp's mean and squared deviations from
 // it, joined over the warps by Chan, Golub and LeVeque's formula, so that one barrier does and nothing cancels.
 template <bool LAYER>
-__device__ __forceinline__ float2 row_stats(const float (&v)[16], int valid, int cols, float inv_cols, float eps, RowSum<2>& sum) {
-  const int lane = threadIdx.x & 31, warps = sum.tpr >> 5, warp = threadIdx.x >> 5, first = warp / warps * warps;
+__device__ __forceinline__ float2 row_stats(const float (&v)[16], int valid, int cols, float inv_cols, float eps, RowSum& sum) {
   if (!LAYER) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s = fmaf(v[j], v[j], s);   // (columns past the end are zeros)
-    s = warp_sum(s);
-    if (warps > 1) {
-      float* const b = sum.next();
-      if (lane == 0) b[warp] = s;
-      __syncthreads();
-      s = warp_sum(lane < warps ? b[first + lane] : 0.f);
-    }
-    return make_float2(0.f, inv_sqrt(fmaf(s, inv_cols, eps)));
+    float s[1] = {dot16(v, v)};      // (columns past the end are zeros)
+    sum(s);
+    return make_float2(0.f, inv_sqrt(fmaf(s[0], inv_cols, eps)));
   }
-  const float n = (float)min(512, max(0, cols - (warp - first) * 512));
-  float m = 0.f, d = 0.f;
+  const float n = (float)min(512, max(0, cols - (sum.warp - sum.first) * 512));
+  const float inv_n = n > 0.f ? __fdividef(1.f, n) : 0.f;
+  float m = warp_sum(sum16(v)) * inv_n, d;
+  float x[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) m += v[j];
-  m = n > 0.f ? __fdividef(warp_sum(m), n) : 0.f;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const float x = j < valid ? v[j] - m : 0.f;
-    d = fmaf(x, x, d);
-  }
-  d = warp_sum(d);
-  if (warps > 1) {
+  for (int j = 0; j < 16; ++j) x[j] = j < valid ? v[j] - m : 0.f;
+  d = warp_sum(dot16(x, x));
+  if (sum.warps > 1) {
     float* const b = sum.next();
-    if (lane == 0) {
-      b[warp * 2] = m;
-      b[warp * 2 + 1] = d;
+    if ((threadIdx.x & 31) == 0) {
+      b[sum.warp] = m;
+      b[32 + sum.warp] = d;
     }
     __syncthreads();
-    const float nl = lane < warps ? (float)min(512, max(0, cols - lane * 512)) : 0.f;
-    const float ml = lane < warps ? b[(first + lane) * 2] : 0.f;
-    m = warp_sum(nl * ml) * inv_cols;
-    d = warp_sum(lane < warps ? fmaf(nl * (ml - m), ml - m, b[(first + lane) * 2 + 1]) : 0.f);
+    float total = 0.f;
+    for (int i = 0; i < sum.warps; ++i) total = fmaf((float)min(512, max(0, cols - i * 512)), b[sum.first + i], total);
+    m = total * inv_cols;
+    d = 0.f;
+    for (int i = 0; i < sum.warps; ++i) {
+      const float off = b[sum.first + i] - m;
+      d += fmaf((float)min(512, max(0, cols - i * 512)) * off, off, b[32 + sum.first + i]);
+    }
   }
   return make_float2(m, inv_sqrt(fmaf(d, inv_cols, eps)));
 }
@@ -184,9 +217,10 @@ __device__ __forceinline__ void scaled_sum(float alpha, const float (&x)[16], fl
   for (int j = 0; j < 16; ++j) v[j] = y[j];
 }
 
-template <class T, bool PRE_LAYER, int POST>
-__global__ void __launch_bounds__(512) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
-  __shared__ float buf[2 * 64];
+// THREADS: 256 where a row takes no more, three CTAs an SM; 512
+template <class T, bool PRE_LAYER, int POST, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
+  __shared__ __align__(16) float buf[kSumFloats];
   extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
   const int col = t * 16, valid = min(16, max(0, a.cols - col)), chunks = a.held_y.pitch / 16;
@@ -194,7 +228,7 @@ __global__ void __launch_bounds__(512) block_norm_forward_kernel(const BlockNorm
   const int chunk = owns ? t : 0;
   const float inv_cols = 1.f / (float)a.cols;
   const Run run = run_of(a);
-  RowSum<2> sum{buf, 0, tpr};
+  RowSum sum(buf, tpr);
   Chunk16<T> cb, cx;
   auto load = [&](long long row) {
     if (row < run.row1) {
@@ -321,106 +355,113 @@ __device__ __forceinline__ void decode_normed(uint4 codes, unsigned s, float mea
   for (int j = 0; j < 16; ++j) v[j] = (LAYER ? v[j] - mean : v[j]) * rstd;
 }
 
-// BLOCK: 0 neither a norm after the block nor a gate, so that b~ is not read; 1 either, without sums of g (G0); 2 with them
-// (a layer norm after the block).
-template <class T, bool PRE_LAYER, int BLOCK>
+// POST: what b~ is read for.  kNoBlock: nothing (neither a norm after the block nor a gate); kGateOnly; an RMS norm, a
+// layer norm, each with or without a gate.
+//
+// The norm backward after the block needs sums over g, which itself needs sums over the row.  One reduction does for
+// both: with f = r c + dy and u = gate w_post,
+//   g = f - k1 y^ - k0,  k1 = r mean(c y^),  k0 = r mean(c) (layer norm before the next block, else 0),
+//   sum u g b^ = sum f u b^ - k1 sum y^ u b^ - k0 sum u b^,      sum u g = sum f u - k1 sum y^ u - k0 sum u,
+// where every sum on the right is known before k1 and k0 are; a second round through the barrier cost a quarter of the
+// kernel.
+enum BlockUse : int { kNoBlock = 0, kGateOnly = 1, kBlockRms = 2, kBlockLayer = 3 };
+
+template <class T, bool PRE_LAYER, int POST>
 __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNormArgs a, int tpr) {
-  constexpr bool TWO = BLOCK > 0;
-  constexpr int B = TWO ? 16 : 1, L = PRE_LAYER ? 16 : 1, Z = BLOCK == 2 ? 16 : 1;
-  __shared__ float buf[2 * 64];
+  constexpr bool TWO = POST != kNoBlock, NORM = POST >= kBlockRms, LAYER = POST == kBlockLayer;
+  constexpr int B = TWO ? 16 : 1, L = PRE_LAYER ? 16 : 1, Z = LAYER ? 16 : 1;
+  // the sums of a row: c y^ | c | f u b^, y^ u b^ | u b^ | f u, y^ u
+  constexpr int kC = 1, kB = kC + (PRE_LAYER ? 1 : 0), kD = kB + (NORM ? 2 : 0), kE = kD + (NORM && PRE_LAYER ? 1 : 0), kN = kE + (LAYER ? 2 : 0);
+  __shared__ __align__(16) float buf[kSumFloats];
   extern __shared__ float4 params[];
   const int rpb = blockDim.x / tpr, lane_row = threadIdx.x / tpr, t = threadIdx.x - lane_row * tpr;
   const int chunks = a.held_y.pitch / 16, chunk = t < chunks ? t : 0, col = t * 16;
   const float inv_cols = 1.f / (float)a.cols;
   const Run run = run_of(a);
-  RowSum<2> sum2{buf, 0, tpr};
-  const bool post = TWO && a.post != kNormNone;
+  RowSum sum(buf, tpr);
   float dw[16] = {}, db[L] = {}, g1[B] = {}, g0[Z] = {};
 
   RowLoads<T, TWO> r;
   r.load(a, run.row0 + lane_row, col, run.row0 + lane_row < run.row1);
-  int used = 0;
-  auto shared_row = [&](const void* p, float none) {
-    const SharedRow r{params + 4 * chunks * used++, chunks};
-    r.template fill<T>(a, p, none);
-    return r;
-  };
-  const SharedRow pre_w = shared_row(a.pre_weight, 1.f);
-  const SharedRow post_w = post ? shared_row(a.post_weight, 1.f) : pre_w;
-  const SharedRow gate = a.gate ? shared_row(gate_of<T>(a, run), 0.f) : pre_w;
+  const SharedRow pre_w{params, chunks}, u_row{params + 4 * chunks, chunks};
+  pre_w.template fill<T>(a, a.pre_weight, 1.f);
+  if (TWO) u_row.template fill_product<T>(a, gate_of<T>(a, run), a.post_weight);
   __syncthreads();
+  float sum_u = 0.f;
+  if constexpr (LAYER && PRE_LAYER) {
+    float u[16], s[1];
+    u_row.get(chunk, u);
+    s[0] = t < chunks ? sum16(u) : 0.f;
+    sum(s);
+    sum_u = s[0];
+  }
 
   for (long long base = run.row0; base < run.row1; base += rpb) {
     const long long row = base + lane_row;
     const bool in = row < run.row1;
-    float c[16], hat[16], bh[B], w[16], s[2] = {0.f, 0.f};
+    float f[16], hat[16], bh[B], w[16], s[kN];
     const float4 stats = r.stats;
-    const Chunk16<T> dy = r.dy;
-    auto row_sum = [&](bool both) {
-      if (both) {
-        sum2(s);
-      } else {
-        RowSum<1> sum1{buf, sum2.parity, tpr};   // (the two share their buffers)
-        float v[1] = {s[0]};
-        sum1(v);
-        s[0] = v[0];
-        sum2.parity = sum1.parity;
-      }
-    };
-    r.dh.get(c);
+    r.dh.get(f);
     decode_normed<PRE_LAYER>(r.qy, r.sy, stats.x, stats.y, hat);
     pre_w.get(chunk, w);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      dw[j] = fmaf(c[j], hat[j], dw[j]);
-      if (PRE_LAYER) db[PRE_LAYER ? j : 0] += c[j];
-      c[j] *= w[j];
-      s[0] = fmaf(c[j], hat[j], s[0]);
-      if (PRE_LAYER) s[1] += c[j];
+      dw[j] = fmaf(f[j], hat[j], dw[j]);
+      if (PRE_LAYER) db[PRE_LAYER ? j : 0] += f[j];
+      f[j] *= w[j];                                  // c
     }
-    if constexpr (TWO) decode_normed<BLOCK == 2>(r.qb, r.sb, stats.z, stats.w, bh);
-    r.load(a, row + rpb, col, row + rpb < run.row1);     // the next row's loads are under way during the sums
-    row_sum(PRE_LAYER);
-    const float m1 = s[0] * inv_cols, m0 = PRE_LAYER ? s[1] * inv_cols : 0.f;
-    s[0] = s[1] = 0.f;
-    dy.get(w);
+    s[0] = dot16(f, hat);
+    if constexpr (PRE_LAYER) s[kC] = sum16(f);
+    r.dy.get(w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) c[j] = fmaf(stats.y, fmaf(-hat[j], m1, PRE_LAYER ? c[j] - m0 : c[j]), w[j]);   // g
+    for (int j = 0; j < 16; ++j) f[j] = fmaf(stats.y, f[j], w[j]);
+    if constexpr (TWO) decode_normed<LAYER>(r.qb, r.sb, stats.z, stats.w, bh);
+    r.load(a, row + rpb, col, row + rpb < run.row1);     // the next row's loads are under way during the sums
+    if constexpr (NORM) {
+      u_row.get(chunk, w);
+      if constexpr (LAYER) {
+        s[kE] = dot16(f, w);
+        s[kE + 1] = dot16(hat, w);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] *= bh[j];      // (u is zero past the end of the row)
+      s[kB] = dot16(f, w);
+      s[kB + 1] = dot16(hat, w);
+      if constexpr (PRE_LAYER) s[kD] = sum16(w);
+      if (t >= chunks) {
+#pragma unroll
+        for (int i = kB; i < kN; ++i) s[i] = 0.f;      // (a thread past the row's end holds another chunk's u)
+      }
+    }
+    sum(s);
+    const float k1 = stats.y * s[0] * inv_cols, k0 = PRE_LAYER ? stats.y * s[PRE_LAYER ? kC : 0] * inv_cols : 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = fmaf(-k1, hat[j], PRE_LAYER ? f[j] - k0 : f[j]);   // g
     if (in && a.dx) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] = a.alpha * c[j];
+      for (int j = 0; j < 16; ++j) w[j] = a.alpha * f[j];
       store16(w, static_cast<T*>(a.dx) + row * a.cols, col, a.cols, a.out_vec);
     }
     if constexpr (TWO) {
       if (!in || col + 16 > a.cols) {   // what does not exist adds nothing
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c[j] = in && col + j < a.cols ? c[j] : 0.f;
+        for (int j = 0; j < 16; ++j) f[j] = in && col + j < a.cols ? f[j] : 0.f;
       }
+      u_row.get(chunk, w);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        g1[j] = fmaf(c[j], bh[j], g1[j]);
-        if (BLOCK == 2) g0[BLOCK == 2 ? j : 0] += c[j];
+        g1[j] = fmaf(f[j], bh[j], g1[j]);
+        if (LAYER) g0[LAYER ? j : 0] += f[j];
+        f[j] *= w[j];
       }
-      if (a.gate) {
-        gate.get(chunk, w);
+      if constexpr (NORM) {
+        const float p1 = (s[kB] - k1 * s[kB + 1] - (PRE_LAYER ? k0 * s[PRE_LAYER ? kD : 0] : 0.f)) * inv_cols;
+        const float p0 = LAYER ? (s[LAYER ? kE : 0] - k1 * s[LAYER ? kE + 1 : 0] - k0 * sum_u) * inv_cols : 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c[j] *= w[j];
-      }
-      if (post) {
-        post_w.get(chunk, w);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          c[j] *= w[j];
-          s[0] = fmaf(c[j], bh[j], s[0]);
-          if (BLOCK == 2) s[1] += c[j];
-        }
-        row_sum(BLOCK == 2);
-        const float p1 = s[0] * inv_cols, p0 = BLOCK == 2 ? s[1] * inv_cols : 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) c[j] = stats.w * fmaf(-bh[j], p1, BLOCK == 2 ? c[j] - p0 : c[j]);
+        for (int j = 0; j < 16; ++j) f[j] = stats.w * fmaf(-bh[j], p1, LAYER ? f[j] - p0 : f[j]);
       }
     }
-    if (in) store16(c, static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
+    if (in) store16(f, static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
   }
   if (!a.sums) return;
   // This run's sums: [4][pitch] floats.  The CTA's row lanes are added in order, each on top of the one before it.
@@ -448,13 +489,13 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
     put(0, dw);
     if constexpr (PRE_LAYER) put(1, db);
     if constexpr (TWO) put(2, g1);
-    if constexpr (BLOCK == 2) put(3, g0);
+    if constexpr (LAYER) put(3, g0);
   }
 }
 
-// Adds the runs' sums.  Block: 32 columns x 32 lanes of runs.  blockIdx.y 0 .. 3: one of the norms' parameters, over all
+// Adds the runs' sums.  Block: 32 columns x 8 lanes of runs.  blockIdx.y 0 .. 3: one of the norms' parameters, over all
 // runs; 4 + s: the gate of sequence s.
-constexpr int kLanes = 32;
+constexpr int kLanes = 8;
 template <class T>
 __global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const BlockNormArgs a, int runs, int gates) {
   __shared__ float part[2][kLanes][33];
@@ -473,7 +514,7 @@ __global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const Bloc
   cudaGridDependencySynchronize();
   float v = 0.f, z = 0.f;
   const float* p = a.sums + (long long)(first + lane) * 4 * pitch + which * pitch + col;
-#pragma unroll 4
+#pragma unroll 8
   for (int u = first + lane; u < last; u += kLanes, p += kLanes * 4 * pitch) {
     float x = *p;
     if (weigh && a.gate_rows) x *= param(a.gate, (long long)(u / per_gate) * a.cols + col);
@@ -483,17 +524,19 @@ __global__ void __launch_bounds__(32 * kLanes) block_norm_sums_kernel(const Bloc
   part[0][lane][threadIdx.x] = v;
   part[1][lane][threadIdx.x] = z;
   __syncthreads();
-  // a warp for each of the block's columns
-  const int c = threadIdx.y, at = blockIdx.x * 32 + c;
-  v = warp_sum(part[0][threadIdx.x][c]);
-  z = warp_sum(part[1][threadIdx.x][c]);
-  if (threadIdx.x != 0 || at >= a.cols) return;
+  if (lane != 0 || col >= a.cols) return;
+  v = z = 0.f;
+#pragma unroll
+  for (int l = 0; l < kLanes; ++l) {
+    v += part[0][l][threadIdx.x];
+    z += part[1][l][threadIdx.x];
+  }
   auto put = [&](void* to, long long i, float x) {
     if (a.params_f32) static_cast<float*>(to)[i] = x;
     else static_cast<T*>(to)[i] = from_f32<T>(x);
   };
-  if (for_gate) put(a.gate_grad, (long long)seq * a.cols + at, (a.post_weight ? param(a.post_weight, at) : 1.f) * v + (second ? param(a.post_bias, at) * z : 0.f));
-  else put(grads[which], at, weigh && !a.gate_rows ? v * param(a.gate, at) : v);
+  if (for_gate) put(a.gate_grad, (long long)seq * a.cols + col, (a.post_weight ? param(a.post_weight, col) : 1.f) * v + (second ? param(a.post_bias, col) * z : 0.f));
+  else put(grads[which], col, weigh && !a.gate_rows ? v * param(a.gate, col) : v);
 }
 
 template <class K>
@@ -511,39 +554,53 @@ cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   a.x_vec = row_align(a.x, a.x_stride, sizeof(T));
   a.block_vec = row_align(a.block, a.block_stride, sizeof(T));
   a.out_vec = std::min(row_align(a.h, a.cols, sizeof(T)), row_align(a.y, a.cols, sizeof(T)));
-  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms);
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, false);
   a.parts = shape.parts;
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
   const bool layer = a.pre == kNormLayer;
   const int rows = 1 + (layer ? 1 : 0) + (a.post ? 1 : 0) + (a.post == kNormLayer ? 1 : 0) + (a.gate ? 1 : 0);
   const size_t smem = (size_t)rows * a.held_y.pitch * 4;
+  auto go = [&](auto kernel) { return launch_shared(kernel, grid, block, smem, stream, a, shape.tpr); };
+  if (block.x > 256) {
+    switch (a.post * 2 + (layer ? 1 : 0)) {
+      case 0: return go(block_norm_forward_kernel<T, false, kNormNone, 512>);
+      case 1: return go(block_norm_forward_kernel<T, true, kNormNone, 512>);
+      case 2: return go(block_norm_forward_kernel<T, false, kNormRms, 512>);
+      case 3: return go(block_norm_forward_kernel<T, true, kNormRms, 512>);
+      case 4: return go(block_norm_forward_kernel<T, false, kNormLayer, 512>);
+      default: return go(block_norm_forward_kernel<T, true, kNormLayer, 512>);
+    }
+  }
   switch (a.post * 2 + (layer ? 1 : 0)) {
-    case 0: return launch_shared(block_norm_forward_kernel<T, false, kNormNone>, grid, block, smem, stream, a, shape.tpr);
-    case 1: return launch_shared(block_norm_forward_kernel<T, true, kNormNone>, grid, block, smem, stream, a, shape.tpr);
-    case 2: return launch_shared(block_norm_forward_kernel<T, false, kNormRms>, grid, block, smem, stream, a, shape.tpr);
-    case 3: return launch_shared(block_norm_forward_kernel<T, true, kNormRms>, grid, block, smem, stream, a, shape.tpr);
-    case 4: return launch_shared(block_norm_forward_kernel<T, false, kNormLayer>, grid, block, smem, stream, a, shape.tpr);
-    default: return launch_shared(block_norm_forward_kernel<T, true, kNormLayer>, grid, block, smem, stream, a, shape.tpr);
+    case 0: return go(block_norm_forward_kernel<T, false, kNormNone, 256>);
+    case 1: return go(block_norm_forward_kernel<T, true, kNormNone, 256>);
+    case 2: return go(block_norm_forward_kernel<T, false, kNormRms, 256>);
+    case 3: return go(block_norm_forward_kernel<T, true, kNormRms, 256>);
+    case 4: return go(block_norm_forward_kernel<T, false, kNormLayer, 256>);
+    default: return go(block_norm_forward_kernel<T, true, kNormLayer, 256>);
   }
 }
 
 template <class T>
 cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape, cudaStream_t stream) {
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
-  const int form = a.held_b.codes == nullptr ? 0 : (a.post == kNormLayer ? 2 : 1);
+  const int use = a.held_b.codes == nullptr ? kNoBlock : (a.post == kNormNone ? kGateOnly : (a.post == kNormRms ? kBlockRms : kBlockLayer));
   const bool layer = a.pre == kNormLayer;
   // the parameters, or (several row lanes) the sums on their way from lane to lane
-  int rows = 1 + (a.post ? 1 : 0) + (a.gate ? 1 : 0);
-  const int sums = 1 + (layer ? 1 : 0) + form;
+  int rows = 1 + (use ? 1 : 0);
+  const int sums = 1 + (layer ? 1 : 0) + (use ? 1 : 0) + (use == kBlockLayer ? 1 : 0);
   if (shape.rpb > 1 && sums > rows) rows = sums;
   const size_t smem = (size_t)rows * a.held_y.pitch * 4;
-  switch (form * 2 + (layer ? 1 : 0)) {
-    case 0: return launch_shared(block_norm_backward_kernel<T, false, 0>, grid, block, smem, stream, a, shape.tpr);
-    case 1: return launch_shared(block_norm_backward_kernel<T, true, 0>, grid, block, smem, stream, a, shape.tpr);
-    case 2: return launch_shared(block_norm_backward_kernel<T, false, 1>, grid, block, smem, stream, a, shape.tpr);
-    case 3: return launch_shared(block_norm_backward_kernel<T, true, 1>, grid, block, smem, stream, a, shape.tpr);
-    case 4: return launch_shared(block_norm_backward_kernel<T, false, 2>, grid, block, smem, stream, a, shape.tpr);
-    default: return launch_shared(block_norm_backward_kernel<T, true, 2>, grid, block, smem, stream, a, shape.tpr);
+  auto go = [&](auto kernel) { return launch_shared(kernel, grid, block, smem, stream, a, shape.tpr); };
+  switch (use * 2 + (layer ? 1 : 0)) {
+    case 0: return go(block_norm_backward_kernel<T, false, kNoBlock>);
+    case 1: return go(block_norm_backward_kernel<T, true, kNoBlock>);
+    case 2: return go(block_norm_backward_kernel<T, false, kGateOnly>);
+    case 3: return go(block_norm_backward_kernel<T, true, kGateOnly>);
+    case 4: return go(block_norm_backward_kernel<T, false, kBlockRms>);
+    case 5: return go(block_norm_backward_kernel<T, true, kBlockRms>);
+    case 6: return go(block_norm_backward_kernel<T, false, kBlockLayer>);
+    default: return go(block_norm_backward_kernel<T, true, kBlockLayer>);
   }
 }
 
@@ -571,13 +628,13 @@ cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, cudaStr
 }  // namespace
 
 // How a pass covers [rows, cols]: a thread takes sixteen columns, an SM as many threads as the pass's registers allow.
-BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms) {
+BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward) {
   BlockNormShape s{};
   s.tpr = ((cols + 31) / 32 * 2 + 31) / 32 * 32;
   s.rpb = s.tpr >= 256 ? 1 : 256 / s.tpr;
   const long long length = gate_rows ? gate_rows : rows;
   s.sequences = (int)(length ? rows / length : 0);
-  const long long target = (long long)sms * 512 / (s.tpr * s.rpb);
+  const long long target = (long long)sms * (backward || s.tpr > 256 ? 512 : 768) / (s.tpr * s.rpb);
   long long parts = s.sequences ? target / s.sequences : 1;
   const long long most = (length + s.rpb - 1) / s.rpb;
   if (parts > most) parts = most;
@@ -601,7 +658,7 @@ cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms
 cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
   if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
-  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms);
+  const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, true);
   if (shape.sequences > 65531) return cudaErrorInvalidValue;
   switch (dtype) {
     case kGradF32: return backward_typed<float>(a, shape, stream);
