@@ -47,18 +47,7 @@ __device__ __forceinline__ float4 load_param(const BlockNormArgs& a, const void*
 struct SharedRow {
   float4* at;
   int chunks;
-  template <class T>
-  __device__ __forceinline__ void fill(const BlockNormArgs& a, const void* p, float none) const {
-    for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) at[(i & 3) * chunks + (i >> 2)] = load_param<T>(a, p, i * 4, none);
-  }
-  template <class T>      // p * q, zeros past the end
-  __device__ __forceinline__ void fill_product(const BlockNormArgs& a, const void* p, const void* q) const {
-    for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
-      const float4 x = load_param<T>(a, p, i * 4, 1.f), y = load_param<T>(a, q, i * 4, 1.f);
-      const int n = a.cols - i * 4;
-      at[(i & 3) * chunks + (i >> 2)] = make_float4(n > 0 ? x.x * y.x : 0.f, n > 1 ? x.y * y.y : 0.f, n > 2 ? x.z * y.z : 0.f, n > 3 ? x.w * y.w : 0.f);
-    }
-  }
+  __device__ __forceinline__ void put(int i, float4 v) const { at[(i & 3) * chunks + (i >> 2)] = v; }   // columns 4 i .. 4 i + 3
   __device__ __forceinline__ void get(int chunk, float (&v)[16]) const {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -67,6 +56,10 @@ struct SharedRow {
     }
   }
 };
+__device__ __forceinline__ float4 times(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
+__device__ __forceinline__ float4 first_of(float4 v, int n) {    // its first n numbers, then zeros
+  return make_float4(n > 0 ? v.x : 0.f, n > 1 ? v.y : 0.f, n > 2 ? v.z : 0.f, n > 3 ? v.w : 0.f);
+}
 
 // The rows of this CTA's run: run = sequence * parts + part, rows [part * L / parts, (part + 1) * L / parts) of the
 // sequence, L = gate_rows (all rows are one sequence where no gate belongs to a sequence).
@@ -144,10 +137,13 @@ __device__ __forceinline__ float sum16(const float (&a)[16]) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// 1 / sqrt(x): the hardware's estimate and one Newton step
-__device__ __forceinline__ float inv_sqrt(float x) {
-  const float r = rsqrtf(x);
-  return r * fmaf(-0.5f * x * r, r, 1.5f);
+// 1 / sqrt(sum / cols + eps): the quotient and the hardware's root each with one correction by their remainder.  An error
+// here is one of the whole row, all of whose values it would push the same way across the borders of their rounding.
+__device__ __forceinline__ float inv_deviation(float sum, float cols, float inv_cols, float eps) {
+  float x = sum * inv_cols;
+  x = fmaf(fmaf(-x, cols, sum), inv_cols, x) + eps;
+  const float r = rsqrtf(x), h = x * r;
+  return fmaf(0.5f * r, fmaf(-h, r, 1.f), r);
 }
 
 // (mean, 1 / deviation) of a row, sixteen columns a thread.  Layer norm: each warp's mean and squared deviations from
@@ -157,7 +153,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[16], int valid, int
   if (!LAYER) {
     float s[1] = {dot16(v, v)};      // (columns past the end are zeros)
     sum(s);
-    return make_float2(0.f, inv_sqrt(fmaf(s[0], inv_cols, eps)));
+    return make_float2(0.f, inv_deviation(s[0], (float)cols, inv_cols, eps));
   }
   const float n = (float)min(512, max(0, cols - (sum.warp - sum.first) * 512));
   const float inv_n = n > 0.f ? __fdividef(1.f, n) : 0.f;
@@ -182,7 +178,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[16], int valid, int
       d += fmaf((float)min(512, max(0, cols - i * 512)) * off, off, b[32 + sum.first + i]);
     }
   }
-  return make_float2(m, inv_sqrt(fmaf(d, inv_cols, eps)));
+  return make_float2(m, inv_deviation(d, (float)cols, inv_cols, eps));
 }
 
 // The codes at columns col .. col + 15 of a row and, from the lane with a group's first columns, its scale byte.
@@ -240,17 +236,21 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
     }
   };
   load(run.row0 + lane_row);
-  int used = 0;
-  auto shared_row = [&](const void* p, float none) {
-    const SharedRow r{params + 4 * chunks * used++, chunks};
-    r.template fill<T>(a, p, none);
-    return r;
-  };
-  const SharedRow pre_w = shared_row(a.pre_weight, 1.f);
-  const SharedRow pre_b = PRE_LAYER ? shared_row(a.pre_bias, 0.f) : pre_w;
-  const SharedRow post_w = POST ? shared_row(a.post_weight, 1.f) : pre_w;
-  const SharedRow post_b = POST == kNormLayer ? shared_row(a.post_bias, 0.f) : pre_w;
-  const SharedRow gate = a.gate ? shared_row(gate_of<T>(a, run), 0.f) : pre_w;
+  // The norm after the block and the gate as one factor (and one summand) for each column.
+  constexpr bool BIAS = POST == kNormLayer;
+  const bool scaled = POST || a.gate;
+  const SharedRow pre_w{params, chunks}, pre_b{params + 4 * chunks, chunks};
+  const SharedRow u_row{params + (PRE_LAYER ? 8 : 4) * chunks, chunks}, ub_row{u_row.at + 4 * chunks, chunks};
+  const void* const g = gate_of<T>(a, run);
+  for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
+    const float4 w = load_param<T>(a, a.pre_weight, i * 4, 1.f), b = load_param<T>(a, a.pre_bias, i * 4, 0.f);
+    const float4 u = load_param<T>(a, a.post_weight, i * 4, 1.f), ub = load_param<T>(a, a.post_bias, i * 4, 0.f);
+    const float4 f = load_param<T>(a, g, i * 4, 1.f);
+    pre_w.put(i, w);
+    if (PRE_LAYER) pre_b.put(i, b);
+    if (scaled) u_row.put(i, times(u, f));
+    if (BIAS) ub_row.put(i, times(ub, f));
+  }
   __syncthreads();
 
   for (long long base = run.row0; base < run.row1; base += rpb) {
@@ -264,21 +264,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
       if (in && owns) put_codes(a.held_b, row, col, codes, s);
     }
     float2 post = make_float2(0.f, 1.f);
-    if (POST) {
-      post = row_stats<POST == kNormLayer>(v, valid, a.cols, inv_cols, a.eps, sum);
-      post_w.get(chunk, w);
+    if (POST) post = row_stats<POST == kNormLayer>(v, valid, a.cols, inv_cols, a.eps, sum);
+    if (scaled) {
+      u_row.get(chunk, w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y * w[j];
-      if (POST == kNormLayer) {
-        post_b.get(chunk, w);
+      for (int j = 0; j < 16; ++j) v[j] = (POST ? (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y : v[j]) * w[j];
+      if (BIAS) {
+        ub_row.get(chunk, w);
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] += w[j];
       }
-    }
-    if (a.gate) {
-      gate.get(chunk, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] *= w[j];
     }
     cx.get(w);
     scaled_sum<T>(a.alpha, w, v);
@@ -384,8 +379,13 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
   RowLoads<T, TWO> r;
   r.load(a, run.row0 + lane_row, col, run.row0 + lane_row < run.row1);
   const SharedRow pre_w{params, chunks}, u_row{params + 4 * chunks, chunks};
-  pre_w.template fill<T>(a, a.pre_weight, 1.f);
-  if (TWO) u_row.template fill_product<T>(a, gate_of<T>(a, run), a.post_weight);
+  const void* const gate = gate_of<T>(a, run);
+  for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
+    const float4 w = load_param<T>(a, a.pre_weight, i * 4, 1.f);
+    const float4 u = load_param<T>(a, a.post_weight, i * 4, 1.f), v = load_param<T>(a, gate, i * 4, 1.f);
+    pre_w.put(i, w);
+    if (TWO) u_row.put(i, first_of(times(u, v), a.cols - i * 4));
+  }
   __syncthreads();
   float sum_u = 0.f;
   if constexpr (LAYER && PRE_LAYER) {
@@ -558,7 +558,7 @@ cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   a.parts = shape.parts;
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
   const bool layer = a.pre == kNormLayer;
-  const int rows = 1 + (layer ? 1 : 0) + (a.post ? 1 : 0) + (a.post == kNormLayer ? 1 : 0) + (a.gate ? 1 : 0);
+  const int rows = 1 + (layer ? 1 : 0) + (a.post || a.gate ? 1 : 0) + (a.post == kNormLayer ? 1 : 0);
   const size_t smem = (size_t)rows * a.held_y.pitch * 4;
   auto go = [&](auto kernel) { return launch_shared(kernel, grid, block, smem, stream, a, shape.tpr); };
   if (block.x > 256) {

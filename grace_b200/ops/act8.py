@@ -161,6 +161,19 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def _at(x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """``_rows`` for a launch: the tensor to keep until then, its address, and the distance between its rows."""
+    if x.is_contiguous():      # no view is made: that would take longer than the checks of the whole call
+        return x, x.data_ptr(), x.shape[-1]
+    x = _rows(x)
+    return x, x.data_ptr(), x.stride(0)
+
+
+def _new_like(x: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``x``'s shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _ptrs(held: Optional[Act8]) -> Tuple[int, int]:
     """Addresses of a checkpoint's codes and scales."""
     if held is None:
@@ -214,8 +227,8 @@ def pack(x: torch.Tensor) -> Act8:
     device = x.device
     held = empty_like(x.shape, x.dtype, device)
     if x.is_cuda:
-        v = _rows(x)
-        _launch(device, native().act8_pack, v.data_ptr(), v.stride(0), held.rows, held.shape[-1], GRAD_DTYPE[x.dtype], *_ptrs(held),
+        v, at, stride = _at(x)
+        _launch(device, native().act8_pack, at, stride, held.rows, held.shape[-1], GRAD_DTYPE[x.dtype], *_ptrs(held),
                 held.pitch, held.spitch)
     else:
         _encode_cpu(x, held)
@@ -271,17 +284,18 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
     if rows == 0 or outs == 0 or ins == 0:
         return (torch.zeros((outs, ins), dtype=dtype, device=grad.device),
                 torch.zeros(outs, dtype=dtype, device=grad.device) if bias else None)
-    C, g, device = native(), _rows(grad), grad.device
-    if g.data_ptr() % 16 or g.stride(0) % 8 or g.stride(0) < outs:   # not what a TMA load takes
+    C, device = native(), grad.device
+    g, at, stride = _at(grad)
+    if at % 16 or stride % 8 or stride < outs:   # not what a TMA load takes
         wide = torch.empty((rows, -(-outs // 8) * 8), dtype=g.dtype, device=device)
-        _launch(device, C.act8_repitch, g.data_ptr(), g.stride(0), wide.data_ptr(), rows, outs)
-        g = wide
+        _launch(device, C.act8_repitch, at, stride, wide.data_ptr(), rows, outs)
+        g, at, stride = wide, wide.data_ptr(), wide.shape[1]
     out = torch.empty((outs, ins), dtype=dtype, device=device)
     db = torch.empty(outs, dtype=dtype, device=device) if bias else None
     f32, sms = int(dtype == torch.float32), _sms(device)
     nbytes = C.act8_wgrad_work_bytes(rows, outs, ins, f32, sms)
     work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _launch(device, C.act8_wgrad, g.data_ptr(), g.stride(0), *_ptrs(held), held.pitch, held.spitch, rows, outs, ins, GRAD_DTYPE[g.dtype],
+    _launch(device, C.act8_wgrad, at, stride, *_ptrs(held), held.pitch, held.spitch, rows, outs, ins, GRAD_DTYPE[g.dtype],
             f32, out.data_ptr(), db.data_ptr() if bias else 0, 0 if work is None else work.data_ptr(), sms)
     return out, db
 
@@ -327,8 +341,9 @@ def activation_forward(x: torch.Tensor, kind: str = "gelu", gated: bool = False,
     if checkpoint_output:
         out = empty_like(shape, dtype, device)
     if x.is_cuda:
-        y, v = torch.empty(shape, dtype=dtype, device=device), _rows(x)
-        _launch(device, native().act8_forward, v.data_ptr(), v.stride(0), y.data_ptr(), v.shape[0], cols, GRAD_DTYPE[dtype], k, int(gated),
+        y = torch.empty(shape, dtype=dtype, device=device) if gated else _new_like(x)
+        v, at, stride = _at(x)
+        _launch(device, native().act8_forward, at, stride, y.data_ptr(), math.prod(shape[:-1]), cols, GRAD_DTYPE[dtype], k, int(gated),
                 *_ptrs(a), *_ptrs(b), *_ptrs(out), *pitch_of(cols))
     else:
         v = x.detach()
@@ -355,8 +370,9 @@ def activation_backward(grad: torch.Tensor, held: Held, kind: str = "gelu", gate
         raise ValueError("act8.activation: grad is on %s, the checkpoint on %s" % (grad.device, a.device))
     cols, device = a.shape[-1], grad.device
     if grad.is_cuda:
-        dx, g = torch.empty(grad.shape[:-1] + (cols * (2 if gated else 1),), dtype=grad.dtype, device=device), _rows(grad)
-        _launch(device, native().act8_backward, g.data_ptr(), g.stride(0), dx.data_ptr(), a.rows, cols, GRAD_DTYPE[grad.dtype], k, int(gated),
+        dx = torch.empty(grad.shape[:-1] + (2 * cols,), dtype=grad.dtype, device=device) if gated else _new_like(grad)
+        g, at, stride = _at(grad)
+        _launch(device, native().act8_backward, at, stride, dx.data_ptr(), a.rows, cols, GRAD_DTYPE[grad.dtype], k, int(gated),
                 *_ptrs(a), *_ptrs(b), a.pitch, a.spitch)
         return dx
     g = grad.detach().float()

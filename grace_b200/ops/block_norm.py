@@ -22,7 +22,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import native
-from .act8 import Act8, _check_tensor, _decode_cpu, _encode_cpu, _launch, _ptrs, _rows, _sms, empty_like, held_bytes, pitch_of
+from .act8 import Act8, _at, _check_tensor, _decode_cpu, _encode_cpu, _launch, _new_like, _ptrs, _sms, empty_like, pitch_of
 from .exchange import GRAD_DTYPE
 
 NORMS = {None: 0, "rms": 1, "layer": 2}
@@ -36,37 +36,54 @@ class Saved:
     """What the backward pass takes from the forward pass: one allocation with the checkpoints and the statistics, the parameters, and the
     forms of the norms."""
 
-    __slots__ = ("data", "shape", "dtype", "params", "pre", "post", "residual_scale", "return_stream", "held_y", "held_block", "held_h", "_at")
+    __slots__ = ("data", "shape", "dtype", "rows", "pitch", "spitch", "two", "params", "pre", "post", "residual_scale", "return_stream", "held_h")
 
     def __init__(self, data: Optional[torch.Tensor], shape, dtype, device, params, pre, post, residual_scale, return_stream, held_h=None):
-        two = post is not None or params[4] is not None
-        n, rows = held_bytes(shape), math.prod(shape[:-1])
-        self._at = n * (2 if two else 1)
-        self.data = torch.empty(self._at + 16 * rows, dtype=torch.uint8, device=device) if data is None else data
-        self.shape, self.dtype, self.params, self.pre, self.post = shape, dtype, params, pre, post
+        self.shape, self.dtype, self.rows = shape, dtype, math.prod(shape[:-1])
+        self.pitch, self.spitch = pitch_of(shape[-1])
+        self.two = post is not None or params[4] is not None       # a checkpoint of block too
+        self.params, self.pre, self.post = params, pre, post
         self.residual_scale, self.return_stream, self.held_h = residual_scale, return_stream, held_h
-        self.held_y = Act8._over(self.data, 0, shape, dtype)
-        self.held_block = Act8._over(self.data, n, shape, dtype) if two else None
+        self.data = torch.empty(self._stats_at() + 16 * self.rows, dtype=torch.uint8, device=device) if data is None else data
+
+    def _held(self) -> int:     # bytes of a checkpoint, a multiple of 16
+        return (self.rows * (self.pitch + self.spitch) + 15) // 16 * 16
+
+    def _stats_at(self) -> int:
+        return self._held() * (2 if self.two else 1)
+
+    def ptrs(self) -> Tuple[int, int, int, int, int]:
+        """Addresses: codes and scales of y, of block (0, 0 without), the statistics."""
+        at, n, codes = self.data.data_ptr(), self._held(), self.rows * self.pitch
+        if self.two:
+            return at, at + codes, at + n, at + n + codes, at + 2 * n
+        return at, at + codes, 0, 0, at + n
+
+    @property
+    def held_y(self) -> Act8:
+        return Act8._over(self.data, 0, self.shape, self.dtype)
+
+    @property
+    def held_block(self) -> Optional[Act8]:
+        return Act8._over(self.data, self._held(), self.shape, self.dtype) if self.two else None
 
     @property
     def stats(self) -> torch.Tensor:
         """fp32 ``[rows, 4]``: mean and 1 / deviation of ``y``, then of ``block`` (0 and 1 without ``post``)."""
-        return self.data[self._at :].view(torch.float32).view(-1, 4)
-
-    def stats_ptr(self) -> int:
-        return self.data.data_ptr() + self._at
+        return self.data[self._stats_at() :].view(torch.float32).view(-1, 4)
 
 
 def _check(x, block, pre, post, params, residual_scale, eps) -> int:
     """Rows of a sequence (0: the gate, if any, is the same for all rows)."""
     _check_tensor(x, "residual_norm: x")
     _check_tensor(block, "residual_norm: block")
-    if x.shape != block.shape or x.dtype != block.dtype or x.device != block.device:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if shape != block.shape or dtype != block.dtype or device != block.device:
         raise ValueError("residual_norm: x %s %s on %s and block %s %s on %s have to be alike"
-                         % (tuple(x.shape), x.dtype, x.device, tuple(block.shape), block.dtype, block.device))
+                         % (tuple(shape), dtype, device, tuple(block.shape), block.dtype, block.device))
     if pre not in ("rms", "layer") or post not in NORMS:
         raise ValueError("residual_norm: pre is 'rms' or 'layer', post one of them or None, not %r and %r" % (pre, post))
-    cols, rows = x.shape[-1], math.prod(x.shape[:-1])
+    cols, rows = shape[-1], math.prod(shape[:-1])
     if cols > MAX_COLS or rows > MAX_ROWS:
         raise ValueError("residual_norm: at most %d columns and 2^31 - 1 rows, not %d and %d" % (MAX_COLS, cols, rows))
     if not (math.isfinite(residual_scale) and math.isfinite(eps) and eps >= 0):
@@ -75,23 +92,25 @@ def _check(x, block, pre, post, params, residual_scale, eps) -> int:
         raise ValueError("residual_norm: post_weight or post_bias without a norm after the block")
     if (pre == "rms" and params[1] is not None) or (post == "rms" and params[3] is not None):
         raise ValueError("residual_norm: an RMS norm has no bias")
-    kinds = {p.dtype for p in params if p is not None}
-    if kinds - {x.dtype, torch.float32} or len(kinds) > 1:
-        raise TypeError("residual_norm: parameters are all %s or all fp32, not %s" % (x.dtype, sorted(map(str, kinds))))
+    kind = None
     gate_rows = 0
     for name, p in zip(PARAMS, params):
         if p is None:
             continue
-        if p.device != x.device:
-            raise ValueError("residual_norm: %s is on %s, x on %s" % (name, p.device, x.device))
+        if p.dtype != kind:
+            if kind is not None or p.dtype not in (dtype, torch.float32):
+                raise TypeError("residual_norm: parameters are all %s or all fp32, not %s" % (dtype, [str(q.dtype) for q in params if q is not None]))
+            kind = p.dtype
+        if p.device != device:
+            raise ValueError("residual_norm: %s is on %s, x on %s" % (name, p.device, device))
         if name == "gate" and p.dim() == 2:
-            if x.dim() < 3 or tuple(p.shape) != (x.shape[0], cols):
+            if len(shape) < 3 or p.shape != (shape[0], cols):
                 raise ValueError("residual_norm: a gate of two axes has a row for each entry of the first of x's three or more axes, "
-                                 "not %s for x %s" % (tuple(p.shape), tuple(x.shape)))
+                                 "not %s for x %s" % (tuple(p.shape), tuple(shape)))
             if p.shape[0] > MAX_SEQUENCES:
                 raise ValueError("residual_norm: a gate has at most %d rows" % MAX_SEQUENCES)
             gate_rows = rows // max(1, p.shape[0])
-        elif tuple(p.shape) != (cols,):
+        elif p.shape != (cols,):
             raise ValueError("residual_norm: %s is %s for %d columns" % (name, tuple(p.shape), cols))
     return gate_rows
 
@@ -116,19 +135,24 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h)
     if not x.is_cuda:
         return _forward_cpu(x, block, saved, float(eps)) + (saved,)
-    h = torch.empty(shape, dtype=dtype, device=device)
-    y = torch.empty(shape, dtype=dtype, device=device) if return_stream else None
-    vx, vb = _rows(x), _rows(block)
+    h = _new_like(x)
+    y = _new_like(x) if return_stream else None
+    vx, x_at, x_stride = _at(x)
+    vb, b_at, b_stride = _at(block)
     ptrs, kept = _param_ptrs(params)
-    _launch(device, native().block_norm_forward, vx.data_ptr(), vx.stride(0), vb.data_ptr(), vb.stride(0), h.data_ptr(),
-            0 if y is None else y.data_ptr(), saved.stats_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params),
-            float(residual_scale), float(eps), gate_rows, ptrs, _ptrs(saved.held_y) + _ptrs(saved.held_block) + _ptrs(held_h), *pitch_of(cols), _sms(device))
+    *held, stats = saved.ptrs()
+    _launch(device, native().block_norm_forward, x_at, x_stride, b_at, b_stride, h.data_ptr(), 0 if y is None else y.data_ptr(), stats, rows,
+            cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params), float(residual_scale), float(eps), gate_rows, ptrs,
+            (*held, *_ptrs(held_h)), saved.pitch, saved.spitch, _sms(device))
     del kept
     return h, y, saved
 
 
 def _f32(params) -> int:
-    return int(any(p is not None and p.dtype == torch.float32 for p in params))
+    for p in params:
+        if p is not None:      # (they are all of one type)
+            return int(p.dtype == torch.float32)
+    return 0
 
 
 def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor], saved: Saved, needs=(True,) * 5
@@ -151,20 +175,21 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     if rows == 0 or cols == 0:
         empty = torch.empty(shape, dtype=dtype, device=device)
         return dict(zip(("x", "block") + PARAMS, [empty, empty] + [torch.zeros_like(p) if w else None for p, w in zip(params, want)]))
-    one = saved.post is None and gate is None and saved.residual_scale == 1.0
-    block = torch.empty(shape, dtype=dtype, device=device)
-    dx = None if one else torch.empty(shape, dtype=dtype, device=device)
-    grads = [torch.empty(p.shape, dtype=p.dtype, device=device) if w else None for p, w in zip(params, want)]
+    one = not saved.two and saved.residual_scale == 1.0
+    block = _new_like(grad_h)
+    dx = None if one else _new_like(grad_h)
+    grads = [(torch.empty_like(p) if p.is_contiguous() else torch.empty(p.shape, dtype=p.dtype, device=device)) if w else None
+             for p, w in zip(params, want)]
     gate_rows = rows // gate.shape[0] if gate is not None and gate.dim() == 2 else 0
     C, sms = native(), _sms(device)
-    pitch, spitch = pitch_of(cols)
-    g, gy = _rows(grad_h), None if grad_y is None else _rows(grad_y)
+    g, g_at, g_stride = _at(grad_h)
+    gy, gy_at, gy_stride = (None, 0, 0) if grad_y is None else _at(grad_y)
     ptrs, kept = _param_ptrs(params)
-    sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * pitch, dtype=torch.float32, device=device) if any(want) else None
-    _launch(device, C.block_norm_backward, g.data_ptr(), g.stride(0), 0 if gy is None else gy.data_ptr(), 0 if gy is None else gy.stride(0),
-            0 if dx is None else dx.data_ptr(), block.data_ptr(), saved.stats_ptr(), 0 if sums is None else sums.data_ptr(), rows, cols,
-            GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post], _f32(params), saved.residual_scale, gate_rows, ptrs,
-            [0 if t is None else t.data_ptr() for t in grads], _ptrs(saved.held_y) + _ptrs(saved.held_block), pitch, spitch, sms)
+    *held, stats = saved.ptrs()
+    sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * saved.pitch, dtype=torch.float32, device=device) if any(want) else None
+    _launch(device, C.block_norm_backward, g_at, g_stride, gy_at, gy_stride, 0 if dx is None else dx.data_ptr(), block.data_ptr(), stats,
+            0 if sums is None else sums.data_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post], _f32(params),
+            saved.residual_scale, gate_rows, ptrs, [0 if t is None else t.data_ptr() for t in grads], held, saved.pitch, saved.spitch, sms)
     del kept
     got = dict(zip(PARAMS, grads))
     got["x"], got["block"] = block if dx is None else dx, block
