@@ -117,7 +117,7 @@ def build_ours_loop(cfg, device, world):
     if cfg["model"] == "bert_large" and cfg.get("bert_impl", "hf") == "hf":
         model = hf_bert_large().to(device)
     else:
-        model = getattr(models, cfg["model"])().to(device)
+        model = getattr(models, cfg["model"])(**cfg.get("model_options", {})).to(device)
     if cfg["model"] in ("resnet50", "resnet20"):
         model = model.to(memory_format=torch.channels_last)
     params = dict(cfg["grace"])
@@ -154,7 +154,7 @@ def build_ours(cfg, device, world):
     if cfg["model"] == "bert_large" and cfg.get("bert_impl", "hf") == "hf":
         model = hf_bert_large().to(device)      # the same model class as the reference arm
     else:
-        model = getattr(models, cfg["model"])().to(device)
+        model = getattr(models, cfg["model"])(**cfg.get("model_options", {})).to(device)
     if cfg["model"] in ("resnet50", "resnet20"):   # VGG-16 stays NCHW: the reference arm's PowerSGD needs it
         model = model.to(memory_format=torch.channels_last)
     named = list(model.named_parameters())
@@ -281,6 +281,8 @@ def main():
     ap.add_argument("--bert-impl", default="hf", choices=["hf", "own"],
                     help="ours, bert_qsgd: transformers' BertForPreTraining as in the reference arm (default) or "
                          "this package's own BERT")
+    ap.add_argument("--activation-checkpoint", default=None, choices=["int8"],
+                    help="ours, bert_qsgd with --bert-impl own: keep activations for the backward pass in 8 bits")
     args = ap.parse_args()
     args.warmup = max(args.warmup, 3)
 
@@ -299,6 +301,10 @@ def main():
     elif cfg.get("bucket_mb"):
         cfg["bucket_bytes"] = int(cfg["bucket_mb"] * (1 << 20))
     cfg["bert_impl"] = args.bert_impl
+    if args.activation_checkpoint:
+        if cfg["model"] != "bert_large" or args.bert_impl != "own" or args.impl == "reference":
+            ap.error("--activation-checkpoint needs --config bert_qsgd --bert-impl own")
+        cfg["model_options"] = {"activation_checkpoint": args.activation_checkpoint}
     if args.overlap_sms is not None:
         cfg["overlap_sms"] = args.overlap_sms
     if args.nvls:

@@ -294,7 +294,10 @@ def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", p
                   post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
                   eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False):
     """``residual_norm_forward`` with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
-    alone comes as it is, several as a tuple."""
+    alone comes as it is, several as a tuple.  Under autocast ``x`` and ``block`` are taken in its type (parameters stay as they are)."""
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        t = torch.get_autocast_dtype("cuda")
+        x, block = x.to(t), block.to(t)      # the stream between kernels; inside, all arithmetic is fp32
     box = []
     out = _ResidualNorm.apply(x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, float(residual_scale), float(eps),
                               return_stream, checkpoint_output, box)
