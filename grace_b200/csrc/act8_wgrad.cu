@@ -26,7 +26,8 @@
 //
 // The tensor core truncates where it adds to an fp32 accumulator, which over thousands of tokens adds up to a bias
 // (2.3e-6 of the result after 4096 tokens).  Where the result itself is fp32 the accumulator is therefore emptied every
-// 1536 tokens into the output, rounding to nearest (0.2e-6).  Sums are fp32 throughout, rounded once to the output's type.
+// 1536 tokens into the other accumulator's place, rounding to nearest (0.3e-6); kept in the output instead, that cost
+// 40 % more traffic through L2 and as much time.  Sums are fp32 throughout, rounded once to the output's type.
 //
 // Every wait is bounded; when one runs out the status block says which and the outputs are NaN.
 #include <type_traits>
@@ -83,6 +84,7 @@ struct WgradArgs {
   int rest, rest_pairs; // tiles after them, and the pairs that share their steps equally
   int steps;            // of 64 tokens, over all tokens
   int chunk;            // steps between two emptyings of the accumulator
+  int single;           // 1: a piece may take several emptyings, which are added up in the second accumulator's place
   int bias_cols;        // columns of its 128 that a CTA adds up (a power of two, 8 to 128), 0: no bias gradient
   void* out;
   void* bias;
@@ -186,14 +188,35 @@ template <class T> constexpr uint32_t instruction_desc() {
   return (1u << 4) | (f << 7) | (f << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(2 * kTileK >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+        "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+        "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]), "r"(addr) : "memory");
+}
+// (the registers are operands so that nothing that uses them can be moved before the wait)
+__device__ __forceinline__ void tmem_wait_load(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                 "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A tile as one of the pair's CTAs sees it.
 struct Tile {
@@ -235,6 +258,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const Status status{wgrad_status};
   const int half = blockIdx.x & 1, pair = blockIdx.x >> 1;
   const bool has_bias = a.bias_cols != 0;
+  const unsigned two = a.single ? 0u : 1u;       // accumulators less one
   Piece p;
 
   if (tid == 0) {
@@ -245,6 +269,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     mbar_init(&sm.done, 1);
     sm.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 32 * 3) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_dy) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_codes) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(kTmemCols)
@@ -306,8 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Tile t = tile_at(a, p.tile, 0);
         const uint32_t idesc = instruction_desc<T>() | ((uint32_t)(t.boxes * 128 >> 3) << 17);
         for (int st = p.st0; ok && st < p.st1; ++item) {
-          const unsigned buf = item & 1;
-          if (item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[buf], ((item >> 1) - 1) & 1, kTimeoutNs, status, 300 + buf));
+          const unsigned buf = item & two, use = item >> two;
+          if (use >= 1) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[buf], (use - 1) & 1, kTimeoutNs, status, 300 + buf));
           if (!ok) break;
           tc_fence_after();
           const int end = min(st + a.chunk, p.st1);
@@ -332,7 +360,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
       // The other CTA's last arrivals here are on their way without being waited for by anything else, and a barrier
       // between the CTAs does not order them: this CTA has to be there when they land.
-      for (unsigned n = item > 2 ? item - 2 : 0; ok && n < item; ++n) ok = mbar_wait(&sm.acc_empty[n & 1], (n >> 1) & 1, 2 * kTimeoutNs, status, 350);
+      for (unsigned n = item > two + 1 ? item - two - 1 : 0; ok && n < item; ++n)
+        ok = mbar_wait(&sm.acc_empty[n & two], (n >> two) & 1, 2 * kTimeoutNs, status, 350);
       if (!ok) sm.failed = 1;
     }
   } else if (warp == 2) {
@@ -469,40 +498,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; piece_at(a, sm, pair, i, p); ++i) {
       const Tile t = tile_at(a, p.tile, half);
       const int k = t.k0 + kl, cols = t.boxes * 128;
+      const uint32_t quarter = (uint32_t)((warp - kEpilogueWarp0) * 32) << 16;
       for (int st = p.st0; st < p.st1; st += a.chunk, ++item) {
-        const unsigned buf = item & 1;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_full[buf], (item >> 1) & 1, 2 * kTimeoutNs, status, 700 + buf));
+        const unsigned buf = item & two, use = item >> two;
+        const bool add = st > p.st0, last = st + a.chunk >= p.st1;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_full[buf], use & 1, 2 * kTimeoutNs, status, 700 + buf));
         tc_fence_after();
-        const uint32_t base = tmem + buf * kTileN + ((uint32_t)((warp - kEpilogueWarp0) * 32) << 16);
-        // sums to q, q + stride, ... of `n` columns; an emptying after the first adds to what the one before it left
-        auto put = [&](auto* q, size_t stride, int n, int c) {
-          using Q = std::remove_pointer_t<decltype(q)>;
-          float old[16];
-          if (st > p.st0) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) old[j] = j < n ? to_f32<Q>(q[j * stride]) : 0.f;
-          }
-          uint32_t v[16];
+        const uint32_t base = tmem + buf * kTileN + quarter, sums = tmem + kTileN + quarter;
+        // columns c .. c + 31 of the accumulator, with what earlier emptyings left of them
+        auto take = [&](int c, float (&v)[32]) {
           __syncwarp();
-          tmem_load16(base + c, v);
+          tmem_load32(base + c, v);
+          if (add) {
+            float old[32];
+            tmem_load32(sums + c, old);
+            tmem_wait_load(v);
+            tmem_wait_load(old);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += old[j];
+          } else {
+            tmem_wait_load(v);
+          }
           if (!ok) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0x7fffffffu;
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fffffffu);
           }
-          if (st > p.st0) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + old[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (j < n) q[j * stride] = from_f32<Q>(__uint_as_float(v[j]));
         };
-        if (p.slot >= 0) {
-          float* const q = a.work + (size_t)p.slot * kSlotFloats + half * (kTileN * kTileK) + kl;
-          for (int c = 0; c < cols; c += 16) put(q + c * kTileK, kTileK, 16, c);
+        auto put = [&](auto* q, size_t stride, int have) {      // to q, q + stride, ...; `have`: columns that exist
+          using Q = std::remove_pointer_t<decltype(q)>;
+          for (int c = 0; c < cols; c += 32) {
+            float v[32];
+            take(c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < have) q[(c + j) * stride] = from_f32<Q>(v[j]);
+          }
+        };
+        if (!last) {
+          for (int c = 0; c < cols; c += 32) {
+            float v[32];
+            take(c, v);
+            tmem_store32(sums + c, v);
+          }
+          tmem_wait_store();
+        } else if (p.slot >= 0) {
+          put(a.work + (size_t)p.slot * kSlotFloats + half * (kTileN * kTileK) + kl, kTileK, cols);
         } else {
-          O* const q = static_cast<O*>(a.out) + (size_t)t.n0 * a.ins + k;
-          for (int c = 0; c < cols; c += 16) put(q + (size_t)c * a.ins, a.ins, k < a.ins ? min(16, a.outs - t.n0 - c) : 0, c);
+          put(static_cast<O*>(a.out) + (size_t)t.n0 * a.ins + k, a.ins, k < a.ins ? a.outs - t.n0 : 0);
         }
         tc_fence_before();
         __syncwarp();
@@ -703,7 +745,7 @@ cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held
     while (bias_cols * plan.tiles_k < kHalfN) bias_cols *= 2;
   }
   const WgradArgs a{held.scales, held.spitch, tokens, outs, ins, plan.tiles_k, plan.pairs, plan.whole, plan.rest, plan.rest_pairs,
-                    plan.steps, plan.chunk, bias_cols, out, bias, static_cast<float*>(work)};
+                    plan.steps, plan.chunk, plan.chunk < plan.steps ? 1 : 0, bias_cols, out, bias, static_cast<float*>(work)};
   if (dtype == kGradBF16)
     return out_f32 ? launch_typed<__nv_bfloat16, float>(map_dy, map_codes, a, stream)
                    : launch_typed<__nv_bfloat16, __nv_bfloat16>(map_dy, map_codes, a, stream);
