@@ -218,6 +218,30 @@ __device__ __forceinline__ void tmem_wait_load(float (&v)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Lane l holds v[0 .. 7] of row l of a 32 x 8 block: afterwards w is eight neighbouring rows, (l & 24) .. (l & 24) + 7, of column
+// l & 7, rounded to the 16-bit type O: 16 bytes of an output row instead of two of eight of them.
+template <class O>
+__device__ __forceinline__ uint4 turn8(const float* v, int lane) {
+  unsigned p[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool odd = lane & 1;
+    const float other = __shfl_xor_sync(0xffffffffu, odd ? v[2 * j] : v[2 * j + 1], 1);
+    p[j] = odd ? pack2<O>(other, v[2 * j + 1]) : pack2<O>(v[2 * j], other);
+  }
+#pragma unroll
+  for (int b = 1; b <= 2; b <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & b) continue;
+      const bool up = lane & (2 * b);
+      const unsigned other = __shfl_xor_sync(0xffffffffu, up ? p[j] : p[j | b], 2 * b);
+      if (up) p[j] = other;
+      else p[j | b] = other;
+    }
+  return make_uint4(p[0], p[1], p[2], p[3]);
+}
+
 // A tile as one of the pair's CTAs sees it.
 struct Tile {
   int k0;        // its first input feature
@@ -261,13 +285,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const unsigned two = a.single ? 0u : 1u;       // accumulators less one
   Piece p;
 
-  if (tid == 0) {
-    for (int s = 0; s < kBStages; ++s) { mbar_init(&sm.b_full[s], 1); mbar_init(&sm.b_used[s], 1); mbar_init(&sm.b_summed[s], 1); }
-    for (int s = 0; s < kCodeStages; ++s) { mbar_init(&sm.c_full[s], 1); mbar_init(&sm.c_empty[s], kGroupWarps); }
-    for (int s = 0; s < kAStages; ++s) mbar_init(&sm.ready[s], 2 * kGroupWarps);
-    for (int b = 0; b < 2; ++b) { mbar_init(&sm.acc_full[b], 1); mbar_init(&sm.acc_empty[b], 2 * 4); }
-    mbar_init(&sm.done, 1);
-    sm.failed = 0;
+  if (warp == 0) {      // (a lane for each stage)
+    if (lane < kBStages) { mbar_init(&sm.b_full[lane], 1); mbar_init(&sm.b_used[lane], 1); mbar_init(&sm.b_summed[lane], 1); }
+    if (lane < kCodeStages) { mbar_init(&sm.c_full[lane], 1); mbar_init(&sm.c_empty[lane], kGroupWarps); }
+    if (lane < kAStages) mbar_init(&sm.ready[lane], 2 * kGroupWarps);
+    if (lane < 2) { mbar_init(&sm.acc_full[lane], 1); mbar_init(&sm.acc_empty[lane], 2 * 4); }
+    if (lane == 0) { mbar_init(&sm.done, 1); sm.failed = 0; }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid == 32 * 3) {
@@ -543,6 +566,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tmem_wait_store();
         } else if (p.slot >= 0) {
           put(a.work + (size_t)p.slot * kSlotFloats + half * (kTileN * kTileK) + kl, kTileK, cols);
+        } else if (sizeof(O) == 2 && a.ins % 8 == 0) {
+          if constexpr (sizeof(O) == 2) {
+            const int k8 = k - (lane & 7), n = t.n0 + (lane & 7);
+            O* const q = static_cast<O*>(a.out) + (size_t)n * a.ins + k8;
+            for (int c = 0; c < cols; c += 32) {
+              float v[32];
+              take(c, v);
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                const uint4 w = turn8<O>(v + j, lane);
+                if (k8 < a.ins && n + c + j < a.outs) *reinterpret_cast<uint4*>(q + (size_t)(c + j) * a.ins) = w;
+              }
+            }
+          }
         } else {
           put(static_cast<O*>(a.out) + (size_t)t.n0 * a.ins + k, a.ins, k < a.ins ? a.outs - t.n0 : 0);
         }
@@ -662,6 +699,7 @@ struct Plan {
   size_t work_bytes;
 };
 Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
+  const bool scattered = !out_f32 && ins % 8 != 0;
   Plan p{};
   p.tiles_k = (ins + 2 * kTileK - 1) / (2 * kTileK);
   p.tiles = p.tiles_k * ((outs + kTileN - 1) / kTileN);
@@ -675,7 +713,7 @@ Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
   if (p.rest) {
     const long long total = (long long)p.rest * p.steps;
     long long n = total / 4 < p.pairs ? total / 4 : p.pairs;
-    if (n > p.rest && p.steps - (total + n - 1) / n >= kMinSavedSteps) p.rest_pairs = (int)n;
+    if (n > p.rest && p.steps - (total + n - 1) / n >= (scattered ? 1 : kMinSavedSteps)) p.rest_pairs = (int)n;
   }
   p.chunk = out_f32 ? kChunkSteps : p.steps;
   p.work_bytes = p.rest_pairs > p.rest ? (size_t)p.rest_pairs * 2 * kSlotFloats * 4 : 0;
