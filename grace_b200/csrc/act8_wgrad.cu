@@ -11,7 +11,7 @@
 //   A = x~     TMA brings the codes (64 tokens x 128 bytes), the decoders fetch their scale bytes; three groups of four warps take the steps in turn, decode them
 //              and store the operand tile
 // For bf16 a code's low seven bits are placed under an exponent that already holds the scale, its sign bit under
-// another, so decoding and scaling are one subtraction of two bf16 pairs; the result is exact.  (fp16: see decode8.)
+// another, so decoding and scaling are one subtraction of two bf16 pairs; the result is exact.  (fp16: see decode8.)  (fp16: see decode8.)
 //
 // Roles: warp 0 loads dY, warp 2 the codes (both by TMA), warp 1 of the pair's first CTA issues the MMAs, warp 3 adds up
 // the bias gradient (the CTAs of a row of tiles share its columns), warps 4 - 15 decode, warps 16 - 19 write results
@@ -85,6 +85,7 @@ struct WgradArgs {
   int steps;            // of 64 tokens, over all tokens
   int chunk;            // steps between two emptyings of the accumulator
   int single;           // 1: a piece may take several emptyings, which are added up in the second accumulator's place
+  unsigned one;         // 1 (see decode8)
   int bias_cols;        // columns of its 128 that a CTA adds up (a power of two, 8 to 128), 0: no bias gradient
   void* out;
   void* bias;
@@ -147,16 +148,21 @@ __device__ __forceinline__ void mbar_arrive_at(void* bar, unsigned cta) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(bar)), "r"(cta));
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// Eight codes as a 16-byte operand chunk.
-__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __nv_bfloat16) {
+// Eight codes as a 16-byte operand chunk.  The codes of a word come out as its even bytes, then its odd bytes, which one
+// mask each finds in place: input features 1 and 2 of every four change places in the operand, and so do the lanes of
+// the result (feature_of).  Integer operations have half the rate of the others and bound this kernel's decoders; `one` is
+// 1, and multiplying by it puts an addition into the multipliers' pipe.
+__device__ __forceinline__ int feature_of(int lane) { return (lane & ~3) | ((lane & 1) << 1) | ((lane >> 1) & 1); }
+
+__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, unsigned one, __nv_bfloat16) {
   // exponent field s + 7: 2^(s - 127) * 128 * (1 + m / 128) = (128 + m) steps
   const unsigned base = s == 255u ? 0x7fc07fc0u : ((s + 7u) << 7) * 0x10001u;
+  const unsigned w[4] = {c.x, c.x >> 8, c.y, c.y >> 8};
   unsigned r[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const unsigned v = __byte_perm(j < 2 ? c.x : c.y, 0u, (j & 1) ? 0x4342 : 0x4140);   // two codes, 16 bits each
-    const unsigned hi = (v & 0x007f007fu) | base;          // (128 + low seven bits) steps
-    const unsigned lo = (v & 0x00800080u) + base;          // 128 steps, or 256 for a negative code
+    const unsigned hi = (w[j] & 0x007f007fu) | base;             // (128 + low seven bits) steps
+    const unsigned lo = (w[j] & 0x00800080u) * one + base;       // 128 steps, or 256 for a negative code
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&hi), *reinterpret_cast<const __nv_bfloat162*>(&lo));
     r[j] = *reinterpret_cast<const unsigned*>(&d);
   }
@@ -165,17 +171,18 @@ __device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __nv_bfloat16) {
 // fp16 has the significand to take a code whole (1024 + byte), but not the exponents: the scale goes on in two factors,
 // 2^-6 and 2^(s - 121), so that its range reaches from 2^-30 to 2^9, that of groups of fp16 values; the first product is
 // exact and the second rounds once, into the subnormals.  A group beyond fp16's range reads as NaN.
-__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, __half) {
+__device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, unsigned, __half) {
   // 2^(s - 121): normal, subnormal, or below 2^-24, where every value rounds to zero
   const unsigned f = s > 136u ? 0x7e00u : (s >= 107u ? (s - 106u) << 10 : (s >= 97u ? 1u << (s - 97u) : 0u));
   const __half2 scale = __half2half2(__ushort_as_half((unsigned short)f));
   const __half2 sixth = __half2half2(__ushort_as_half(0x2400)), offset = __half2half2(__ushort_as_half(0xcc80));   // 2^-6, -18 = -1152 * 2^-6
   c.x ^= 0x80808080u;
   c.y ^= 0x80808080u;
+  const unsigned w[4] = {c.x, c.x >> 8, c.y, c.y >> 8};
   unsigned r[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const unsigned v = __byte_perm(j < 2 ? c.x : c.y, 0x64006400u, (j & 1) ? 0x5352 : 0x5150);   // 1024 + code + 128
+    const unsigned v = (w[j] & 0x00ff00ffu) | 0x64006400u;   // 1024 + code + 128
     const __half2 d = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&v), sixth, offset), scale);
     r[j] = *reinterpret_cast<const unsigned*>(&d);
   }
@@ -239,7 +246,9 @@ __device__ __forceinline__ uint4 turn8(const float* v, int lane) {
       if (up) p[j] = other;
       else p[j | b] = other;
     }
-  return make_uint4(p[0], p[1], p[2], p[3]);
+  // (features 1 and 2 of every four back in their places: see decode8)
+  return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x5410),
+                    __byte_perm(p[2], p[3], 0x7632));
 }
 
 // A tile as one of the pair's CTAs sees it.
@@ -502,8 +511,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           unsigned char* const row = sm.a[as] + swap * kBoxBytes + m * 128;
           const uint2 u = swap ? make_uint2(q[j].z, q[j].w) : make_uint2(q[j].x, q[j].y);
           const uint2 v = swap ? make_uint2(q[j].x, q[j].y) : make_uint2(q[j].z, q[j].w);
-          *reinterpret_cast<uint4*>(row + ((j0 ^ (m & 7)) << 4)) = decode8(u, s[j], T{});
-          *reinterpret_cast<uint4*>(row + ((j1 ^ (m & 7)) << 4)) = decode8(v, s[j], T{});
+          *reinterpret_cast<uint4*>(row + ((j0 ^ (m & 7)) << 4)) = decode8(u, s[j], a.one, T{});
+          *reinterpret_cast<uint4*>(row + ((j1 ^ (m & 7)) << 4)) = decode8(v, s[j], a.one, T{});
         }
         fence_async_shared();   // the tensor core reads the tile through the async proxy
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[n % kBStages], (n / kBStages) & 1, kTimeoutNs, status, 640));   // the step's dY is here too
@@ -515,7 +524,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (!ok) sm.failed = 1;
   } else {
     // ---- results: TMEM lane = input feature, column = output feature ----
-    const int kl = (warp - kEpilogueWarp0) * 32 + lane;
+    const int kl = (warp - kEpilogueWarp0) * 32 + feature_of(lane);
     unsigned item = 0;
     bool ok = true;
     for (int i = 0; piece_at(a, sm, pair, i, p); ++i) {
@@ -568,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           put(a.work + (size_t)p.slot * kSlotFloats + half * (kTileN * kTileK) + kl, kTileK, cols);
         } else if (sizeof(O) == 2 && a.ins % 8 == 0) {
           if constexpr (sizeof(O) == 2) {
-            const int k8 = k - (lane & 7), n = t.n0 + (lane & 7);
+            const int k8 = t.k0 + (warp - kEpilogueWarp0) * 32 + (lane & 24), n = t.n0 + (lane & 7);
             O* const q = static_cast<O*>(a.out) + (size_t)n * a.ins + k8;
             for (int c = 0; c < cols; c += 32) {
               float v[32];
@@ -783,7 +792,7 @@ cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held
     while (bias_cols * plan.tiles_k < kHalfN) bias_cols *= 2;
   }
   const WgradArgs a{held.scales, held.spitch, tokens, outs, ins, plan.tiles_k, plan.pairs, plan.whole, plan.rest, plan.rest_pairs,
-                    plan.steps, plan.chunk, plan.chunk < plan.steps ? 1 : 0, bias_cols, out, bias, static_cast<float*>(work)};
+                    plan.steps, plan.chunk, plan.chunk < plan.steps ? 1 : 0, 1u, bias_cols, out, bias, static_cast<float*>(work)};
   if (dtype == kGradBF16)
     return out_f32 ? launch_typed<__nv_bfloat16, float>(map_dy, map_codes, a, stream)
                    : launch_typed<__nv_bfloat16, __nv_bfloat16>(map_dy, map_codes, a, stream);
