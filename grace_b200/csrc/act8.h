@@ -45,7 +45,7 @@ struct BlockNormArgs {
   int cols;
   int pre, post;             // NormKind (pre: not kNormNone)
   int params_f32;            // parameters, gate and their gradients are fp32 (else of the activations' type)
-  float alpha, eps;
+  float alpha, alpha_low, eps;         // the residual's factor as the sum of two fp32 numbers
   long long gate_rows;       // rows of a sequence with a gate of its own; 0: one gate for all rows, or none
   const void *pre_weight, *pre_bias, *post_weight, *post_bias, *gate;   // null: ones, zeros, ones, zeros, no gate
   Held held_y, held_b, held_h;   // held_b: with N_post or a gate; held_h: on request; their codes null: not kept

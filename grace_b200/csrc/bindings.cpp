@@ -43,12 +43,13 @@ Held held(uintptr_t codes, uintptr_t scales, int pitch, int spitch) {
   return {ptr<signed char>(codes), ptr<unsigned char>(scales), pitch, spitch};
 }
 
-BlockNormArgs block_norm_args(long long rows, int cols, int pre, int post, int params_f32, float alpha, float eps, long long gate_rows,
+BlockNormArgs block_norm_args(long long rows, int cols, int pre, int post, int params_f32, double alpha, float eps, long long gate_rows,
                               const std::array<uintptr_t, 5>& params, uintptr_t stats) {
   if (pre < kNormRms || pre > kNormLayer || post < kNormNone || post > kNormLayer) throw std::invalid_argument("block_norm: unknown norm");
   if (gate_rows < 0 || (gate_rows && rows % gate_rows)) throw std::invalid_argument("block_norm: rows are not whole sequences");
   BlockNormArgs a{};
-  a.rows = rows; a.cols = cols; a.pre = pre; a.post = post; a.params_f32 = params_f32; a.alpha = alpha; a.eps = eps;
+  a.rows = rows; a.cols = cols; a.pre = pre; a.post = post; a.params_f32 = params_f32; a.alpha = (float)alpha;
+  a.alpha_low = (float)(alpha - (double)a.alpha); a.eps = eps;
   a.gate_rows = gate_rows;
   a.pre_weight = ptr<const void>(params[0]); a.pre_bias = ptr<const void>(params[1]); a.post_weight = ptr<const void>(params[2]);
   a.post_bias = ptr<const void>(params[3]); a.gate = ptr<const void>(params[4]);
@@ -348,7 +349,7 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
   // params: pre_weight, pre_bias, post_weight, post_bias, gate; held: codes and scales of y, block and h
   m.def("block_norm_forward",
         [](uintptr_t x, long long x_stride, uintptr_t block, long long block_stride, uintptr_t h, uintptr_t y, uintptr_t stats,
-           long long rows, int cols, int dtype, int pre, int post, int params_f32, float alpha, float eps, long long gate_rows,
+           long long rows, int cols, int dtype, int pre, int post, int params_f32, double alpha, float eps, long long gate_rows,
            const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 6>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
           BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, eps, gate_rows, params, stats);
           a.held_y = held(helds[0], helds[1], pitch, spitch);
@@ -361,7 +362,7 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
   // grads: of params, in their order
   m.def("block_norm_backward",
         [](uintptr_t grad_h, long long grad_h_stride, uintptr_t grad_y, long long grad_y_stride, uintptr_t dx, uintptr_t dblock,
-           uintptr_t stats, uintptr_t sums, long long rows, int cols, int dtype, int pre, int post, int params_f32, float alpha,
+           uintptr_t stats, uintptr_t sums, long long rows, int cols, int dtype, int pre, int post, int params_f32, double alpha,
            long long gate_rows, const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 5>& grads,
            const std::array<uintptr_t, 4>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
           BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, 0.f, gate_rows, params, stats);

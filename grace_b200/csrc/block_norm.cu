@@ -187,30 +187,14 @@ __device__ __forceinline__ void put_codes(const Held& h, long long row, int col,
   if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
 }
 
-// alpha x + n as an fp32 number that rounds to T as the exact sum does.  The fp32 sum itself may round onto the middle
-// between two 16-bit values (one in 2^13 for fp16), whence ties go to even whatever was cut off: there the sum is
-// taken in 64 bits, and the fp32 one moved off the middle towards it.
-template <class T> constexpr unsigned tie_mask() { return sizeof(T) == 4 ? 0u : (__is_same(T, __half) ? 0x1fffu : 0xffffu); }
-template <class T>
-__device__ __forceinline__ void scaled_sum(float alpha, const float (&x)[16], float (&v)[16]) {
-  constexpr unsigned mask = tie_mask<T>(), tie = (mask + 1) >> 1;
-  float y[16];
-  unsigned least = ~0u;
+// v += alpha x, where alpha is the sum of two fp32 numbers (a caller's 2.63 is none) of which the second is mostly zero
+__device__ __forceinline__ void add_scaled(float alpha, float alpha_low, const float (&x)[16], float (&v)[16]) {
+  if (alpha_low != 0.f) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    y[j] = fmaf(alpha, x[j], v[j]);
-    if (mask) least = min(least, (__float_as_uint(y[j]) ^ tie) & mask);     // 0: on a middle
-  }
-  if (mask && least == 0) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if ((__float_as_uint(y[j]) & mask) != tie) continue;
-      const double exact = (double)alpha * (double)x[j] + (double)v[j], at = (double)y[j];
-      if (exact != at) y[j] = __uint_as_float(__float_as_uint(y[j]) + ((exact > at) == (at > 0.0) ? 1u : ~0u));
-    }
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(alpha_low, x[j], v[j]);
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = y[j];
+  for (int j = 0; j < 16; ++j) v[j] = fmaf(alpha, x[j], v[j]);
 }
 
 // THREADS: 256 where a row takes no more, three CTAs an SM; 512
@@ -276,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
       }
     }
     cx.get(w);
-    scaled_sum<T>(a.alpha, w, v);
+    add_scaled(a.alpha, a.alpha_low, w, v);
     load(row + rpb);       // the next row's loads are under way during the rest of this one
     if (valid < 16) {
 #pragma unroll

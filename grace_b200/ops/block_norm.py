@@ -86,8 +86,8 @@ def _check(x, block, pre, post, params, residual_scale, eps) -> int:
     cols, rows = shape[-1], math.prod(shape[:-1])
     if cols > MAX_COLS or rows > MAX_ROWS:
         raise ValueError("residual_norm: at most %d columns and 2^31 - 1 rows, not %d and %d" % (MAX_COLS, cols, rows))
-    if not (math.isfinite(residual_scale) and math.isfinite(eps) and eps >= 0):
-        raise ValueError("residual_norm: a finite residual_scale and eps >= 0, not %r and %r" % (residual_scale, eps))
+    if not (abs(residual_scale) < 3e38 and 0 <= eps < 3e38):      # (fp32 numbers in the kernels)
+        raise ValueError("residual_norm: residual_scale and eps >= 0 within fp32's range, not %r and %r" % (residual_scale, eps))
     if post is None and (params[2] is not None or params[3] is not None):
         raise ValueError("residual_norm: post_weight or post_bias without a norm after the block")
     if (pre == "rms" and params[1] is not None) or (post == "rms" and params[3] is not None):

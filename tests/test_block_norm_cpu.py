@@ -87,7 +87,8 @@ def test_refusals():
     f, x, b = block_norm.residual_norm_forward, d["x"], d["block"]
     bad = [dict(p, pre="batch"), dict(p, pre=None), dict(p, post=None), dict(p, post="rms"), dict(p, pre="rms"),
            dict(p, gate=p["gate"][:1]), dict(p, gate=p["gate"][0, :39]), dict(p, pre_weight=p["pre_weight"][:39]),
-           dict(p, pre_weight=p["pre_weight"].view(1, 40)), dict(p, residual_scale=float("nan")), dict(p, eps=-1.0)]
+           dict(p, pre_weight=p["pre_weight"].view(1, 40)), dict(p, residual_scale=float("nan")), dict(p, eps=-1.0),
+           dict(p, residual_scale=-1e39), dict(p, eps=1e39)]
     for q in bad:
         with pytest.raises(ValueError):
             f(x, b, **q)
