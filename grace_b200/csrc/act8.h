@@ -48,8 +48,8 @@ struct BlockNormArgs {
   float alpha, alpha_low, eps;         // the residual's factor as the sum of two fp32 numbers
   long long gate_rows;       // rows of a sequence with a gate of its own; 0: one gate for all rows, or none
   const void *pre_weight, *pre_bias, *post_weight, *post_bias, *gate;   // null: ones, zeros, ones, zeros, no gate
-  Held held_y, held_b, held_h;   // held_b: with N_post or a gate; held_h: on request; their codes null: not kept
-  float* stats;              // [rows][4]: mean and rstd of y, mean and rstd of block
+  Held held_y, held_b, held_h;   // held_b: with N_post or a gate; held_h: on request; codes null: not kept (pitch is set all the same)
+  float* stats;              // [rows][4]: mean and rstd of y, mean and rstd of block; null: not kept
   // forward
   const void *x, *block;
   long long x_stride, block_stride;

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
     cy.set(v);       // the stream as it is rounded to its type
     cy.get(v);
     if (in && a.y) store16(v, static_cast<T*>(a.y) + row * a.cols, col, a.cols, a.out_vec);
-    {
+    if (a.held_y.codes) {
       const uint4 codes = act8_encode(v, s);
       if (in && owns) put_codes(a.held_y, row, col, codes, s);
     }
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
       const uint4 codes = act8_encode(v, s);
       if (in && owns) put_codes(a.held_h, row, col, codes, s);
     }
-    if (in && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(pre.x, pre.y, post.x, post.y);
+    if (in && t == 0 && a.stats) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(pre.x, pre.y, post.x, post.y);
   }
 }
 
@@ -632,7 +632,7 @@ BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, i
 
 cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
-  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll || !a.stats || !a.held_y.codes) return cudaErrorInvalidValue;
+  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
   switch (dtype) {
     case kGradF32: return forward_typed<float>(a, sms, stream);
     case kGradBF16: return forward_typed<__nv_bfloat16>(a, sms, stream);

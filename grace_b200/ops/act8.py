@@ -52,6 +52,8 @@ class Act8:
             raise ValueError("Act8: a checkpoint has at least one axis")
         if dtype not in GRAD_DTYPE:
             raise TypeError("Act8: fp32, bf16 or fp16, not %s" % dtype)
+        if shape[-1] > MAX_COLS:
+            raise ValueError("Act8: at most 2^30 columns")
         pitch, spitch = pitch_of(shape[-1])
         rows = math.prod(shape[:-1])
         if codes.dtype != torch.int8 or scales.dtype != torch.uint8:

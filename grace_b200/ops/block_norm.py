@@ -38,13 +38,14 @@ class Saved:
 
     __slots__ = ("data", "shape", "dtype", "rows", "pitch", "spitch", "two", "params", "pre", "post", "residual_scale", "return_stream", "held_h")
 
-    def __init__(self, data: Optional[torch.Tensor], shape, dtype, device, params, pre, post, residual_scale, return_stream, held_h=None):
+    def __init__(self, data: Optional[torch.Tensor], shape, dtype, device, params, pre, post, residual_scale, return_stream, held_h=None,
+                 keep=True):
         self.shape, self.dtype, self.rows = shape, dtype, math.prod(shape[:-1])
         self.pitch, self.spitch = pitch_of(shape[-1])
         self.two = post is not None or params[4] is not None       # a checkpoint of block too
         self.params, self.pre, self.post = params, pre, post
         self.residual_scale, self.return_stream, self.held_h = residual_scale, return_stream, held_h
-        self.data = torch.empty(self._stats_at() + 16 * self.rows, dtype=torch.uint8, device=device) if data is None else data
+        self.data = torch.empty(self._stats_at() + 16 * self.rows, dtype=torch.uint8, device=device) if data is None and keep else data
 
     def _held(self) -> int:     # bytes of a checkpoint, a multiple of 16
         return (self.rows * (self.pitch + self.spitch) + 15) // 16 * 16
@@ -124,15 +125,17 @@ def _param_ptrs(params):
 def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", pre_weight: Optional[torch.Tensor] = None,
                           pre_bias: Optional[torch.Tensor] = None, post: Optional[str] = None, post_weight: Optional[torch.Tensor] = None,
                           post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
-                          eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False
+                          eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False, checkpoint: bool = True
                           ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Saved]:
-    """``(h, y, saved)`` (``y`` None without ``return_stream``); with ``checkpoint_output`` ``saved.held_h`` is what ``act8.pack(h)`` gives."""
+    """``(h, y, saved)`` (``y`` None without ``return_stream``); with ``checkpoint_output`` ``saved.held_h`` is what ``act8.pack(h)`` gives.  With
+    ``checkpoint=False``, where no backward pass follows, ``saved`` holds nothing else.  A row of which the squares' sum passes fp32's
+    range has no deviation: NaN on the GPU."""
     params = (pre_weight, pre_bias, post_weight, post_bias, gate)
     gate_rows = _check(x, block, pre, post, params, residual_scale, eps)
     shape, dtype, device = x.shape, x.dtype, x.device
     cols, rows = shape[-1], math.prod(shape[:-1])
     held_h = empty_like(shape, dtype, device) if checkpoint_output else None
-    saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h)
+    saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h, checkpoint)
     if not x.is_cuda:
         return _forward_cpu(x, block, saved, float(eps)) + (saved,)
     h = _new_like(x)
@@ -140,7 +143,7 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     vx, x_at, x_stride = _at(x)
     vb, b_at, b_stride = _at(block)
     ptrs, kept = _param_ptrs(params)
-    *held, stats = saved.ptrs()
+    *held, stats = saved.ptrs() if checkpoint else (0,) * 5
     _launch(device, native().block_norm_forward, x_at, x_stride, b_at, b_stride, h.data_ptr(), 0 if y is None else y.data_ptr(), stats, rows,
             cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params), float(residual_scale), float(eps), gate_rows, ptrs,
             (*held, *_ptrs(held_h)), saved.pitch, saved.spitch, _sms(device))
@@ -160,6 +163,8 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     """The gradients of ``x``, ``block`` and the parameters (``PARAMS``), by name; None where there is no such parameter or ``needs`` (as
     ``PARAMS``) does not ask for it.  ``grad_y`` is that of the stream, None where nothing reads it.  Without ``post`` and gate and with a
     ``residual_scale`` of 1, ``x`` and ``block`` have one gradient: both names give the same tensor."""
+    if saved.data is None:
+        raise ValueError("residual_norm: the forward pass ran with checkpoint=False")
     params, shape, dtype, device = saved.params, saved.shape, saved.dtype, saved.data.device
     for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
         if g is None and name == "grad_y":
@@ -218,14 +223,17 @@ def _forward_cpu(x, block, saved: Saved, eps: float):
     n = b if saved.post is None else (b - mb) * rb * _wide(post_w, x.shape, 1.0) + _wide(post_b, x.shape, 0.0)
     if gate is not None:
         n = n * _wide(gate, x.shape, 1.0)
-    y = (saved.residual_scale * x.detach().float() + n).to(x.dtype)
+    y = (saved.residual_scale * x.detach().double() + n).to(x.dtype)
     v = y.float()
     m, r = _stats_cpu(v, saved.pre, eps)
     h = ((v - m) * r * _wide(pre_w, x.shape, 1.0) + _wide(pre_b, x.shape, 0.0)).to(x.dtype)
-    saved.stats.copy_(torch.stack([t.reshape(-1) for t in (m, r, mb, rb)], -1))
-    for part, into in ((y, saved.held_y), (block.detach(), saved.held_block), (h, saved.held_h)):
-        if into is not None:
-            _encode_cpu(part, into)
+    if saved.held_h is not None:
+        _encode_cpu(h, saved.held_h)
+    if saved.data is not None:
+        saved.stats.copy_(torch.stack([t.reshape(-1) for t in (m, r, mb, rb)], -1))
+        _encode_cpu(y, saved.held_y)
+        if saved.two:
+            _encode_cpu(block.detach(), saved.held_block)
     return h, y if saved.return_stream else None
 
 
@@ -298,6 +306,12 @@ def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", p
     if x.is_cuda and torch.is_autocast_enabled("cuda"):
         t = torch.get_autocast_dtype("cuda")
         x, block = x.to(t), block.to(t)      # the stream between kernels; inside, all arithmetic is fp32
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, pre_weight, pre_bias, post_weight, post_bias, gate))):
+        h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
+                                            post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps, return_stream=return_stream,
+                                            checkpoint_output=checkpoint_output, checkpoint=False)
+        out = (h,) + ((y,) if return_stream else ()) + ((saved.held_h,) if checkpoint_output else ())
+        return out[0] if len(out) == 1 else out
     box = []
     out = _ResidualNorm.apply(x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, float(residual_scale), float(eps),
                               return_stream, checkpoint_output, box)

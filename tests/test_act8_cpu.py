@@ -159,3 +159,8 @@ def test_weight_shared_by_two_layers():
     want = ones.t() @ held_value(h) + (ones @ w.detach().double()).t() @ held_value(x.detach())
     close(w.grad, want, 1e-3, "dW")
     assert half_step(torch.float32) == 2.0 ** -24
+
+
+def test_a_checkpoint_too_wide_is_refused():
+    with pytest.raises(ValueError, match="2\\^30 columns"):
+        act8.Act8(torch.empty(0, 0, dtype=torch.int8), torch.empty(0, 0, dtype=torch.uint8), (0, (1 << 30) + 1), torch.bfloat16)

@@ -139,3 +139,30 @@ def test_graph_replay():
     torch.cuda.synchronize()
     for got in outs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("pre,post,gate", [("layer", None, None), ("rms", "rms", "sequence"), ("layer", "layer", "channel")])
+@pytest.mark.parametrize("with_stream", [False, True])
+def test_without_a_backward_pass(pre, post, gate, with_stream):
+    """The same results, and nothing kept."""
+    d, p = make((2, 5, 72), torch.bfloat16, pre, post, gate, seed=21, device="cuda")
+    q = dict(p, return_stream=with_stream, checkpoint_output=True)
+    h, y, saved = block_norm.residual_norm_forward(d["x"], d["block"], **q)
+    h2, y2, kept = block_norm.residual_norm_forward(d["x"], d["block"], checkpoint=False, **q)
+    with torch.no_grad():
+        out = block_norm.residual_norm(d["x"].requires_grad_(), d["block"], **q)
+    assert kept.data is None and torch.equal(h, h2) and torch.equal(h, out[0]) and torch.equal(kept.held_h.codes, saved.held_h.codes)
+    assert torch.equal(out[-1].scales[:, :3], saved.held_h.scales[:, :3]) and len(out) == (3 if with_stream else 2)
+    if with_stream:
+        assert torch.equal(y, y2) and torch.equal(y, out[1])
+    with pytest.raises(ValueError):
+        block_norm.residual_norm_backward(d["dh"], d["dy"], kept)
+
+
+@pytest.mark.parametrize("alpha", [2.63, 0.1, 1 / 3])
+def test_residual_factor_is_not_rounded(alpha):
+    """y = alpha x to half a step (and 2^-20 of one for the part of alpha that 48 bits do not hold)."""
+    x = torch.randn(7, 96, generator=torch.Generator().manual_seed(22)).cuda()
+    y = block_norm.residual_norm_forward(x, torch.zeros_like(x), pre="rms", residual_scale=alpha)[1].double()
+    want = alpha * x.double()
+    assert bool(((y - want).abs() <= 2 ** -24 * (1 + 2 ** -20) * torch.exp2(torch.floor(torch.log2(want.abs())) + 1)).all())
