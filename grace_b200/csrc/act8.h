@@ -62,6 +62,7 @@ struct BlockNormArgs {
   float* sums;               // [runs of the backward pass][4][pitch] scratch (BlockNormShape)
   // filled in by the launchers
   int x_vec, block_vec, out_vec, grad_h_vec, grad_y_vec;   // RowAlign (act8.cuh)
+  int params_vec;                // the parameters may be read in fours
   int parts;
 };
 

@@ -293,6 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const bool has_bias = a.bias_cols != 0;
   const unsigned two = a.single ? 0u : 1u;       // accumulators less one
   Piece p;
+  cudaTriggerProgrammaticLaunchCompletion();     // (the second kernel's blocks take an SM as soon as one is left; it waits for all)
 
   if (warp == 0) {      // (a lane for each stage)
     if (lane < kBStages) { mbar_init(&sm.b_full[lane], 1); mbar_init(&sm.b_used[lane], 1); mbar_init(&sm.b_summed[lane], 1); }
@@ -641,9 +642,13 @@ __global__ void __launch_bounds__(256) wgrad_runs_kernel(const WgradArgs a) {
   if (c < t.boxes * 128 && n < a.outs && k < a.ins) {
     const float* const q = a.work + (half * kTileN + c) * kTileK + kl;
     float4 s = *reinterpret_cast<const float4*>(q + (size_t)p0 * kSlotFloats);
-    for (int p = (p0 | 1) + 1; p <= p1; p += 2) {
-      const float4 v = *reinterpret_cast<const float4*>(q + (size_t)p * kSlotFloats);
-      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    for (int p = (p0 | 1) + 1; p <= p1; p += 8) {      // four loads under way at a time
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = p + 2 * i <= p1 ? *reinterpret_cast<const float4*>(q + (size_t)(p + 2 * i) * kSlotFloats) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { s.x += v[i].x; s.y += v[i].y; s.z += v[i].z; s.w += v[i].w; }
     }
     O* const out = static_cast<O*>(a.out) + (size_t)n * a.ins + k;
     const float f[4] = {s.x, s.y, s.z, s.w};

@@ -31,16 +31,45 @@
 namespace grace {
 namespace {
 
-// Columns col .. col + 3 of a row of parameters, fp32 or of the activations' type; null, or past the end: `none`.
+// Columns col .. col + 3 of a row of parameters, fp32 or of the activations' type; past the end, or without such parameters:
+// `none`.  Loading and converting are two steps, so that the loads of all parameters are under way together: one after
+// the other they took most of a small call's time.
 template <class T>
-__device__ __forceinline__ float4 load_param(const BlockNormArgs& a, const void* p, int col, float none) {
-  float v[4];
+struct Param4 {
+  unsigned w[4];
+  __device__ __forceinline__ void load(const BlockNormArgs& a, const void* p, int col) {
+    w[0] = w[1] = w[2] = w[3] = 0u;
+    if (p == nullptr || col >= a.cols) return;
+    if (a.params_vec) {       // (then columns come in fours)
+      if (sizeof(T) == 4 || a.params_f32) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(p) + col));
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + col));
+        w[0] = v.x & 0xffffu; w[1] = v.x >> 16; w[2] = v.y & 0xffffu; w[3] = v.y >> 16;
+      }
+      return;
+    }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    v[j] = p == nullptr || col + j >= a.cols ? none
-                                              : (a.params_f32 ? __ldg(static_cast<const float*>(p) + col + j) : to_f32<T>(static_cast<const T*>(p)[col + j]));
-  return make_float4(v[0], v[1], v[2], v[3]);
-}
+    for (int j = 0; j < 4; ++j)
+      if (col + j < a.cols) w[j] = sizeof(T) == 4 || a.params_f32 ? __ldg(static_cast<const unsigned*>(p) + col + j) : __ldg(static_cast<const unsigned short*>(p) + col + j);
+  }
+  __device__ __forceinline__ float4 get(const BlockNormArgs& a, const void* p, int col, float none) const {
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (p == nullptr || col + j >= a.cols) {
+        v[j] = none;
+      } else if (sizeof(T) == 4 || a.params_f32) {
+        v[j] = __uint_as_float(w[j]);
+      } else {
+        const unsigned short bits = (unsigned short)w[j];
+        v[j] = to_f32<T>(*reinterpret_cast<const T*>(&bits));
+      }
+    }
+    return make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
 
 // A row of parameters in shared memory, fp32, for `chunks` chunks of sixteen columns: the first quarters of all chunks,
 // then the second ones, and so on, so that a quarter warp's 16-byte accesses are consecutive.
@@ -227,13 +256,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
   const SharedRow u_row{params + (PRE_LAYER ? 8 : 4) * chunks, chunks}, ub_row{u_row.at + 4 * chunks, chunks};
   const void* const g = gate_of<T>(a, run);
   for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
-    const float4 w = load_param<T>(a, a.pre_weight, i * 4, 1.f), b = load_param<T>(a, a.pre_bias, i * 4, 0.f);
-    const float4 u = load_param<T>(a, a.post_weight, i * 4, 1.f), ub = load_param<T>(a, a.post_bias, i * 4, 0.f);
-    const float4 f = load_param<T>(a, g, i * 4, 1.f);
-    pre_w.put(i, w);
-    if (PRE_LAYER) pre_b.put(i, b);
-    if (scaled) u_row.put(i, times(u, f));
-    if (BIAS) ub_row.put(i, times(ub, f));
+    Param4<T> w, b, u, ub, f;
+    w.load(a, a.pre_weight, i * 4);
+    if (PRE_LAYER) b.load(a, a.pre_bias, i * 4);
+    if (POST) u.load(a, a.post_weight, i * 4);
+    if (BIAS) ub.load(a, a.post_bias, i * 4);
+    f.load(a, g, i * 4);
+    pre_w.put(i, w.get(a, a.pre_weight, i * 4, 1.f));
+    if (PRE_LAYER) pre_b.put(i, b.get(a, a.pre_bias, i * 4, 0.f));
+    if (scaled) {
+      const float4 gate = f.get(a, g, i * 4, 1.f);
+      if (POST) u_row.put(i, times(u.get(a, a.post_weight, i * 4, 1.f), gate));
+      else u_row.put(i, gate);
+      if (BIAS) ub_row.put(i, times(ub.get(a, a.post_bias, i * 4, 0.f), gate));
+    }
   }
   __syncthreads();
 
@@ -360,15 +396,22 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
   RowSum sum(buf, tpr);
   float dw[16] = {}, db[L] = {}, g1[B] = {}, g0[Z] = {};
 
+  cudaTriggerProgrammaticLaunchCompletion();     // (the sums kernel's blocks take an SM as soon as one is left; it waits for all)
   RowLoads<T, TWO> r;
   r.load(a, run.row0 + lane_row, col, run.row0 + lane_row < run.row1);
   const SharedRow pre_w{params, chunks}, u_row{params + 4 * chunks, chunks};
   const void* const gate = gate_of<T>(a, run);
   for (int i = threadIdx.x; i < 4 * chunks; i += blockDim.x) {
-    const float4 w = load_param<T>(a, a.pre_weight, i * 4, 1.f);
-    const float4 u = load_param<T>(a, a.post_weight, i * 4, 1.f), v = load_param<T>(a, gate, i * 4, 1.f);
-    pre_w.put(i, w);
-    if (TWO) u_row.put(i, first_of(times(u, v), a.cols - i * 4));
+    Param4<T> w, u, f;
+    w.load(a, a.pre_weight, i * 4);
+    if (NORM) u.load(a, a.post_weight, i * 4);
+    if (TWO) f.load(a, gate, i * 4);
+    pre_w.put(i, w.get(a, a.pre_weight, i * 4, 1.f));
+    if (TWO) {
+      float4 v = f.get(a, gate, i * 4, 1.f);
+      if (NORM) v = times(v, u.get(a, a.post_weight, i * 4, 1.f));
+      u_row.put(i, first_of(v, a.cols - i * 4));
+    }
   }
   __syncthreads();
   float sum_u = 0.f;
@@ -534,10 +577,18 @@ cudaError_t launch_shared(K kernel, dim3 grid, dim3 block, size_t smem, cudaStre
   return cudaGetLastError();
 }
 
+// Whether every row of parameters starts where four of its elements do, and ends after a multiple of four.
+bool params_vec(const BlockNormArgs& a, size_t es) {
+  uintptr_t all = 0;
+  for (const void* p : {a.pre_weight, a.pre_bias, a.post_weight, a.post_bias, a.gate}) all |= reinterpret_cast<uintptr_t>(p);
+  return a.cols % 4 == 0 && all % (4 * (a.params_f32 ? 4 : es)) == 0;
+}
+
 template <class T>
 cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   a.x_vec = row_align(a.x, a.x_stride, sizeof(T));
   a.block_vec = row_align(a.block, a.block_stride, sizeof(T));
+  a.params_vec = params_vec(a, sizeof(T));
   a.out_vec = std::min(row_align(a.h, a.cols, sizeof(T)), row_align(a.y, a.cols, sizeof(T)));
   const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, false);
   a.parts = shape.parts;
@@ -593,6 +644,7 @@ template <class T>
 cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, int sms, cudaStream_t stream) {
   a.grad_h_vec = row_align(a.grad_h, a.grad_h_stride, sizeof(T));
   a.grad_y_vec = row_align(a.grad_y, a.grad_y_stride, sizeof(T));
+  a.params_vec = params_vec(a, sizeof(T));
   a.out_vec = std::min(row_align(a.dblock, a.cols, sizeof(T)), row_align(a.dx, a.cols, sizeof(T)));
   a.parts = shape.parts;
   const cudaError_t err = backward_launch<T>(a, shape, stream);

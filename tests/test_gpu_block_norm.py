@@ -166,3 +166,21 @@ def test_residual_factor_is_not_rounded(alpha):
     y = block_norm.residual_norm_forward(x, torch.zeros_like(x), pre="rms", residual_scale=alpha)[1].double()
     want = alpha * x.double()
     assert bool(((y - want).abs() <= 2 ** -24 * (1 + 2 ** -20) * torch.exp2(torch.floor(torch.log2(want.abs())) + 1)).all())
+
+
+@pytest.mark.parametrize("cols", [96, 90])
+def test_parameters_off_their_boundaries(cols):
+    """Slices that start where no four elements do, and rows of a gate that do."""
+    d, p = make((3, 5, cols), BF16, "layer", "layer", "sequence", seed=23, device="cuda")
+    want = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+    back = block_norm.residual_norm_backward(d["dh"], d["dy"], want[2])
+    for off in (1, 4):
+        q = dict(p)
+        for k in ("pre_weight", "pre_bias", "post_weight", "post_bias", "gate"):
+            t = torch.zeros(p[k].numel() + off, dtype=BF16, device="cuda")
+            t[off:] = p[k].reshape(-1)
+            q[k] = t[off:].view(p[k].shape)
+        got = block_norm.residual_norm_forward(d["x"], d["block"], **q)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        grads = block_norm.residual_norm_backward(d["dh"], d["dy"], got[2])
+        assert all(torch.equal(grads[k], back[k]) for k in back)
