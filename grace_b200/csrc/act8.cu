@@ -80,36 +80,94 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return r;
 }
 
-template <int KIND, bool FAST>
+constexpr float kInvSqrt2Pi = 0.3989422804f, kLog2e = 1.4426950409f;
+constexpr float kTanhC = 0.7978845608f, kTanhA = 0.044715f;
+
+__device__ __forceinline__ F2 exp2_fast(F2 x) {
+  float a, b;
+  x.get(a, b);
+  return F2(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ F2 rcp_fast(F2 x) {
+  float a, b;
+  x.get(a, b);
+  return F2(rcp_fast(a), rcp_fast(b));
+}
+__device__ __forceinline__ F2 one_minus(F2 x) { return fma2(x, F2(-1.f), F2(1.f)); }
+
+// f and f' at two numbers, for 16-bit tensors
+template <int KIND>
+__device__ __forceinline__ void function(F2 x, F2& f, F2& d) {
+  const F2 one(1.f);
+  F2 p;
+  if (KIND == kActGelu) {   // p: the normal distribution function, e: exp(-x^2 / 2)
+    float a, b, qa, qb;
+    x.get(a, b);
+    const F2 t = rcp_fast(F2(fmaf(0.3275911f * 0.70710678f, fabsf(a), 1.f), fmaf(0.3275911f * 0.70710678f, fabsf(b), 1.f)));
+    const F2 e = exp2_fast(mul2(mul2(x, x), F2(-0.5f * kLog2e)));
+    F2 poly = fma2(t, F2(0.5f * 1.061405429f), F2(0.5f * -1.453152027f));
+    poly = fma2(t, poly, F2(0.5f * 1.421413741f));
+    poly = fma2(t, poly, F2(0.5f * -0.284496736f));
+    poly = fma2(t, poly, F2(0.5f * 0.254829592f));
+    mul2(mul2(t, poly), e).get(qa, qb);      // erfc(|x| / sqrt 2) / 2
+    p = F2(a < 0.f ? qa : 1.f - qa, b < 0.f ? qb : 1.f - qb);
+    d = fma2(mul2(x, F2(kInvSqrt2Pi)), e, p);
+  } else if (KIND == kActGeluTanh) {
+    float a, b;
+    mul2(x, x).get(a, b);
+    const F2 xx(fminf(a, 1e4f), fminf(b, 1e4f));      // past |x| = 100 the sigmoid is 0 or 1 to the last bit
+    const F2 u = mul2(mul2(x, F2(-2.f * kTanhC * kLog2e)), fma2(xx, F2(kTanhA), one));
+    p = rcp_fast(add2(exp2_fast(u), one));            // (1 + tanh) / 2
+    d = fma2(mul2(mul2(mul2(x, F2(2.f * kTanhC)), p), one_minus(p)), fma2(xx, F2(3.f * kTanhA), one), p);
+  } else {
+    p = rcp_fast(add2(exp2_fast(mul2(x, F2(-kLog2e))), one));
+    d = mul2(p, fma2(x, one_minus(p), one));
+  }
+  f = mul2(x, p);
+}
+// the same with CUDA's functions, for fp32 tensors
+template <int KIND>
 __device__ __forceinline__ float2 function(float x) {
-  constexpr float kInvSqrt2Pi = 0.3989422804f, kLog2e = 1.4426950409f;
   if (KIND == kActGelu) {
-    float p, e;   // p: the normal distribution function, e: exp(-x^2 / 2)
-    if (FAST) {
-      const float t = rcp_fast(fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.f));
-      e = exp2_fast(-0.5f * kLog2e * (x * x));
-      const float poly = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f),
-                              0.5f * 0.254829592f);
-      const float q = t * poly * e;              // erfc(|x| / sqrt 2) / 2
-      p = x < 0.f ? q : 1.f - q;
-    } else {
-      e = expf(-0.5f * x * x);
-      p = 0.5f * erfcf(-0.70710678f * x);
-    }
+    const float e = expf(-0.5f * x * x), p = 0.5f * erfcf(-0.70710678f * x);
     return make_float2(x * p, fmaf(x * kInvSqrt2Pi, e, p));
   }
   if (KIND == kActGeluTanh) {
-    constexpr float c = 0.7978845608f, a = 0.044715f;
-    const float xx = fminf(x * x, 1e4f);   // past |x| = 100 the sigmoid is 0 or 1 to the last bit
-    const float u = 2.f * c * x * fmaf(a, xx, 1.f);
-    const float p = FAST ? rcp_fast(1.f + exp2_fast(-kLog2e * u)) : 1.f / (1.f + expf(-u));   // (1 + tanh(u / 2)) / 2
-    return make_float2(x * p, fmaf(2.f * c * x * p * (1.f - p), fmaf(3.f * a, xx, 1.f), p));
+    const float xx = fminf(x * x, 1e4f), p = 1.f / (1.f + expf(-2.f * kTanhC * x * fmaf(kTanhA, xx, 1.f)));
+    return make_float2(x * p, fmaf(2.f * kTanhC * x * p * (1.f - p), fmaf(3.f * kTanhA, xx, 1.f), p));
   }
-  const float p = FAST ? rcp_fast(1.f + exp2_fast(-kLog2e * x)) : 1.f / (1.f + expf(-x));
+  const float p = 1.f / (1.f + expf(-x));
   return make_float2(x * p, p * fmaf(x, 1.f - p, 1.f));
+}
+// f(x) and f'(x) of sixteen
+template <class T, int KIND>
+__device__ __forceinline__ void function16(const float (&x)[16], float (&f)[16], float (&d)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      F2 y, z;
+      function<KIND>(pair(x, i), y, z);
+      put(f, i, y);
+      put(d, i, z);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 y = function<KIND>(x[j]);
+      f[j] = y.x;
+      d[j] = y.y;
+    }
+  }
+}
+__device__ __forceinline__ void mul16(float (&v)[16], const float (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, mul2(pair(v, i), pair(w, i)));
 }
 
 // ---- kernels: thread t of block b takes chunk 256 b + t ----
+// The gated kernels would take 58 registers and 4 blocks an SM, which cost the backward pass an eighth of its time.
+template <class T, bool GATED> constexpr int blocks_an_sm() { return sizeof(T) == 4 ? 1 : (GATED ? 5 : 6); }
+
 struct Place {
   unsigned row, col;
   bool in;
@@ -147,9 +205,8 @@ __global__ void __launch_bounds__(kBlock) unpack_kernel(Held held, T* __restrict
 }
 
 template <class T, int KIND, bool GATED>
-__global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x, long long stride, int vec_x, T* __restrict__ y,
+__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>()) forward_kernel(const T* __restrict__ x, long long stride, int vec_x, T* __restrict__ y,
                                                         int vec_y, Rows r, Held held, Held held_b, Held held_y) {
-  constexpr bool kFast = sizeof(T) == 2;
   const Place p = place_of(r);
   const int col = (int)p.col;
   Chunk16<T> ca, cb;
@@ -168,16 +225,14 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x
     codes = act8_encode(v, s);
     if (p.in) put_held(held, p.row, col, codes, s);
   }
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = function<KIND, kFast>(v[j]).x;
+  function16<T, KIND>(v, v, w);
   if (GATED) {
     cb.get(w);
     if (held_b.codes) {
       codes = act8_encode(w, s);
       if (p.in) put_held(held_b, p.row, col, codes, s);
     }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] *= w[j];
+    mul16(v, w);
   }
   if (p.in) store16(v, y + (size_t)p.row * r.cols, col, r.cols, vec_y);
   if (held_y.codes) {
@@ -190,9 +245,8 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(const T* __restrict__ x
 }
 
 template <class T, int KIND, bool GATED>
-__global__ void __launch_bounds__(kBlock) backward_kernel(const T* __restrict__ grad, long long stride, int vec_g, T* __restrict__ dx,
+__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>()) backward_kernel(const T* __restrict__ grad, long long stride, int vec_g, T* __restrict__ dx,
                                                          int vec_x, Rows r, Held held, Held held_b) {
-  constexpr bool kFast = sizeof(T) == 2;
   const Place p = place_of(r);
   if (!p.in) return;
   const int col = (int)p.col;
@@ -201,24 +255,19 @@ __global__ void __launch_bounds__(kBlock) backward_kernel(const T* __restrict__ 
   c.load(grad + (long long)p.row * stride, col, r.cols, vec_g);
   qa.load(held, p.row, col);
   if (GATED) qb.load(held_b, p.row, col);
-  float g[16], a[16], b[16];
+  float g[16], a[16], b[16], d[16];
   c.get(g);
   qa.get(a);
+  function16<T, KIND>(a, a, d);
+  mul16(d, g);
   T* const out = dx + (size_t)p.row * (GATED ? 2 : 1) * r.cols;
   if (GATED) {
     qb.get(b);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float2 f = function<KIND, kFast>(a[j]);
-      a[j] = g[j] * b[j] * f.y;
-      b[j] = g[j] * f.x;
-    }
-    store16(b, out + r.cols, col, r.cols, vec_x);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) a[j] = g[j] * function<KIND, kFast>(a[j]).y;
+    mul16(d, b);
+    mul16(a, g);
+    store16(a, out + r.cols, col, r.cols, vec_x);
   }
-  store16(a, out, col, r.cols, vec_x);
+  store16(d, out, col, r.cols, vec_x);
 }
 
 Held rows_from(Held h, long long row) {

@@ -31,51 +31,88 @@ __device__ __forceinline__ unsigned act8_scale_byte(unsigned top_bits) {   // bi
 __device__ __forceinline__ float act8_inverse(unsigned s) { return __uint_as_float(s == 255u ? 0u : (254u - s) << 23); }
 __device__ __forceinline__ float act8_step(unsigned s) { return __uint_as_float(s == 255u ? 0x7fffffffu : s << 23); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // a NaN where either is one (its sign bit clear)
+__device__ __forceinline__ float max_abs(float a, float b, float c) {   // a NaN where one of them is one
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+
+// Two fp32 numbers in a register pair, and arithmetic on both in one instruction, each rounded as by itself.  The kernels
+// that use these are short of issue slots before they are short of arithmetic.
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ explicit F2(float x) : F2(x, x) {}
+  F2() = default;
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+  __device__ __forceinline__ float sum() const {
+    float x, y;
+    get(x, y);
+    return x + y;
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+template <int N> __device__ __forceinline__ F2 pair(const float (&v)[N], int i) { return F2(v[2 * i], v[2 * i + 1]); }
+template <int N> __device__ __forceinline__ void put(float (&v)[N], int i, F2 x) { x.get(v[2 * i], v[2 * i + 1]); }
 
 // Sixteen values of a group whose other half is held by the neighbouring lane (lanes 2i and 2i + 1, both active): their
 // codes, and the group's scale byte.
 __device__ __forceinline__ uint4 act8_encode(const float (&v)[16], unsigned& s) {
-  float m[4];      // (four chains of maxima: one would be sixteen latencies long)
+  float m[5];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m[j] = max_nan(max_nan(fabsf(v[j]), fabsf(v[j + 4])), max_nan(fabsf(v[j + 8]), fabsf(v[j + 12])));
-  unsigned top = __float_as_uint(max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])));     // from here on as integers: a NaN is the largest
+  for (int j = 0; j < 5; ++j) m[j] = max_abs(v[3 * j], v[3 * j + 1], v[3 * j + 2]);
+  unsigned top = __float_as_uint(max_abs(max_abs(m[0], m[1], m[2]), max_abs(m[3], m[4], v[15]), 0.f)) & 0x7fffffffu;     // from here on as integers: a NaN is the largest
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   s = act8_scale_byte(top);
   const float inv = act8_inverse(s);
   constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: the sum's low byte is the integer nearest to x * inv, ties to even
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(x, i, fma2(pair(v, i), F2(inv), F2(kMagic)));
+  if (__uint_as_float(top) * inv >= 127.5f) {     // one group in two hundred: without the clamp all others take two instructions an element less
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = fminf(fmaxf(x[j], kMagic - 127.f), kMagic + 127.f);
+  }
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     unsigned u[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      u[j] = __float_as_uint(fminf(fmaxf(__fmaf_rn(v[4 * i + j], inv, kMagic), kMagic - 127.f), kMagic + 127.f));
+    for (int j = 0; j < 4; ++j) u[j] = __float_as_uint(x[4 * i + j]);
     w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   }
-  // (an infinity times 0 is a NaN, which the clamp above turns into a bound)
   return s == 255u ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The values of N codes (four in each of N / 4 words).
-template <int N>
-__device__ __forceinline__ void act8_decode(const unsigned (&codes)[N / 4], unsigned s, float (&v)[N]) {
-  const float step = act8_step(s);
+// f(i, codes 2 i and 2 i + 1 as numbers) of sixteen codes
+template <class F>
+__device__ __forceinline__ void act8_codes(uint4 codes, F f) {
+  const unsigned w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const unsigned c = codes[i] ^ 0x80808080u;   // code + 128, an unsigned byte
-#pragma unroll
-    for (int j = 0; j < 4; ++j)   // a byte in the low bits of 2^23 is the number 2^23 + byte
-      v[4 * i + j] = (__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7540 + j)) - 8388736.f) * step;
+  for (int i = 0; i < 8; ++i) {
+    const unsigned c = w[i / 2] ^ 0x80808080u;   // code + 128, an unsigned byte; in the low bits of 2^23 it is the number 2^23 + byte
+    const int j = i % 2 * 2;
+    f(i, add2(F2(__uint_as_float(__byte_perm(c, 0x4b000000u, 0x7540 + j)), __uint_as_float(__byte_perm(c, 0x4b000000u, 0x7541 + j))), F2(-8388736.f)));
   }
 }
+// The values of sixteen codes.
 __device__ __forceinline__ void act8_decode(uint4 codes, unsigned s, float (&v)[16]) {
-  const unsigned w[4] = {codes.x, codes.y, codes.z, codes.w};
-  act8_decode<16>(w, s, v);
+  const F2 step(act8_step(s));
+  act8_codes(codes, [&](int i, F2 q) { put(v, i, mul2(q, step)); });
 }
 
 // ---- eight neighbouring elements of a row of fp32, bf16 or fp16, as fp32 ----

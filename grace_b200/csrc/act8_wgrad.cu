@@ -11,7 +11,7 @@
 //   A = x~     TMA brings the codes (64 tokens x 128 bytes), the decoders fetch their scale bytes; three groups of four warps take the steps in turn, decode them
 //              and store the operand tile
 // For bf16 a code's low seven bits are placed under an exponent that already holds the scale, its sign bit under
-// another, so decoding and scaling are one subtraction of two bf16 pairs; the result is exact.  (fp16: see decode8.)  (fp16: see decode8.)
+// another, so decoding and scaling are one subtraction of two bf16 pairs; the result is exact.  (fp16: see decode8.)
 //
 // Roles: warp 0 loads dY, warp 2 the codes (both by TMA), warp 1 of the pair's first CTA issues the MMAs, warp 3 adds up
 // the bias gradient (the CTAs of a row of tiles share its columns), warps 4 - 15 decode, warps 16 - 19 write results

@@ -154,16 +154,45 @@ struct RowSum {
 
 // sum of a[j] b[j], in four chains
 __device__ __forceinline__ float dot16(const float (&a)[16], const float (&b)[16]) {
-  float s[4] = {};
+  F2 s = mul2(pair(a, 0), pair(b, 0)), t = mul2(pair(a, 1), pair(b, 1));
 #pragma unroll
-  for (int j = 0; j < 16; ++j) s[j & 3] = fmaf(a[j], b[j], s[j & 3]);
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  for (int i = 2; i < 8; i += 2) {
+    s = fma2(pair(a, i), pair(b, i), s);
+    t = fma2(pair(a, i + 1), pair(b, i + 1), t);
+  }
+  return s.sum() + t.sum();
 }
 __device__ __forceinline__ float sum16(const float (&a)[16]) {
-  float s[4] = {};
+  F2 s = pair(a, 0), t = pair(a, 1);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) s[j & 3] += a[j];
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  for (int i = 2; i < 8; i += 2) {
+    s = add2(s, pair(a, i));
+    t = add2(t, pair(a, i + 1));
+  }
+  return s.sum() + t.sum();
+}
+// v = v * w, v * w + u and the like, for sixteen columns
+__device__ __forceinline__ void mul16(float (&v)[16], const float (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, mul2(pair(v, i), pair(w, i)));
+}
+__device__ __forceinline__ void add16(float (&v)[16], const float (&w)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, add2(pair(v, i), pair(w, i)));
+}
+__device__ __forceinline__ void add_product16(float (&v)[16], const float (&a)[16], const float (&b)[16]) {      // v += a b
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, fma2(pair(a, i), pair(b, i), pair(v, i)));
+}
+__device__ __forceinline__ void add_scaled16(float (&v)[16], float c, const float (&a)[16]) {      // v += c a
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, fma2(F2(c), pair(a, i), pair(v, i)));
+}
+// (v - mean) * r: the difference first, since a mean far from zero must not cost digits
+template <bool LAYER>
+__device__ __forceinline__ void normalise16(float (&v)[16], float mean, float r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) put(v, i, mul2(LAYER ? add2(pair(v, i), F2(-mean)) : pair(v, i), F2(r)));
 }
 
 // 1 / sqrt(sum / cols + eps): the quotient and the hardware's root each with one correction by their remainder.  An error
@@ -218,12 +247,8 @@ __device__ __forceinline__ void put_codes(const Held& h, long long row, int col,
 
 // v += alpha x, where alpha is the sum of two fp32 numbers (a caller's 2.63 is none) of which the second is mostly zero
 __device__ __forceinline__ void add_scaled(float alpha, float alpha_low, const float (&x)[16], float (&v)[16]) {
-  if (alpha_low != 0.f) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmaf(alpha_low, x[j], v[j]);
-  }
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = fmaf(alpha, x[j], v[j]);
+  if (alpha_low != 0.f) add_scaled16(v, alpha_low, x);
+  add_scaled16(v, alpha, x);
 }
 
 // THREADS: 256 where a row takes no more, three CTAs an SM; 512
@@ -287,12 +312,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
     if (POST) post = row_stats<POST == kNormLayer>(v, valid, a.cols, inv_cols, a.eps, sum);
     if (scaled) {
       u_row.get(chunk, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = (POST ? (POST == kNormLayer ? v[j] - post.x : v[j]) * post.y : v[j]) * w[j];
+      if (POST) normalise16<POST == kNormLayer>(v, post.x, post.y);
+      mul16(v, w);
       if (BIAS) {
         ub_row.get(chunk, w);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] += w[j];
+        add16(v, w);
       }
     }
     cx.get(w);
@@ -312,12 +336,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
     }
     const float2 pre = row_stats<PRE_LAYER>(v, valid, a.cols, inv_cols, a.eps, sum);
     pre_w.get(chunk, w);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = (PRE_LAYER ? v[j] - pre.x : v[j]) * pre.y * w[j];
+    normalise16<PRE_LAYER>(v, pre.x, pre.y);
+    mul16(v, w);
     if (PRE_LAYER) {
       pre_b.get(chunk, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] += w[j];
+      add16(v, w);
     }
     if (in) store16(v, static_cast<T*>(a.h) + row * a.cols, col, a.cols, a.out_vec);
     if (a.held_h.codes) {
@@ -365,9 +388,9 @@ struct RowLoads {
 // (value - mean) * rstd of held values; the difference first: a mean far from zero must not cost digits
 template <bool LAYER>
 __device__ __forceinline__ void decode_normed(uint4 codes, unsigned s, float mean, float rstd, float (&v)[16]) {
-  act8_decode(codes, s, v);
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = (LAYER ? v[j] - mean : v[j]) * rstd;
+  const float step = act8_step(s);      // (a code times a step is exact, so these round as often as the formula)
+  const F2 scale(LAYER ? step : step * rstd), off(-mean), r(rstd);
+  act8_codes(codes, [&](int i, F2 q) { put(v, i, LAYER ? mul2(fma2(q, scale, off), r) : mul2(q, scale)); });
 }
 
 // POST: what b~ is read for.  kNoBlock: nothing (neither a norm after the block nor a gate); kGateOnly; an RMS norm, a
@@ -431,17 +454,14 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
     r.dh.get(f);
     decode_normed<PRE_LAYER>(r.qy, r.sy, stats.x, stats.y, hat);
     pre_w.get(chunk, w);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      dw[j] = fmaf(f[j], hat[j], dw[j]);
-      if (PRE_LAYER) db[PRE_LAYER ? j : 0] += f[j];
-      f[j] *= w[j];                                  // c
-    }
+    add_product16(dw, f, hat);
+    if constexpr (PRE_LAYER) add16(db, f);
+    mul16(f, w);                                     // c
     s[0] = dot16(f, hat);
     if constexpr (PRE_LAYER) s[kC] = sum16(f);
     r.dy.get(w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = fmaf(stats.y, f[j], w[j]);
+    for (int i = 0; i < 8; ++i) put(f, i, fma2(F2(stats.y), pair(f, i), pair(w, i)));
     if constexpr (TWO) decode_normed<LAYER>(r.qb, r.sb, stats.z, stats.w, bh);
     r.load(a, row + rpb, col, row + rpb < run.row1);     // the next row's loads are under way during the sums
     if constexpr (NORM) {
@@ -450,8 +470,7 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
         s[kE] = dot16(f, w);
         s[kE + 1] = dot16(hat, w);
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] *= bh[j];      // (u is zero past the end of the row)
+      mul16(w, bh);      // (u is zero past the end of the row)
       s[kB] = dot16(f, w);
       s[kB + 1] = dot16(hat, w);
       if constexpr (PRE_LAYER) s[kD] = sum16(w);
@@ -463,10 +482,10 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
     sum(s);
     const float k1 = stats.y * s[0] * inv_cols, k0 = PRE_LAYER ? stats.y * s[PRE_LAYER ? kC : 0] * inv_cols : 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = fmaf(-k1, hat[j], PRE_LAYER ? f[j] - k0 : f[j]);   // g
+    for (int i = 0; i < 8; ++i) put(f, i, fma2(F2(-k1), pair(hat, i), PRE_LAYER ? add2(pair(f, i), F2(-k0)) : pair(f, i)));   // g
     if (in && a.dx) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] = a.alpha * f[j];
+      for (int i = 0; i < 8; ++i) put(w, i, mul2(F2(a.alpha), pair(f, i)));
       store16(w, static_cast<T*>(a.dx) + row * a.cols, col, a.cols, a.out_vec);
     }
     if constexpr (TWO) {
@@ -475,17 +494,14 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
         for (int j = 0; j < 16; ++j) f[j] = in && col + j < a.cols ? f[j] : 0.f;
       }
       u_row.get(chunk, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        g1[j] = fmaf(f[j], bh[j], g1[j]);
-        if (LAYER) g0[LAYER ? j : 0] += f[j];
-        f[j] *= w[j];
-      }
+      add_product16(g1, f, bh);
+      if constexpr (LAYER) add16(g0, f);
+      mul16(f, w);
       if constexpr (NORM) {
         const float p1 = (s[kB] - k1 * s[kB + 1] - (PRE_LAYER ? k0 * s[PRE_LAYER ? kD : 0] : 0.f)) * inv_cols;
         const float p0 = LAYER ? (s[LAYER ? kE : 0] - k1 * s[LAYER ? kE + 1 : 0] - k0 * sum_u) * inv_cols : 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = stats.w * fmaf(-bh[j], p1, LAYER ? f[j] - p0 : f[j]);
+        for (int i = 0; i < 8; ++i) put(f, i, mul2(F2(stats.w), fma2(pair(bh, i), F2(-p1), LAYER ? add2(pair(f, i), F2(-p0)) : pair(f, i))));
       }
     }
     if (in) store16(f, static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
