@@ -7,14 +7,16 @@
 //             gated: x = [a | b], y = f(a) b, checkpoints of a and b      3 es + 2 1/16 (+ 1 1/32), for an element of y
 //   backward  dx = dy f'(x~);  gated: da = dy b~ f'(a~), db = dy f(a~)    2 es + 1 1/32;  3 es + 2 1/16
 //
-// All four are bound by memory: a thread takes a chunk of sixteen neighbouring elements (32 bytes of a 16-bit type in, 16
-// bytes of codes out: with eight, half of both, pack took 41.6 us where it takes 34.5), two lanes share a group of 32
-// and agree on its largest magnitude by one shuffle.  What hides the latency is the number of threads: with two chunks each,
-// all loads first, the gated backward pass took 89 us for 77, the others as long as with one.  The issue slots are the second limit: at 6.5 TB/s an SM has
-// about 16 of them an element of a bf16 pack and 25 of a forward pass, so the encoder takes a maximum, an FMA, a clamp and
-// 3/4 of a byte shuffle an element, and the functions take one exponential and one reciprocal.
-// Measured, bf16 16384 x 4096 (L2 cold): pack 34.5 us, 5.9 TB/s; unpack 29.5 us, 6.9 TB/s; gated SiLU forward 83 us, 6.5
-// TB/s, and backward 77 us, 7.0 TB/s; 4096 x 4096 GELU forward with both checkpoints 24.1 us, backward 17.3 us.
+// All four are bound by memory, the GELU forward pass with both checkpoints by its issue slots: a thread takes a chunk of
+// sixteen neighbouring elements (32 bytes of a 16-bit type in, 16 bytes of codes out; with eight, half of both, pack took a
+// fifth longer), two lanes share a group of 32 and agree on its largest magnitude by one shuffle.  What hides the latency is
+// the number of threads: with two chunks each, all loads first, the gated backward pass took 89 us for 77, the others as
+// long as with one.  At 6.5 TB/s an SM has about 16 issue slots an element of a bf16 pack and 25 of a forward pass, so
+// arithmetic is on pairs of numbers, the encoder clamps only where a group needs it (together 34.6 -> 29.2 us for
+// pack), and the functions take one exponential and one reciprocal.
+// Measured, bf16 16384 x 4096 (L2 cold): pack 29.2 us, 7.0 TB/s; unpack 28.8 us, 7.1 TB/s; gated SiLU forward 78 us, 6.9
+// TB/s, and backward 77 us, 7.0 TB/s; 4096 x 4096 GELU forward with both checkpoints 19.8 us, 5.1 TB/s, backward 16.1 us,
+// 5.3 TB/s.  (Above the copy rate of 6.5 where the last writes are still in L2.)
 //
 // f is GELU (erf form), GELU (tanh form) or SiLU.  For 16-bit tensors the error function is the rational approximation
 // 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error below 1.5e-7, 2^-22.6: far
@@ -165,20 +167,9 @@ __device__ __forceinline__ void mul16(float (&v)[16], const float (&w)[16]) {
 }
 
 // ---- kernels: thread t of block b takes chunk 256 b + t ----
-// The gated kernels would take 58 registers and 4 blocks an SM, which cost the backward pass an eighth of its time.
-template <class T, bool GATED> constexpr int blocks_an_sm() { return sizeof(T) == 4 ? 1 : (GATED ? 5 : 6); }
-
-struct Place {
-  unsigned row, col;
-  bool in;
-};
-__device__ __forceinline__ Place place_of(const Rows& r) {
-  const unsigned at = blockIdx.x * kBlock + threadIdx.x;
-  Place p{0, 0, at < r.chunks};
-  if (p.in) divmod(r.per_row, at, p.row, p.col);
-  p.col *= 16;
-  return p;
-}
+// Blocks an SM of the gated 16-bit kernels, 5 forward and 4 backward, is what measured best (SiLU, 16384 x 4096): forward 78 us with
+// 5 (48 registers, a few of them spilled) and 80 with 4; backward 77 with 4, 81 with 5; with 6 they spill and take 100 and 118.
+template <class T, bool GATED> constexpr int blocks_an_sm(int gated) { return sizeof(T) == 4 ? 1 : (GATED ? gated : 6); }
 
 template <class T>
 __global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, long long stride, int vec, Rows r, Held held) {
@@ -205,7 +196,7 @@ __global__ void __launch_bounds__(kBlock) unpack_kernel(Held held, T* __restrict
 }
 
 template <class T, int KIND, bool GATED>
-__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>()) forward_kernel(const T* __restrict__ x, long long stride, int vec_x, T* __restrict__ y,
+__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>(5)) forward_kernel(const T* __restrict__ x, long long stride, int vec_x, T* __restrict__ y,
                                                         int vec_y, Rows r, Held held, Held held_b, Held held_y) {
   const Place p = place_of(r);
   const int col = (int)p.col;
@@ -245,7 +236,7 @@ __global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>()) forward_kern
 }
 
 template <class T, int KIND, bool GATED>
-__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>()) backward_kernel(const T* __restrict__ grad, long long stride, int vec_g, T* __restrict__ dx,
+__global__ void __launch_bounds__(kBlock, blocks_an_sm<T, GATED>(4)) backward_kernel(const T* __restrict__ grad, long long stride, int vec_g, T* __restrict__ dx,
                                                          int vec_x, Rows r, Held held, Held held_b) {
   const Place p = place_of(r);
   if (!p.in) return;
