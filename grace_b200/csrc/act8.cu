@@ -171,6 +171,18 @@ __device__ __forceinline__ void mul16(float (&v)[16], const float (&w)[16]) {
 // 5 (48 registers, a few of them spilled) and 80 with 4; backward 77 with 4, 81 with 5; with 6 they spill and take 100 and 118.
 template <class T, bool GATED> constexpr int blocks_an_sm(int gated) { return sizeof(T) == 4 ? 1 : (GATED ? gated : 6); }
 
+struct Place {
+  unsigned row, col;
+  bool in;
+};
+__device__ __forceinline__ Place place_of(const Rows& r) {
+  const unsigned at = blockIdx.x * kBlock + threadIdx.x;
+  Place p{0, 0, at < r.chunks};
+  if (p.in) divmod(r.per_row, at, p.row, p.col);
+  p.col *= 16;
+  return p;
+}
+
 template <class T>
 __global__ void __launch_bounds__(kBlock) pack_kernel(const T* __restrict__ x, long long stride, int vec, Rows r, Held held) {
   const Place p = place_of(r);
