@@ -51,7 +51,7 @@ __device__ __forceinline__ void divmod(const FastDiv& f, unsigned n, unsigned& q
 }
 
 struct Rows {          // which chunks a launch covers
-  unsigned chunks;     // of sixteen columns: rows * (pitch / 16), below 2^31; a multiple of 2
+  unsigned chunks;     // of sixteen columns: rows * (pitch / 16), below 2^28; a multiple of 2
   FastDiv per_row;     // pitch / 16
   int cols;
 };
@@ -281,11 +281,11 @@ Held rows_from(Held h, long long row) {
   return h;
 }
 
-// Calls f(first row, Rows, grid) for slabs of rows whose chunk count fits 31 bits.
+// Calls f(first row, Rows, grid) for slabs of rows of less than 2^28 chunks (2^32 elements; only the rows' offsets need 64 bits).
 template <class F>
 cudaError_t over_slabs(long long rows, int cols, F f) {
   const long long per_row = ((long long)cols + 31) / 32 * 2;
-  const long long slab = ((1ll << 31) - 1) / per_row;
+  const long long slab = ((1ll << 28) - 1) / per_row;
   for (long long at = 0; at < rows; at += slab) {
     const long long n = rows - at < slab ? rows - at : slab;
     Rows r{(unsigned)(n * per_row), make_div((unsigned)per_row), cols};

@@ -59,8 +59,8 @@ def test_extremes(dtype):
     close(got, held_value(x), 0.0)
 
 
-def test_more_chunks_than_31_bits_count_as_slabs():
-    """Offsets in a tensor of more than 2^32 elements (the last rows are compared)."""
+def test_more_elements_than_a_launch_takes():
+    """More than 2^32 elements: offsets past 32 bits, and a second launch for the last rows (which are compared)."""
     rows, cols = (1 << 32) // 4096 + 3, 4096
     x = torch.zeros(rows, cols, dtype=FP16, device="cuda")
     x[-3:] = rand(3, cols, dtype=FP16, seed=2)
@@ -319,3 +319,26 @@ def test_weight_grad_with_a_cold_cache():
         flush.zero_()
         assert torch.equal(act8.weight_grad(g, held, dtype=FP32)[0], want)
     act8.check()
+
+
+def test_largest_magnitude_anywhere():
+    """Each place of a group in turn holds its largest magnitude, of either sign, finite or not."""
+    for dtype in (BF16, FP16, FP32):
+        x = rand(96 * 4, 32, dtype=dtype, seed=31)
+        rows = torch.arange(96 * 4, device="cuda")
+        x[rows, rows % 32] = torch.where(rows % 96 < 48, 9.0, -9.0).to(dtype)
+        x[rows[96:192], rows[96:192] % 32] *= math.inf
+        x[rows[192:288], rows[192:288] % 32] = math.nan
+        held, host = act8.pack(x), act8.pack(x.cpu())
+        assert torch.equal(held.codes.cpu(), host.codes) and torch.equal(held.scales[:, :1].cpu(), host.scales[:, :1])
+
+
+def test_codes_at_their_bounds():
+    """Values that round to +-128 steps are kept at +-127, and only those."""
+    steps = torch.tensor([127.0, 127.25, 127.49999, 127.5, 127.75, 127.99999, 126.5, 125.5])
+    x = torch.cat([steps, -steps, steps / 3, -steps / 7]).repeat(40, 1) * torch.exp2(torch.arange(-20.0, 20.0)).unsqueeze(1)
+    x[::2, 3:6] = 0.25
+    x[::4, 11:14] = -0.125
+    held = act8.pack(x.cuda())
+    assert torch.equal(held.codes.cpu(), act8.pack(x).codes) and held.codes.abs().max() == 127
+    assert torch.equal(act8.unpack(held).cpu().double(), held_value(x))

@@ -169,7 +169,7 @@ def test_residual_factor_is_not_rounded(alpha):
 
 
 @pytest.mark.parametrize("cols", [96, 90])
-def test_parameters_off_their_boundaries(cols):
+def test_parameters_off_their_boundaries_by_one_and_by_four(cols):
     """Slices that start where no four elements do, and rows of a gate that do."""
     d, p = make((3, 5, cols), BF16, "layer", "layer", "sequence", seed=23, device="cuda")
     want = block_norm.residual_norm_forward(d["x"], d["block"], **p)
