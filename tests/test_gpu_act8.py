@@ -342,3 +342,32 @@ def test_codes_at_their_bounds():
     held = act8.pack(x.cuda())
     assert torch.equal(held.codes.cpu(), act8.pack(x).codes) and held.codes.abs().max() == 127
     assert torch.equal(act8.unpack(held).cpu().double(), held_value(x))
+
+
+def test_one_row_without_leading_axes():
+    x = rand(72, dtype=BF16, seed=41).requires_grad_()
+    w, b = rand(40, 72, dtype=BF16, seed=42).requires_grad_(), rand(40, dtype=BF16, seed=43).requires_grad_()
+    y, held = act8.activation(x, "silu", checkpoint_output=True)
+    act8.linear(y, w, b, checkpoint=held).backward(rand(40, dtype=BF16, seed=44))
+    g = rand(40, dtype=BF16, seed=44).double()
+    want = g.unsqueeze(1) * act8.unpack(held, FP32).double()
+    close(w.grad, want, half_step(BF16) * want.abs(), "weight")      # one product, exact in fp32, and one rounding, relative to the value
+    assert torch.equal(b.grad, g.to(BF16)) and x.grad.shape == (72,)
+
+
+def test_calls_on_two_streams_at_once():
+    """Products that fill the GPU, each with its partial sums, next to each other and to a step of the other kernels."""
+    x, g = rand(6000, 1000, dtype=BF16, seed=45), rand(6000, 1032, dtype=BF16, seed=46)
+    held = act8.pack(x)
+    want = act8.weight_grad(g, held, bias=True, dtype=FP32)
+    y = act8.activation_forward(x, "gelu", checkpoint_output=True)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams * 8:
+        with torch.cuda.stream(s):
+            got.append((act8.weight_grad(g, held, bias=True, dtype=FP32), act8.activation_forward(x, "gelu", checkpoint_output=True)))
+    torch.cuda.synchronize()
+    for (dw, db), (z, a, out) in got:
+        assert torch.equal(dw, want[0]) and torch.equal(db, want[1]) and torch.equal(z, y[0])
+        assert torch.equal(a.codes, y[1].codes) and torch.equal(out.codes, y[2].codes)
+    act8.check()
