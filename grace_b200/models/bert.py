@@ -57,9 +57,11 @@ class BertLayer(nn.Module):
         if self.int8:
             from ..ops.block_norm import residual_norm
 
-            return residual_norm(x, block, pre="layer", pre_weight=ln.weight, pre_bias=ln.bias, post=self.post_norm,
-                                 post_weight=None if post is None else post.weight, post_bias=getattr(post, "bias", None), gate=gate,
-                                 residual_scale=self.residual_scale, eps=EPS, return_stream=False, checkpoint_output=True)
+            keep = torch.is_grad_enabled()      # (without a backward pass nothing reads a checkpoint)
+            out = residual_norm(x, block, pre="layer", pre_weight=ln.weight, pre_bias=ln.bias, post=self.post_norm,
+                                post_weight=None if post is None else post.weight, post_bias=getattr(post, "bias", None), gate=gate,
+                                residual_scale=self.residual_scale, eps=EPS, return_stream=False, checkpoint_output=keep)
+            return out if keep else (out, None)
         if post is not None:
             block = post(block)
         if gate is not None:
@@ -77,7 +79,10 @@ class BertLayer(nn.Module):
         a = a.transpose(1, 2).reshape(b, s, h)
         x, held = self._join(x, linear(self.proj, a), self.ln1, self.post1, self.gate1)
         f = linear(self.fc1, x, held)
-        g, held = act8.activation(f, "gelu", checkpoint_output=True) if self.int8 else (F.gelu(f), None)
+        if self.int8 and torch.is_grad_enabled():
+            g, held = act8.activation(f, "gelu", checkpoint_output=True)
+        else:
+            g, held = act8.activation(f, "gelu") if self.int8 else F.gelu(f), None
         return self._join(x, linear(self.fc2, g, held), self.ln2, self.post2, self.gate2)
 
 

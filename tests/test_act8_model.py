@@ -150,3 +150,21 @@ def test_gpu_dropout_and_graph_capture():
     drop = bert_tiny(dropout=0.1, activation_checkpoint="int8").to("cuda", torch.bfloat16)
     drop(ids, mlm_labels=labels, nsp_labels=nsp).backward()
     assert all(torch.isfinite(p.grad).all() for p in drop.parameters())
+
+
+def without_gradients(device, dtype):
+    for form in FORMS:
+        _, held = pair(device, dtype, **form)
+        ids, labels, nsp = batch(device)
+        want = held(ids, mlm_labels=labels, nsp_labels=nsp)
+        with torch.no_grad():
+            assert torch.equal(held(ids, mlm_labels=labels, nsp_labels=nsp), want.detach())
+
+
+def test_cpu_without_gradients():
+    without_gradients("cpu", torch.float32)
+
+
+@pytest.mark.gpu
+def test_gpu_without_gradients():
+    without_gradients("cuda", torch.bfloat16)
