@@ -68,22 +68,34 @@ class BertLayer(nn.Module):
             block = block * gate
         return ln((x if self.residual_scale == 1.0 else self.residual_scale * x) + block), None
 
-    def forward(self, x, mask=None, held=None):
-        """``held``: the checkpoint of ``x`` where the layer before it wrote one.  Returns the new ``x`` and its checkpoint (None without)."""
+    def _linear(self, layer, x, held=None):
+        if not self.int8:
+            return layer(x)
         from ..ops import act8
 
+        return act8.linear(x, layer.weight, layer.bias, checkpoint=held)
+
+    def _gelu(self, x):
+        """GELU, with checkpoints also the Act8 of it."""
+        if not self.int8:
+            return F.gelu(x), None
+        from ..ops import act8
+
+        if torch.is_grad_enabled():
+            return act8.activation(x, "gelu", checkpoint_output=True)
+        return act8.activation(x, "gelu"), None
+
+    def forward(self, x, mask=None, held=None):
+        """The new ``x``.  With ``activation_checkpoint="int8"`` the pair of it and its checkpoint (None without a backward pass), which the
+        next layer takes as ``held``."""
         b, s, h = x.shape
-        linear = (lambda m, v, c=None: act8.linear(v, m.weight, m.bias, checkpoint=c)) if self.int8 else (lambda m, v, c=None: m(v))
-        q, k, v = linear(self.qkv, x, held).view(b, s, 3, self.heads, h // self.heads).permute(2, 0, 3, 1, 4)
+        q, k, v = self._linear(self.qkv, x, held).view(b, s, 3, self.heads, h // self.heads).permute(2, 0, 3, 1, 4)
         a = F.scaled_dot_product_attention(q, k, v, attn_mask=mask)
         a = a.transpose(1, 2).reshape(b, s, h)
-        x, held = self._join(x, linear(self.proj, a), self.ln1, self.post1, self.gate1)
-        f = linear(self.fc1, x, held)
-        if self.int8 and torch.is_grad_enabled():
-            g, held = act8.activation(f, "gelu", checkpoint_output=True)
-        else:
-            g, held = act8.activation(f, "gelu") if self.int8 else F.gelu(f), None
-        return self._join(x, linear(self.fc2, g, held), self.ln2, self.post2, self.gate2)
+        x, held = self._join(x, self._linear(self.proj, a), self.ln1, self.post1, self.gate1)
+        g, held = self._gelu(self._linear(self.fc1, x, held))
+        x, held = self._join(x, self._linear(self.fc2, g, held), self.ln2, self.post2, self.gate2)
+        return (x, held) if self.int8 else x
 
 
 class BertForPreTraining(nn.Module):
@@ -120,7 +132,10 @@ class BertForPreTraining(nn.Module):
         x = self.drop(self.ln(self.tok(ids) + self.pos(pos) + self.typ(token_type)))
         held = None
         for layer in self.layers:
-            x, held = layer(x, held=held)
+            if self.int8:
+                x, held = layer(x, held=held)
+            else:
+                x = layer(x)
         pooled = torch.tanh(self.pooler(x[:, 0]))
         if self.int8:
             from ..ops import act8

@@ -1,6 +1,7 @@
 """BERT with 8-bit activation checkpoints against the same model without: outputs, gradients, parameters, a training step."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from grace_b200.models import bert_tiny
 from grace_b200.models.bert import BertForPreTraining
@@ -168,3 +169,18 @@ def test_cpu_without_gradients():
 @pytest.mark.gpu
 def test_gpu_without_gradients():
     without_gradients("cuda", torch.bfloat16)
+
+
+def test_a_layer_without_the_option_returns_a_tensor():
+    """Callers of a layer, its hooks and wrappers around it get the tensor itself; with the option the pair that the next layer takes."""
+    full, held = pair("cpu", torch.float32)
+    x, seen = torch.randn(2, 16, 64), []
+    for model in (full, held):
+        model.layers[0].register_forward_hook(lambda module, args, out: seen.append(out))
+    ids, _, _ = batch("cpu")
+    full(ids), held(ids)
+    assert isinstance(seen[0], torch.Tensor) and seen[0].shape == (4, 16, 64)
+    y = full.layers[0](x)
+    assert isinstance(y, torch.Tensor) and y.shape == x.shape and torch.equal(torch.utils.checkpoint.checkpoint(full.layers[0], x, use_reentrant=False), y)
+    z, kept = held.layers[0](x)
+    assert kept.shape == x.shape and torch.allclose(y, z, atol=1e-5)
