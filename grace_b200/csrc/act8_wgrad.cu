@@ -24,10 +24,11 @@
 // (where that saves more than it costs: see make_plan); a run that is not a whole tile leaves fp32 partial sums
 // in a workspace, and a second kernel adds a tile's runs in order (no atomics: the same bits on every run).
 //
-// The tensor core truncates where it adds to an fp32 accumulator, which over thousands of tokens adds up to a bias
-// (2.3e-6 of the result after 4096 tokens).  Where the result itself is fp32 the accumulator is therefore emptied every
-// 1536 tokens into the other accumulator's place, rounding to nearest (0.3e-6); kept in the output instead, that cost
-// 40 % more traffic through L2 and as much time.  Sums are fp32 throughout, rounded once to the output's type.
+// The tensor core truncates where it adds to an fp32 accumulator, which adds up to a bias that grows with the tokens (2.2e-6
+// of the result after 4096 of them, half a step of fp16 after some hundred thousand).  The accumulator is therefore emptied every 1536
+// tokens for an fp32 result and every 2048 for a 16-bit one into the other accumulator's place, rounding to nearest; kept in
+// the output instead, that cost 40 % more traffic through L2 and as much time.  What is left of the bias (some 1e-6) does not
+// grow any more.  Sums are fp32 throughout, rounded once to the output's type.
 //
 // What bounds it: shared memory. A step moves 96 KB in and out of an SM's (dY and codes in, codes out and operand in for the
 // decoders, both operands out for the product), 750 cycles at its 128 bytes a cycle, where the product itself takes 512; a
@@ -56,7 +57,11 @@ constexpr int kBoxBytes = kStep * 128; // 64 tokens x 64 features of 16 bits
 constexpr int kBStages = 7, kCodeStages = 5, kAStages = 4;
 constexpr int kDecodeWarp0 = 4, kGroups = 3, kGroupWarps = 4, kEpilogueWarp0 = kDecodeWarp0 + kGroups * kGroupWarps;
 constexpr int kMinSavedSteps = 24;
-constexpr int kChunkSteps = 24;        // steps between two emptyings of the accumulator for an fp32 result
+// Steps between two emptyings of the accumulator, fp32 and 16-bit results (see the header).  4096 x 4096 at 16384 tokens: an fp32
+// result takes 435 us and is off by 2.2e-6 with 64 steps, 453 and 0.6e-6 with 24, 487 and 0.3e-6 with 12; a bf16 one 409 us never
+// emptied, 420 with 64 steps, 434 with 32, 442 with 24, and differs from the rounded product of fp32 matrices by 21e-5, 9.8e-5,
+// 8.0e-5 and 7.7e-5 of itself, of which 7.4e-5 are that product's.
+constexpr int kChunkStepsF32 = 24, kChunkSteps16 = 32;
 constexpr unsigned long long kTimeoutNs = 2000000000ull;
 constexpr unsigned kTmemCols = 512;
 
@@ -736,7 +741,7 @@ Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
     long long n = total / 4 < p.pairs ? total / 4 : p.pairs;
     if (n > p.rest && p.steps - (total + n - 1) / n >= (scattered ? 1 : kMinSavedSteps)) p.rest_pairs = (int)n;
   }
-  p.chunk = out_f32 ? kChunkSteps : p.steps;
+  p.chunk = out_f32 ? kChunkStepsF32 : kChunkSteps16;
   p.work_bytes = p.rest_pairs > p.rest ? (size_t)p.rest_pairs * 2 * kSlotFloats * 4 : 0;
   return p;
 }

@@ -371,3 +371,18 @@ def test_calls_on_two_streams_at_once():
         assert torch.equal(dw, want[0]) and torch.equal(db, want[1]) and torch.equal(z, y[0])
         assert torch.equal(a.codes, y[1].codes) and torch.equal(out.codes, y[2].codes)
     act8.check()
+
+
+@pytest.mark.parametrize("dtype,out", [(FP16, FP16), (BF16, FP32)])
+def test_weight_grad_over_a_quarter_of_a_million_tokens(dtype, out):
+    """Terms of one sign: a sum that stayed in the tensor core's truncating accumulator all along would be short by about 2^-11.5 of itself, with
+    the rounding to fp16 more than half a step for many results."""
+    tokens, n = 1 << 18, 9 * 256                                      # more tiles than pairs of CTAs: none is cut along its tokens
+    g = (torch.rand(tokens, n, generator=torch.Generator(device="cuda").manual_seed(47), device="cuda") * 2 ** -8 + 2 ** -9).to(dtype)
+    x = (torch.rand(tokens, n, generator=torch.Generator(device="cuda").manual_seed(48), device="cuda") + 0.5).to(dtype)
+    held = act8.pack(x)
+    dw, _ = act8.weight_grad(g, held, dtype=out)
+    at = torch.arange(0, n, 67, device="cuda")
+    want = (g[:, at].double().t() @ act8.unpack(held, FP32)[:, at].double()).cpu()
+    # what is truncated is at most a step (2^-23) for each of the 4 x 32 products between two emptyings, each of those rounds once (2^-24)
+    close(dw[at][:, at], want, half_step(out) * want + (128 + tokens / 1536 + 24) * 2.0 ** -23 * want, "dW")
