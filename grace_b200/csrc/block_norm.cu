@@ -249,9 +249,16 @@ __device__ __forceinline__ void put_codes(const Held& h, long long row, int col,
   if ((col & 31) == 0) h.scales[row * h.spitch + (col >> 5)] = (unsigned char)s;
 }
 
-// v += alpha x, where alpha is the sum of two fp32 numbers (a caller's 2.63 is none) of which the second is mostly zero
+// v += alpha x, where alpha is the sum of two fp32 numbers (a caller's 2.63 is none) of which the second is mostly zero.  Where
+// x or the product is infinite the second part says nothing, and of the other sign it would make a NaN of the sum.
 __device__ __forceinline__ void add_scaled(float alpha, float alpha_low, const float (&x)[16], float (&v)[16]) {
-  if (alpha_low != 0.f) add_scaled16(v, alpha_low, x);
+  if (alpha_low != 0.f) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float low = alpha_low * x[j];
+      v[j] += fabsf(low) <= 3.4028235e38f ? low : 0.f;      // (a NaN comes with the other part)
+    }
+  }
   add_scaled16(v, alpha, x);
 }
 

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from _act8_oracle import half_step
 from _block_norm_cases import check, make
 from grace_b200.ops import act8, block_norm
 
@@ -184,3 +185,32 @@ def test_parameters_off_their_boundaries_by_one_and_by_four(cols):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         grads = block_norm.residual_norm_backward(d["dh"], d["dy"], got[2])
         assert all(torch.equal(grads[k], back[k]) for k in back)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("alpha", [2.63, 0.1, -1 / 3, 1.0])
+def test_infinite_stream_keeps_its_sign(alpha, dtype):
+    """alpha x is infinite where x is, whatever the part of alpha that fp32 does not hold, as on the CPU."""
+    x = torch.randn(4, 96, generator=torch.Generator().manual_seed(24)).to(dtype)
+    x[1, 3], x[1, 50], x[2, 7], x[3, 9] = math.inf, -math.inf, -math.inf, math.nan
+    b = torch.full_like(x, 0.25)
+    want = block_norm.residual_norm_forward(x, b, pre="rms", residual_scale=alpha)[1]
+    y = block_norm.residual_norm_forward(x.cuda(), b.cuda(), pre="rms", residual_scale=alpha)[1].cpu()
+    assert torch.equal(y.isnan(), x.isnan()) and torch.equal(want.isnan(), x.isnan())
+    assert torch.equal(y.isinf(), x.isinf()) and torch.equal(y[x.isinf()], (x * math.copysign(1, alpha))[x.isinf()])
+    # b + alpha_low x and the sum with alpha x are each rounded to fp32 (2^-24 of themselves, the first at most 0.25 and 2^-24 of the product),
+    # then y to its type; equal bits are not owed, since the CPU rounds a 64-bit sum once
+    finite = x.isfinite()
+    exact = (alpha * x.double() + 0.25)[finite]
+    part = 0.25 + 2.0 ** -24 * (alpha * x.double()).abs()[finite]
+    least = 2.0 ** -25 if dtype == FP16 else 0.0
+    assert ((y[finite].double() - exact).abs() <= (half_step(dtype) + 2.0 ** -24) * exact.abs() + 2.0 ** -24 * (1 + 2.0 ** -20) * part + least).all()
+
+
+@pytest.mark.parametrize("alpha", [1.1e30, -2.7e37])
+def test_a_product_beyond_the_range_is_infinite(alpha):
+    x = torch.tensor([[1e38, -1e38, 3e20, 1.0]])
+    y = block_norm.residual_norm_forward(x.cuda(), torch.zeros_like(x).cuda(), pre="rms", residual_scale=alpha)[1].cpu()
+    want = (alpha * x.double()).float()
+    assert torch.equal(y.isinf(), want.isinf()) and torch.equal(y[want.isinf()], want[want.isinf()])
+    assert ((y - want)[~want.isinf()].abs() <= 2.0 ** -23 * want[~want.isinf()].abs()).all()
