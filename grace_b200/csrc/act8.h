@@ -32,8 +32,10 @@ cudaError_t launch_act8_backward(const void* grad, long long grad_stride, void* 
 cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held, long long tokens, int outs, int ins, int dtype,
                               int out_f32, void* out, void* bias, void* work, int sms, cudaStream_t stream);
 size_t act8_wgrad_work_bytes(long long tokens, int outs, int ins, int out_f32, int sms);
-// The current device's status block of the bounded waits (16 words, the first 0 if none ran out), cleared if one did.
+// Waits for the current device, all of its streams: its status block of the bounded waits (16 words, the first 0 if none ran
+// out), cleared if one did.
 cudaError_t act8_wgrad_status(unsigned* words);
+cudaError_t act8_wgrad_status_block(void** block);      // where it is in the device's memory
 cudaError_t launch_act8_repitch(const void* src, long long stride, void* dst, long long rows, int cols, cudaStream_t stream);
 
 // ---- residual and norm step between two blocks (block_norm.cu) ----

@@ -782,12 +782,17 @@ size_t act8_wgrad_work_bytes(long long tokens, int outs, int ins, int out_f32, i
   return tokens > 0 && outs > 0 && ins > 0 ? make_plan(tokens, outs, ins, out_f32 != 0, sms).work_bytes : 0;
 }
 
+// The copies run on the legacy stream, which torch's streams do not wait for: read and cleared only once the device is idle.
 cudaError_t act8_wgrad_status(unsigned* words) {
-  cudaError_t err = cudaMemcpyFromSymbol(words, wgrad_status, sizeof(wgrad_status));   // waits for the device's work
+  cudaError_t err = cudaDeviceSynchronize();
+  if (err == cudaSuccess) err = cudaMemcpyFromSymbol(words, wgrad_status, sizeof(wgrad_status));
   if (err != cudaSuccess || words[0] == kOk) return err;
   const unsigned zeros[16] = {};
-  return cudaMemcpyToSymbol(wgrad_status, zeros, sizeof(zeros));
+  err = cudaMemcpyToSymbol(wgrad_status, zeros, sizeof(zeros));
+  return err != cudaSuccess ? err : cudaDeviceSynchronize();
 }
+
+cudaError_t act8_wgrad_status_block(void** block) { return cudaGetSymbolAddress(block, wgrad_status); }
 
 cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held, long long tokens, int outs, int ins, int dtype,
                               int out_f32, void* out, void* bias, void* work, int sms, cudaStream_t stream) {

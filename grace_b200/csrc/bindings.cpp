@@ -341,6 +341,12 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
     return words;
   });
 
+  m.def("act8_wgrad_status_block", []() {
+    void* block = nullptr;
+    check(act8_wgrad_status_block(&block), "act8_wgrad_status_block");
+    return reinterpret_cast<uintptr_t>(block);
+  });
+
   // ---- residual and norm step between two blocks ----
   m.attr("BLOCK_NORM_MAX_COLS") = (int)kBlockNormMaxCols;
   m.def("block_norm_sum_rows", [](long long rows, int cols, long long gate_rows, int sms) {

@@ -303,7 +303,7 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
 
 
 def check(device=None) -> None:
-    """Waits for the device and raises ``GraceCommError`` if a bounded wait of a ``weight_grad`` kernel ran out since the last
+    """Waits for the device, all of its streams, and raises ``GraceCommError`` if a bounded wait of a ``weight_grad`` kernel ran out since the last
     check (its results are NaN)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(device):

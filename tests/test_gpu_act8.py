@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from _act8_oracle import close, function, half_step, held_value
-from grace_b200.ops import act8
+from grace_b200.ops import act8, native
+from grace_b200.ops.exchange import GraceCommError
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -386,3 +387,22 @@ def test_weight_grad_over_a_quarter_of_a_million_tokens(dtype, out):
     want = (g[:, at].double().t() @ act8.unpack(held, FP32)[:, at].double()).cpu()
     # what is truncated is at most a step (2^-23) for each of the 4 x 32 products between two emptyings, each of those rounds once (2^-24)
     close(dw[at][:, at], want, half_step(out) * want + (128 + tokens / 1536 + 24) * 2.0 ** -23 * want, "dW")
+
+
+def test_check_waits_for_side_streams():
+    """A failure that a kernel on a side stream records only after check() was called is reported, once."""
+    class Block:      # the device's status block as an array
+        __cuda_array_interface__ = dict(shape=(16,), typestr="<i4", data=(native().act8_wgrad_status_block(), False), version=3)
+
+    status, fail = torch.as_tensor(Block(), device="cuda"), torch.zeros(16, dtype=torch.int32, device="cuda")
+    fail[:3] = torch.tensor([6, 300, 0], dtype=torch.int32)      # (a bounded wait at a barrier)
+    act8.check()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)                              # some 50 ms
+        status.copy_(fail)
+    assert not s.query()
+    with pytest.raises(GraceCommError):
+        act8.check()
+    assert s.query() and not status.any()
+    act8.check()
