@@ -435,12 +435,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int sub = lane / chunks, rows = 32 / chunks;       // a thread takes the tokens sub, sub + rows, ...
       unsigned it = 0;
       bool ok = true;
-      for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
+      for (int i = 0; piece_at(a, sm, pair, i, p); ++i) {        // (after a failure too: all that is left of the bias is NaN)
         const Tile t = tile_at(a, p.tile, half);
         const int col = t.share * a.bias_cols + (lane % chunks) * 8;      // (tiles past the last share have none)
         const bool mine = col < t.boxes * 64;
         float acc[8] = {};
-        for (int st = p.st0; st < p.st1; ++st, ++it) {
+        for (int st = p.st0; ok && st < p.st1; ++st, ++it) {
           const unsigned slot = it % kBStages;
           ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[slot], (it / kBStages) & 1, kTimeoutNs, status, 550 + slot));
           if (!ok) break;
