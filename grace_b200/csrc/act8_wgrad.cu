@@ -346,8 +346,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Tile t = tile_at(a, p.tile, half);
       for (int st = p.st0; st < p.st1; ++st, ++it, r.next()) {
         if (it >= kBStages) {
-          ok = mbar_wait(&sm.b_used[r.slot], r.parity ^ 1, kTimeoutNs, status, 100 + r.slot) &&
-               (!has_bias || mbar_wait(&sm.b_summed[r.slot], r.parity ^ 1, kTimeoutNs, status, 150 + r.slot));
+          ok = mbar_wait_hint(&sm.b_used[r.slot], r.parity ^ 1, kTimeoutNs, status, 100 + r.slot) &&
+               (!has_bias || mbar_wait_hint(&sm.b_summed[r.slot], r.parity ^ 1, kTimeoutNs, status, 150 + r.slot));
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
@@ -363,8 +363,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // loads that were issued, before the shared memory is let go.
     bool landed = true;
     for (unsigned s = it > kBStages ? it - kBStages : 0; s < it; ++s)
-      landed = mbar_wait(ok ? &sm.b_used[s % kBStages] : &sm.b_full[s % kBStages], (s / kBStages) & 1, 2 * kTimeoutNs, status, 400) && landed;
-    landed = mbar_wait(&sm.done, 0, 2 * kTimeoutNs, status, 800) && landed;
+      landed = mbar_wait_hint(ok ? &sm.b_used[s % kBStages] : &sm.b_full[s % kBStages], (s / kBStages) & 1, 2 * kTimeoutNs, status, 400) && landed;
+    landed = mbar_wait_hint(&sm.done, 0, 2 * kTimeoutNs, status, 800) && landed;
     if (!ok || !landed) sm.failed = 1;
   } else if (warp == 1) {
     // ---- MMAs, by one thread of the pair ----
@@ -380,12 +380,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint32_t idesc = instruction_desc<T>() | ((uint32_t)(t.boxes * 128 >> 3) << 17);
         for (int st = p.st0; ok && st < p.st1; ++item) {
           const unsigned buf = item & two, use = item >> two;
-          if (use >= 1) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[buf], (use - 1) & 1, kTimeoutNs, status, 300 + buf));
+          if (use >= 1) ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.acc_empty[buf], (use - 1) & 1, kTimeoutNs, status, 300 + buf));
           if (!ok) break;
           tc_fence_after();
           const int end = min(st + a.chunk, p.st1);
           for (bool fresh = true; st < end; ++st, ra.next(), rb.next(), fresh = false) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sm.ready[ra.slot], ra.parity, kTimeoutNs, status, 200 + ra.slot));
+            ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.ready[ra.slot], ra.parity, kTimeoutNs, status, 200 + ra.slot));
             if (!ok) break;
             tc_fence_after();
             const uint64_t ad = a_desc + ra.slot * (2 * kBoxBytes >> 4), bd = b_desc + rb.slot * (2 * kBoxBytes >> 4);
@@ -406,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // The other CTA's last arrivals here are on their way without being waited for by anything else, and a barrier
       // between the CTAs does not order them: this CTA has to be there when they land.
       for (unsigned n = item > two + 1 ? item - two - 1 : 0; ok && n < item; ++n)
-        ok = mbar_wait(&sm.acc_empty[n & two], (n >> two) & 1, 2 * kTimeoutNs, status, 350);
+        ok = mbar_wait_hint(&sm.acc_empty[n & two], (n >> two) & 1, 2 * kTimeoutNs, status, 350);
       if (!ok) sm.failed = 1;
     }
   } else if (warp == 2) {
@@ -417,7 +417,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; ok && piece_at(a, sm, pair, i, p); ++i) {
       const Tile t = tile_at(a, p.tile, half);
       for (int st = p.st0; st < p.st1; ++st, ++it, r.next()) {
-        if (it >= kCodeStages) ok = __all_sync(0xffffffffu, mbar_wait(&sm.c_empty[r.slot], r.parity ^ 1, kTimeoutNs, status, 500 + r.slot));
+        if (it >= kCodeStages) ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.c_empty[r.slot], r.parity ^ 1, kTimeoutNs, status, 500 + r.slot));
         if (!ok) break;
         if (elect_one()) {
           mbar_expect_tx(&sm.c_full[r.slot], kStep * kTileK);
@@ -427,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok)
-      for (unsigned s = it > kCodeStages ? it - kCodeStages : 0; s < it; ++s) mbar_wait(&sm.c_full[s % kCodeStages], (s / kCodeStages) & 1, kTimeoutNs, status, 450);
+      for (unsigned s = it > kCodeStages ? it - kCodeStages : 0; s < it; ++s) mbar_wait_hint(&sm.c_full[s % kCodeStages], (s / kCodeStages) & 1, kTimeoutNs, status, 450);
   } else if (warp == 3) {
     // ---- bias gradient: this CTA's share of its columns, eight a thread, the step's tokens dealt to the threads ----
     if (has_bias) {
@@ -442,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float acc[8] = {};
         for (int st = p.st0; ok && st < p.st1; ++st, ++it) {
           const unsigned slot = it % kBStages;
-          ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[slot], (it / kBStages) & 1, kTimeoutNs, status, 550 + slot));
+          ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.b_full[slot], (it / kBStages) & 1, kTimeoutNs, status, 550 + slot));
           if (!ok) break;
           if (mine) {
             const unsigned char* q = sm.b[slot] + (col >> 6) * kBoxBytes;
@@ -502,8 +502,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // codes, and not only for that: a parity tells a phase from its neighbours alone, loads may land out of order, and a
         // group does not look at the other groups' steps.  That an MMA is done means that the codes of all steps before it
         // have been decoded, so that the codes' barrier is in this step's phase or past it.
-        if (n >= kAStages) ok = mbar_wait(&sm.b_used[(n - kAStages) % kBStages], ((n - kAStages) / kBStages) & 1, kTimeoutNs, status, 620 + as);
-        if (ok) ok = mbar_wait(&sm.c_full[cs], (n / kCodeStages) & 1, kTimeoutNs, status, 600 + cs);
+        if (n >= kAStages) ok = mbar_wait_hint(&sm.b_used[(n - kAStages) % kBStages], ((n - kAStages) / kBStages) & 1, kTimeoutNs, status, 620 + as);
+        if (ok) ok = mbar_wait_hint(&sm.c_full[cs], (n / kCodeStages) & 1, kTimeoutNs, status, 600 + cs);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -528,7 +528,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(row + ((j1 ^ (m & 7)) << 4)) = decode8(v, s[j], a.one, T{});
         }
         fence_async_shared();   // the tensor core reads the tile through the async proxy
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.b_full[n % kBStages], (n / kBStages) & 1, kTimeoutNs, status, 640));   // the step's dY is here too
+        ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.b_full[n % kBStages], (n / kBStages) & 1, kTimeoutNs, status, 640));   // the step's dY is here too
         if (!ok) break;
         if (lane == 0) mbar_arrive_at(&sm.ready[as], 0);
       }
@@ -547,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int st = p.st0; st < p.st1; st += a.chunk, ++item) {
         const unsigned buf = item & two, use = item >> two;
         const bool add = st > p.st0, last = st + a.chunk >= p.st1;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_full[buf], use & 1, 2 * kTimeoutNs, status, 700 + buf));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.acc_full[buf], use & 1, 2 * kTimeoutNs, status, 700 + buf));
         tc_fence_after();
         const uint32_t base = tmem + buf * kTileN + quarter, sums = tmem + kTileN + quarter;
         // columns c .. c + 31 of the accumulator, with what earlier emptyings left of them

@@ -21,9 +21,38 @@ __device__ __forceinline__ void mbar_expect_tx(void* bar, unsigned bytes) {
 __device__ __forceinline__ void mbar_arrive(void* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// One try: the hardware suspends the thread until the phase is over or the hint (nanoseconds) has passed, whichever is
-// first.
-__device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity, unsigned hint_ns) {
+__device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Bounded wait; returns false (and records the failure) when the limit expires or another role already failed.
+__device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, uint64_t timeout_ns, const Status& status,
+                                          unsigned detail) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  unsigned spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 0x3f) == 0) {
+      if (status.failed()) return false;
+      if (globaltimer_ns() - t0 > timeout_ns) {
+        status.fail(kTimeoutMbarrier, detail, 0);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
+// The same for kernels whose waits are many and short: a try suspends the thread until the phase is over or the hint
+// (nanoseconds) has passed, and the status word and the clock are looked at once in 64 tries that ran out, about every 1.3 ms,
+// from the first of which the limit counts.  A global load and a clock read in between would answer the barrier a
+// microsecond late, which is longer than the usual wait.
+__device__ __forceinline__ bool mbar_try_wait_hint(void* bar, unsigned parity, unsigned hint_ns) {
   unsigned ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -32,13 +61,10 @@ __device__ __forceinline__ bool mbar_try_wait(void* bar, unsigned parity, unsign
       : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns) : "memory");
   return ok != 0;
 }
-// Bounded wait; returns false (and records the failure) when the limit expires or another role already failed.  The
-// status word and the clock are looked at once in 64 tries that ran out: a global load and a clock read in between
-// would answer the barrier a microsecond late, which is longer than the usual wait.
-__device__ __forceinline__ bool mbar_wait(void* bar, unsigned parity, uint64_t timeout_ns, const Status& status,
-                                          unsigned detail) {
+__device__ __forceinline__ bool mbar_wait_hint(void* bar, unsigned parity, uint64_t timeout_ns, const Status& status,
+                                               unsigned detail) {
   uint64_t t0 = 0;
-  for (unsigned spins = 1; !mbar_try_wait(bar, parity, 20000); ++spins) {
+  for (unsigned spins = 1; !mbar_try_wait_hint(bar, parity, 20000); ++spins) {
     if ((spins & 0x3f) == 0) {
       if (status.failed()) return false;
       const uint64_t now = globaltimer_ns();
