@@ -530,6 +530,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         fence_async_shared();   // the tensor core reads the tile through the async proxy
         ok = __all_sync(0xffffffffu, mbar_wait_hint(&sm.b_full[n % kBStages], (n / kBStages) & 1, kTimeoutNs, status, 640));   // the step's dY is here too
         if (!ok) break;
+        __syncwarp();      // (lane 0 arrives for the whole warp's stores; a vote orders no memory)
         if (lane == 0) mbar_arrive_at(&sm.ready[as], 0);
       }
       it += p.st1 - p.st0;
