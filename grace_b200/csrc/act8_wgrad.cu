@@ -723,6 +723,7 @@ bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64
 // How a call is cut up.
 struct Plan {
   int tiles_k, tiles, steps, pairs, whole, rest, rest_pairs, chunk;
+  int longest;          // steps of the longest piece
   size_t work_bytes;
 };
 Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
@@ -743,6 +744,7 @@ Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
     if (n > p.rest && p.steps - (total + n - 1) / n >= (scattered ? 1 : kMinSavedSteps)) p.rest_pairs = (int)n;
   }
   p.chunk = out_f32 ? kChunkStepsF32 : kChunkSteps16;
+  p.longest = p.whole || p.rest_pairs == p.rest ? p.steps : (int)(((long long)p.rest * p.steps + p.rest_pairs - 1) / p.rest_pairs);
   p.work_bytes = p.rest_pairs > p.rest ? (size_t)p.rest_pairs * 2 * kSlotFloats * 4 : 0;
   return p;
 }
@@ -815,7 +817,7 @@ cudaError_t launch_act8_wgrad(const void* grad, long long grad_stride, Held held
     while (bias_cols * plan.tiles_k < kHalfN) bias_cols *= 2;
   }
   const WgradArgs a{held.scales, held.spitch, tokens, outs, ins, plan.tiles_k, plan.pairs, plan.whole, plan.rest, plan.rest_pairs,
-                    plan.steps, plan.chunk, plan.chunk < plan.steps ? 1 : 0, 1u, bias_cols, out, bias, static_cast<float*>(work)};
+                    plan.steps, plan.chunk, plan.chunk < plan.longest ? 1 : 0, 1u, bias_cols, out, bias, static_cast<float*>(work)};
   if (dtype == kGradBF16)
     return out_f32 ? launch_typed<__nv_bfloat16, float>(map_dy, map_codes, a, stream)
                    : launch_typed<__nv_bfloat16, __nv_bfloat16>(map_dy, map_codes, a, stream);
