@@ -141,6 +141,11 @@ def _launch(device: torch.device, launch, *args) -> None:
             launch(*args, _stream_ptr(index))
 
 
+def _autocast_type(x: torch.Tensor) -> Optional[torch.dtype]:
+    """The type that products are computed in on ``x``'s device, None without autocast."""
+    return torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else None
+
+
 def _check_tensor(x, what: str) -> None:
     if not isinstance(x, torch.Tensor):
         raise TypeError("%s: a tensor, not %s" % (what, type(x).__name__))
@@ -409,8 +414,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            ) -> torch.Tensor:
     """``x W^T + b`` whose backward pass keeps an 8-bit checkpoint of ``x`` in the place of ``x``.  ``checkpoint``: that of ``x``, where
     the operation that made ``x`` wrote it already (``activation`` and ``residual_norm`` do on request)."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        t = torch.get_autocast_dtype("cuda")
+    t = _autocast_type(x)
+    if t is not None:
         x, weight, bias = x.to(t), weight.to(t), None if bias is None else bias.to(t)
     if not (torch.is_grad_enabled() and weight.requires_grad):
         return F.linear(x, weight, bias)       # nothing reads x again

@@ -22,7 +22,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import native
-from .act8 import Act8, _at, _check_tensor, _decode_cpu, _encode_cpu, _launch, _new_like, _ptrs, _sms, empty_like, pitch_of
+from .act8 import Act8, _at, _autocast_type, _check_tensor, _decode_cpu, _encode_cpu, _launch, _new_like, _ptrs, _sms, empty_like, pitch_of
 from .exchange import GRAD_DTYPE
 
 NORMS = {None: 0, "rms": 1, "layer": 2}
@@ -302,10 +302,14 @@ def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", p
                   post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
                   eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False):
     """``residual_norm_forward`` with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
-    alone comes as it is, several as a tuple.  Under autocast ``x`` and ``block`` are taken in its type (parameters stay as they are)."""
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
-        t = torch.get_autocast_dtype("cuda")
-        x, block = x.to(t), block.to(t)      # the stream between kernels; inside, all arithmetic is fp32
+    alone comes as it is, several as a tuple.  Under autocast ``x`` and ``block`` are taken, and results returned, in the wider of their two
+    types, as a sum of them has it: a stream in fp32 stays in fp32 where the blocks compute in 16 bits."""
+    if _autocast_type(x) is not None:
+        t = torch.promote_types(x.dtype, block.dtype)
+        t = t if t in GRAD_DTYPE else torch.float32
+        x, block = x.to(t), block.to(t)
+        pre_weight, pre_bias, post_weight, post_bias, gate = (
+            p if p is None or p.dtype in (t, torch.float32) else p.to(t) for p in (pre_weight, pre_bias, post_weight, post_bias, gate))
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, pre_weight, pre_bias, post_weight, post_bias, gate))):
         h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
                                             post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps, return_stream=return_stream,

@@ -184,3 +184,20 @@ def test_a_layer_without_the_option_returns_a_tensor():
     assert isinstance(y, torch.Tensor) and y.shape == x.shape and torch.equal(torch.utils.checkpoint.checkpoint(full.layers[0], x, use_reentrant=False), y)
     z, kept = held.layers[0](x)
     assert kept.shape == x.shape and torch.allclose(y, z, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS)
+def test_gpu_autocast_has_the_same_stream(form):
+    """Under autocast the stream of fp32 parameters is fp32 with and without the option, and one sub-layer's join on the same values gives
+    the same to fp32's rounding."""
+    full, held = pair("cuda", torch.float32, **form)
+    g = torch.Generator().manual_seed(5)
+    x, block = torch.randn(3, 16, 64, generator=g).cuda(), torch.randn(3, 16, 64, generator=g).to("cuda", torch.bfloat16)
+    a, b = full.layers[0], held.layers[0]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want, _ = a._join(x, block.float(), a.ln1, a.post1, a.gate1)      # (a norm of a bf16 block would round to bf16 on its way)
+        got, kept = b._join(x, block, b.ln1, b.post1, b.gate1)
+        outs = a(x), b(x)[0]
+    assert got.dtype == want.dtype == kept.dtype == outs[0].dtype == outs[1].dtype == torch.float32
+    assert ((got - want).abs() <= 2e-6 * (1 + want.abs())).all()

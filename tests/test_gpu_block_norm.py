@@ -214,3 +214,25 @@ def test_a_product_beyond_the_range_is_infinite(alpha):
     want = (alpha * x.double()).float()
     assert torch.equal(y.isinf(), want.isinf()) and torch.equal(y[want.isinf()], want[want.isinf()])
     assert ((y - want)[~want.isinf()].abs() <= 2.0 ** -23 * want[~want.isinf()].abs()).all()
+
+
+@pytest.mark.parametrize("kind", [BF16, FP16])
+def test_autocast_keeps_the_stream(kind):
+    """A stream in fp32 next to blocks in 16 bits: the sum is fp32's own, to the bit, and the norm of it that of fp32."""
+    g = torch.Generator().manual_seed(25)
+    x, b, w = (torch.randn(*s, generator=g).cuda() for s in ((6, 72), (6, 72), (72,)))
+    b = b.to(kind).requires_grad_()
+    x.requires_grad_()
+    with torch.autocast("cuda", dtype=kind):
+        h, y, held = block_norm.residual_norm(x, b, pre="rms", pre_weight=w, checkpoint_output=True)
+    assert h.dtype == y.dtype == held.dtype == FP32 and torch.equal(y, x + b)
+    want = torch.nn.functional.rms_norm((x + b).double(), (72,), w.double(), 1e-5)
+    assert ((h - want).abs() <= 1e-6 * (1 + want.abs())).all()
+    torch.autograd.backward((h, y), (torch.ones_like(h), torch.ones_like(y)))
+    assert x.grad.dtype == FP32 and b.grad.dtype == kind and torch.equal(b.grad, x.grad.to(kind))
+    with torch.autocast("cuda", dtype=kind):       # a stream in 16 bits stays in 16 bits; one without gradients is treated alike
+        assert block_norm.residual_norm(x.detach().to(kind), b.detach(), pre="rms", pre_weight=w)[1].dtype == kind
+        assert torch.equal(block_norm.residual_norm(x.detach(), b.detach(), pre="rms", pre_weight=w.to(kind))[1], y.detach())
+        assert block_norm.residual_norm(x.detach().double(), b.detach(), pre="rms", pre_weight=w)[1].dtype == FP32
+    with pytest.raises(ValueError):
+        block_norm.residual_norm(x.detach(), b.detach(), pre="rms", pre_weight=w)
