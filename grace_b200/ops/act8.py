@@ -143,7 +143,8 @@ def _launch(device: torch.device, launch, *args) -> None:
 
 def _autocast_type(x: torch.Tensor) -> Optional[torch.dtype]:
     """The type that products are computed in on ``x``'s device, None without autocast."""
-    return torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else None
+    kind = "cuda" if x.is_cuda else "cpu"
+    return torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else None
 
 
 def _check_tensor(x, what: str) -> None:
@@ -283,7 +284,9 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
         raise TypeError("act8.weight_grad: results in grad's type or fp32, not %s" % dtype)
     if not grad.is_cuda:
         g = _rows(grad).float()
-        return (g.t() @ _decode_cpu(held).reshape(rows, ins)).to(dtype), g.sum(0).to(dtype) if bias else None
+        with torch.autocast("cpu", enabled=False):      # (the product is one of fp32 numbers whatever the caller's)
+            dw = g.t() @ _decode_cpu(held).reshape(rows, ins)
+        return dw.to(dtype), g.sum(0).to(dtype) if bias else None
     if grad.dtype == torch.float32:
         raise TypeError("act8.weight_grad: the tensor cores take bf16 or fp16 gradients; run the layer in one of them")
     if rows > MAX_TOKENS or outs * 2 > 1 << 31:

@@ -164,3 +164,34 @@ def test_weight_shared_by_two_layers():
 def test_a_checkpoint_too_wide_is_refused():
     with pytest.raises(ValueError, match="2\\^30 columns"):
         act8.Act8(torch.empty(0, 0, dtype=torch.int8), torch.empty(0, 0, dtype=torch.uint8), (0, (1 << 30) + 1), torch.bfloat16)
+
+
+@pytest.mark.parametrize("given", [None, "act8"])
+def test_linear_under_autocast(given):
+    """As the library's layer: computed in autocast's type, gradients in the leaves' own."""
+    x, w, b = rand(6, 40, seed=14).requires_grad_(), rand(24, 40, seed=15).requires_grad_(), rand(24, seed=16).requires_grad_()
+    g = rand(6, 24, seed=17, dtype=torch.bfloat16)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = act8.linear(x, w, b, checkpoint=None if given is None else act8.pack(x.detach()))
+        assert torch.equal(y, torch.nn.functional.linear(x, w, b))
+        with torch.no_grad():
+            assert torch.equal(act8.linear(x, w, b), y)
+    assert y.dtype == torch.bfloat16
+    y.backward(g)
+    assert x.grad.dtype == w.grad.dtype == b.grad.dtype == torch.float32
+    held, gd = held_value(x.detach() if given else x.detach().bfloat16()), g.double()
+    half = half_step(torch.bfloat16)
+    want, size = gd.t() @ held, gd.abs().t() @ held.abs()
+    close(w.grad, want, half * want.abs() + 6 * 2.0 ** -24 * size, "dW")
+    close(b.grad, gd.sum(0), half * gd.sum(0).abs() + 6 * 2.0 ** -24 * gd.abs().sum(0), "db")
+    wd = w.detach().bfloat16().double()
+    want, size = gd @ wd, gd.abs() @ wd.abs()
+    close(x.grad, want, half * want.abs() + 24 * 2.0 ** -24 * size, "dx")
+
+
+def test_weight_grad_sums_in_fp32_under_autocast():
+    x, g = rand(50, 32, seed=18), rand(50, 8, seed=19)
+    want = act8.weight_grad(g, act8.pack(x), bias=True)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = act8.weight_grad(g, act8.pack(x), bias=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

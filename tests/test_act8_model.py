@@ -201,3 +201,10 @@ def test_gpu_autocast_has_the_same_stream(form):
         outs = a(x), b(x)[0]
     assert got.dtype == want.dtype == kept.dtype == outs[0].dtype == outs[1].dtype == torch.float32
     assert ((got - want).abs() <= 2e-6 * (1 + want.abs())).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_cpu_autocast(form):
+    full, held = pair("cpu", torch.float32, **form)
+    # as on the GPU: both arms round to bf16 between the layers' products, at different places
+    compare(losses_and_gradients(full, "cpu", torch.bfloat16), losses_and_gradients(held, "cpu", torch.bfloat16), 2e-2, 0.15)

@@ -136,3 +136,15 @@ def test_residual_factor_is_not_rounded(alpha):
     y = block_norm.residual_norm_forward(x, torch.zeros_like(x), pre="rms", residual_scale=alpha)[1].double()
     want = alpha * x.double()
     assert bool(((y - want).abs() <= 2 ** -24 * (1 + 2 ** -20) * torch.exp2(torch.floor(torch.log2(want.abs())) + 1)).all())
+
+
+def test_autocast_keeps_the_stream():
+    """A stream in fp32 next to blocks in 16 bits: the sum is fp32's own, to the bit."""
+    g = torch.Generator().manual_seed(25)
+    x, b, w = torch.randn(6, 72, generator=g), torch.randn(6, 72, generator=g).bfloat16().requires_grad_(), torch.randn(72, generator=g)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        h, y, held = block_norm.residual_norm(x, b, pre="rms", pre_weight=w, checkpoint_output=True)
+        assert block_norm.residual_norm(x.bfloat16(), b.detach(), pre="rms", pre_weight=w)[1].dtype == torch.bfloat16
+    assert h.dtype == y.dtype == held.dtype == torch.float32 and torch.equal(y, x + b)
+    h.sum().backward()
+    assert b.grad.dtype == torch.bfloat16 and b.grad.isfinite().all()
