@@ -406,3 +406,20 @@ def test_check_waits_for_side_streams():
         act8.check()
     assert s.query() and not status.any()
     act8.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gelu_in_its_negative_tail(dtype):
+    """Relative to the value, down to where it leaves fp32's normal range: the approximation of the distribution function (2.2e-5), the exponent's
+    rounding (x^2 / 2 times a few 2^-24) and the rounding to the type."""
+    x = -torch.linspace(0.01, 13.0, 4001).to(dtype).view(-1, 1)
+    y, held, _ = act8.activation_forward(x.cuda(), "gelu")
+    dx = act8.activation_backward(torch.ones_like(x).cuda(), held, "gelu")
+    least = 2.0 ** -25 if dtype == FP16 else 0.0
+    rel = lambda v: 2.2e-5 + (v * v / 2 + 2) * 2.0 ** -22  # noqa: E731
+    f, _ = function(x, "gelu")
+    close(y, f, (half_step(dtype) + rel(x.double())) * f.abs() + least, "y")
+    h = held_value(x)
+    _, d = function(h, "gelu")
+    p, density = 0.5 * torch.special.erfc(-h / math.sqrt(2)), torch.exp(-h * h / 2) / math.sqrt(2 * math.pi)
+    close(dx, d, half_step(dtype) * d.abs() + rel(h) * (p + h.abs() * density) + least, "dx")
