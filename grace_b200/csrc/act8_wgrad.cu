@@ -181,13 +181,16 @@ __device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, unsigned one, __nv
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 // fp16 has the significand to take a code whole (1024 + byte), but not the exponents: the scale goes on in two factors,
-// 2^-6 and 2^(s - 121), so that its range reaches from 2^-30 to 2^9, that of groups of fp16 values; the first product is
-// exact and the second rounds once, into the subnormals.  A group beyond fp16's range reads as NaN.
+// 2^-6 and 2^(s - 121), so that its range reaches from 2^-30 to 2^9, that of groups of fp16 values (2^-7 and 2^-24 for one
+// scale more, which only groups of wider types have); the first product is exact and the second rounds once, into the
+// subnormals.  A group with a value of 2^16 or more reads as NaN.
 __device__ __forceinline__ uint4 decode8(uint2 c, unsigned s, unsigned, __half) {
-  // 2^(s - 121): normal, subnormal, or below 2^-24, where every value rounds to zero
-  const unsigned f = s > 136u ? 0x7e00u : (s >= 107u ? (s - 106u) << 10 : (s >= 97u ? 1u << (s - 97u) : 0u));
+  // 2^(s - 121): normal or subnormal; below s = 96 every value is below 2^-25 and rounds to zero
+  const bool least = s == 96u;
+  const unsigned f = s > 136u ? 0x7e00u : (s >= 107u ? (s - 106u) << 10 : (s >= 97u ? 1u << (s - 97u) : (least ? 1u : 0u)));
   const __half2 scale = __half2half2(__ushort_as_half((unsigned short)f));
-  const __half2 sixth = __half2half2(__ushort_as_half(0x2400)), offset = __half2half2(__ushort_as_half(0xcc80));   // 2^-6, -18 = -1152 * 2^-6
+  const __half2 sixth = __half2half2(__ushort_as_half(least ? 0x2000 : 0x2400));       // 2^-6, or 2^-7,
+  const __half2 offset = __half2half2(__ushort_as_half(least ? 0xc880 : 0xcc80));      // times -1152: -18, or -9
   c.x ^= 0x80808080u;
   c.y ^= 0x80808080u;
   const unsigned w[4] = {c.x, c.x >> 8, c.y, c.y >> 8};

@@ -215,6 +215,15 @@ def _decode_cpu(held: Act8) -> torch.Tensor:
     return v.view(rows, pitch)[:, : held.shape[-1]].reshape(held.shape)
 
 
+def _operand_cpu(held: Act8, dtype: torch.dtype) -> torch.Tensor:
+    """``_decode_cpu`` as the product with a gradient of ``dtype`` takes it."""
+    v = _decode_cpu(held)
+    if dtype != torch.float16:
+        return v
+    wide = (held.scales[:, : held.pitch // GROUP] > 136).repeat_interleave(GROUP, 1)[:, : held.shape[-1]].reshape(held.shape)
+    return torch.where(wide, torch.full_like(v, math.nan), v.half().float())
+
+
 def _function_cpu(x: torch.Tensor, kind: str) -> Tuple[torch.Tensor, torch.Tensor]:
     if kind == "gelu":
         p = 0.5 * torch.erfc(-x * math.sqrt(0.5))
@@ -270,8 +279,9 @@ def _sms(device: torch.device) -> int:
 def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optional[torch.dtype] = None
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(dW, db)`` of ``y = x W^T + b``: ``dW [outs, ins] = sum over rows of grad^T x~`` with ``x~`` the values of ``held``, and with
-    ``bias`` the column sums of ``grad`` (else None).  ``grad`` is ``[..., outs]`` with ``held``'s leading axes and, on the GPU,
-    bf16 or fp16 like it; the results are of ``grad``'s type or, with ``dtype=torch.float32``, not rounded below fp32."""
+    ``bias`` the column sums of ``grad`` (else None).  ``grad`` is ``[..., outs]`` with ``held``'s leading axes and, on the GPU, bf16 or
+    fp16; the results are of ``grad``'s type or, with ``dtype=torch.float32``, not rounded below fp32.  With an fp16 gradient ``x~`` is
+    taken in fp16: a checkpoint of another type is rounded where fp16 is subnormal, and a group of it with a value of 2^16 or more is NaN."""
     _check_tensor(grad, "act8.weight_grad: grad")
     outs, ins, rows = grad.shape[-1], held.shape[-1], held.rows
     if grad.shape[:-1] != held.shape[:-1]:
@@ -285,7 +295,7 @@ def weight_grad(grad: torch.Tensor, held: Act8, bias: bool = False, dtype: Optio
     if not grad.is_cuda:
         g = _rows(grad).float()
         with torch.autocast("cpu", enabled=False):      # (the product is one of fp32 numbers whatever the caller's)
-            dw = g.t() @ _decode_cpu(held).reshape(rows, ins)
+            dw = g.t() @ _operand_cpu(held, grad.dtype).reshape(rows, ins)
         return dw.to(dtype), g.sum(0).to(dtype) if bias else None
     if grad.dtype == torch.float32:
         raise TypeError("act8.weight_grad: the tensor cores take bf16 or fp16 gradients; run the layer in one of them")

@@ -195,3 +195,24 @@ def test_weight_grad_sums_in_fp32_under_autocast():
     with torch.autocast("cpu", dtype=torch.bfloat16):
         got = act8.weight_grad(g, act8.pack(x), bias=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def check_fp16_operand(dtype, device):
+    """A checkpoint of a wider type meets an fp16 gradient as its values rounded to fp16, half a step of 2^-24 at most where they are
+    subnormal; a group with a value of 2^16 or more is NaN, and with it its columns."""
+    g = torch.Generator().manual_seed(20)
+    x = torch.zeros(50, 128)
+    x[:, :64] = (torch.rand(50, 64, generator=g) * 2 - 1) * torch.exp2(torch.arange(50) - 34.0).unsqueeze(1)      # groups from 2^-35 to 2^15
+    x[:, 64:] = torch.randn(50, 64, generator=g)
+    x[7, 70], x[9, 100] = 65536.0, 65000.0
+    held = act8.pack(x.to(device, dtype))
+    dw = act8.weight_grad(torch.eye(50, dtype=torch.float16, device=device), held, dtype=torch.float32)[0].cpu()
+    want = act8.unpack(held, torch.float32).cpu().half().float()
+    assert dw[:, 64:96].isnan().all()
+    keep = [c for c in range(128) if not 64 <= c < 96]
+    assert torch.equal(dw[:, keep], want[:, keep]) and (want[:12, :64] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weight_grad_with_an_fp16_gradient_of_another_types_checkpoint(dtype):
+    check_fp16_operand(dtype, "cpu")

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from _act8_oracle import close, function, half_step, held_value
+from test_act8_cpu import check_fp16_operand
 from grace_b200.ops import act8, native
 from grace_b200.ops.exchange import GraceCommError
 
@@ -423,3 +424,8 @@ def test_gelu_in_its_negative_tail(dtype):
     _, d = function(h, "gelu")
     p, density = 0.5 * torch.special.erfc(-h / math.sqrt(2)), torch.exp(-h * h / 2) / math.sqrt(2 * math.pi)
     close(dx, d, half_step(dtype) * d.abs() + rel(h) * (p + h.abs() * density) + least, "dx")
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_weight_grad_with_an_fp16_gradient_of_another_types_checkpoint(dtype):
+    check_fp16_operand(dtype, "cuda")
