@@ -171,6 +171,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 def _at(x: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
     """``_rows`` for a launch: the tensor to keep until then, its address, and the distance between its rows."""
+    if x.is_neg():             # a view that changes the sign (``z.conj().imag``): memory has the other one
+        x = x.detach().resolve_neg()
     if x.is_contiguous():      # no view is made: that would take longer than the checks of the whole call
         return x, x.data_ptr(), x.shape[-1]
     x = _rows(x)

@@ -118,7 +118,7 @@ def _check(x, block, pre, post, params, residual_scale, eps) -> int:
 
 def _param_ptrs(params):
     """The parameters' addresses, and the tensors that have to live until the launch."""
-    kept = [p if p is None or p.is_contiguous() else p.detach().contiguous() for p in params]
+    kept = [p if p is None or (p.is_contiguous() and not p.is_neg()) else p.detach().resolve_neg().contiguous() for p in params]
     return [0 if p is None else p.data_ptr() for p in kept], kept
 
 

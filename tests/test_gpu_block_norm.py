@@ -236,3 +236,19 @@ def test_autocast_keeps_the_stream(kind):
         assert block_norm.residual_norm(x.detach().double(), b.detach(), pre="rms", pre_weight=w)[1].dtype == FP32
     with pytest.raises(ValueError):
         block_norm.residual_norm(x.detach(), b.detach(), pre="rms", pre_weight=w)
+
+
+def test_views_that_change_the_sign():
+    """The imaginary part of a conjugate is a view of memory with the other sign, in rows of one column without a stride to show it."""
+    z = torch.randn(6, 40, dtype=torch.complex64, generator=torch.Generator().manual_seed(26)).cuda()
+    for v in (z.conj().imag, z[:, :1].conj().imag, torch._neg_view(z.real.contiguous())):
+        assert v.is_neg()
+        c = v.clone()
+        assert not c.is_neg() and torch.equal(act8.unpack(act8.pack(v)), act8.unpack(act8.pack(c)))
+        assert torch.equal(act8.activation(v, "silu"), act8.activation(c, "silu"))
+        w = v[0]
+        h, y, saved = block_norm.residual_norm_forward(v, v, pre="rms", pre_weight=w)
+        h2, y2, saved2 = block_norm.residual_norm_forward(c, c, pre="rms", pre_weight=c[0])
+        assert torch.equal(h, h2) and torch.equal(y, y2)
+        a, b = block_norm.residual_norm_backward(v, v, saved), block_norm.residual_norm_backward(c, c, saved2)
+        assert torch.equal(a["x"], b["x"]) and torch.equal(a["pre_weight"], b["pre_weight"])
