@@ -23,7 +23,20 @@ cudaError_t symm_alloc(void** ptr, size_t bytes) {
   return cudaDeviceSynchronize();
 }
 
-cudaError_t symm_free(void* ptr) { return cudaFree(ptr); }
+namespace {
+// The garbage collector may release a heap while this process captures a graph.  Freeing is no part of the capture, but would
+// invalidate it in any mode but the relaxed one.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
+cudaError_t symm_free(void* ptr) {
+  RelaxedCapture relaxed;
+  return cudaFree(ptr);
+}
 
 cudaError_t symm_export(void* ptr, char* handle_out) {
   cudaIpcMemHandle_t h;
@@ -39,7 +52,10 @@ cudaError_t symm_import(const char* handle, void** ptr) {
   return cudaIpcOpenMemHandle(ptr, h, cudaIpcMemLazyEnablePeerAccess);
 }
 
-cudaError_t symm_release(void* ptr) { return cudaIpcCloseMemHandle(ptr); }
+cudaError_t symm_release(void* ptr) {
+  RelaxedCapture relaxed;
+  return cudaIpcCloseMemHandle(ptr);
+}
 
 cudaError_t symm_enable_peer(int peer_device) {
   int dev = 0;

@@ -221,3 +221,31 @@ def test_general_qsgd_buckets_and_levels(bucket, q, W):
         torch.testing.assert_close(outs[0][off:off + n], expect / W, rtol=1e-5, atol=1e-6)
         for r in range(1, W):     # (the gaps between tensors are nobody's business)
             assert torch.equal(outs[0][off:off + n], outs[r][off:off + n])
+
+
+def test_a_heap_released_during_a_capture_leaves_the_graph_whole():
+    """The garbage collector may come upon a dropped communicator in the middle of a capture: its memory is freed, the capture goes on."""
+    import gc
+
+    from grace_b200 import grace_from_params
+    from grace_b200.ops.exchange import FlatLayout
+
+    def dropped():      # a communicator in a cycle, which reference counting alone does not free
+        grc = grace_from_params({"compressor": "qsgd", "memory": "residual", "communicator": "allgather", "quantum_num": 64, "world_size": 1,
+                                 "fused": True})
+        grc.step_flat(_rand(4096), FlatLayout(["a"], [4096]))
+        grc.check()
+        grc.itself = grc
+
+    gc.collect()
+    dropped()
+    x = torch.ones(64, device=_dev())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        assert gc.collect() > 0
+        z = y * 2
+    x.fill_(3)
+    graph.replay()
+    assert (z == 8).all()
