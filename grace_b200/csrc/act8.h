@@ -56,6 +56,7 @@ struct BlockNormArgs {
   const void *x, *block;
   long long x_stride, block_stride;
   void *h, *y;               // contiguous; y null: not wanted
+  // (block and dblock may be of a 16-bit type where all else is fp32)
   // backward
   const void *grad_h, *grad_y;   // grad_y null: nothing reads the stream
   long long grad_h_stride, grad_y_stride;
@@ -63,7 +64,7 @@ struct BlockNormArgs {
   void *pre_weight_grad, *pre_bias_grad, *post_weight_grad, *post_bias_grad, *gate_grad;   // null: not wanted
   float* sums;               // [runs of the backward pass][4][pitch] scratch (BlockNormShape)
   // filled in by the launchers
-  int x_vec, block_vec, out_vec, grad_h_vec, grad_y_vec;   // RowAlign (act8.cuh)
+  int x_vec, block_vec, out_vec, dblock_vec, grad_h_vec, grad_y_vec;   // RowAlign (act8.cuh)
   int params_vec;                // the parameters may be read in fours
   int parts;
 };
@@ -73,7 +74,8 @@ struct BlockNormShape {
   int sequences, parts, runs;
 };
 BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, int sms, bool backward);
-cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
-cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream);
+// block_dtype: of block and dblock; dtype's own, or one of 16 bits beside fp32
+cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int block_dtype, int sms, cudaStream_t stream);
+cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int block_dtype, int sms, cudaStream_t stream);
 
 }  // namespace grace

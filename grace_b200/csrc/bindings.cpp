@@ -355,7 +355,7 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
   // params: pre_weight, pre_bias, post_weight, post_bias, gate; held: codes and scales of y, block and h
   m.def("block_norm_forward",
         [](uintptr_t x, long long x_stride, uintptr_t block, long long block_stride, uintptr_t h, uintptr_t y, uintptr_t stats,
-           long long rows, int cols, int dtype, int pre, int post, int params_f32, double alpha, float eps, long long gate_rows,
+           long long rows, int cols, int dtype, int block_dtype, int pre, int post, int params_f32, double alpha, float eps, long long gate_rows,
            const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 6>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
           BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, eps, gate_rows, params, stats);
           a.held_y = held(helds[0], helds[1], pitch, spitch);
@@ -363,12 +363,12 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
           a.held_h = held(helds[4], helds[5], pitch, spitch);
           a.x = ptr<const void>(x); a.x_stride = x_stride; a.block = ptr<const void>(block); a.block_stride = block_stride;
           a.h = ptr<void>(h); a.y = ptr<void>(y);
-          check(launch_block_norm_forward(a, dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_forward");
+          check(launch_block_norm_forward(a, dtype, block_dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_forward");
         });
   // grads: of params, in their order
   m.def("block_norm_backward",
         [](uintptr_t grad_h, long long grad_h_stride, uintptr_t grad_y, long long grad_y_stride, uintptr_t dx, uintptr_t dblock,
-           uintptr_t stats, uintptr_t sums, long long rows, int cols, int dtype, int pre, int post, int params_f32, double alpha,
+           uintptr_t stats, uintptr_t sums, long long rows, int cols, int dtype, int block_dtype, int pre, int post, int params_f32, double alpha,
            long long gate_rows, const std::array<uintptr_t, 5>& params, const std::array<uintptr_t, 5>& grads,
            const std::array<uintptr_t, 4>& helds, int pitch, int spitch, int sms, uintptr_t stream) {
           BlockNormArgs a = block_norm_args(rows, cols, pre, post, params_f32, alpha, 0.f, gate_rows, params, stats);
@@ -381,7 +381,7 @@ PYBIND11_MODULE(GRACE_MODULE_NAME, m) {
           a.dx = ptr<void>(dx); a.dblock = ptr<void>(dblock); a.sums = ptr<float>(sums);
           a.pre_weight_grad = ptr<void>(grads[0]); a.pre_bias_grad = ptr<void>(grads[1]); a.post_weight_grad = ptr<void>(grads[2]);
           a.post_bias_grad = ptr<void>(grads[3]); a.gate_grad = ptr<void>(grads[4]);
-          check(launch_block_norm_backward(a, dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_backward");
+          check(launch_block_norm_backward(a, dtype, block_dtype, sms, reinterpret_cast<cudaStream_t>(stream)), "block_norm_backward");
         });
 
   // ---- host engine of the exchange protocol (CPU ranks over POSIX shared memory) ----

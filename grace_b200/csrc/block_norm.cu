@@ -262,8 +262,8 @@ __device__ __forceinline__ void add_scaled(float alpha, float alpha_low, const f
   add_scaled16(v, alpha, x);
 }
 
-// THREADS: 256 where a row takes no more, three CTAs an SM; 512
-template <class T, bool PRE_LAYER, int POST, int THREADS>
+// T: the stream's type, TB: the block's.  THREADS: 256 where a row takes no more, three CTAs an SM; 512
+template <class T, class TB, bool PRE_LAYER, int POST, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_forward_kernel(const BlockNormArgs a, int tpr) {
   __shared__ __align__(16) float buf[kSumFloats];
   extern __shared__ float4 params[];
@@ -274,10 +274,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) block_norm_fo
   const float inv_cols = 1.f / (float)a.cols;
   const Run run = run_of(a);
   RowSum sum(buf, tpr);
-  Chunk16<T> cb, cx;
+  Chunk16<TB> cb;
+  Chunk16<T> cx;
   auto load = [&](long long row) {
     if (row < run.row1) {
-      cb.load(static_cast<const T*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
+      cb.load(static_cast<const TB*>(a.block) + row * a.block_stride, col, a.cols, a.block_vec);
       cx.load(static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols, a.x_vec);
     } else {
       cb.zero();
@@ -415,7 +416,7 @@ __device__ __forceinline__ void decode_normed(uint4 codes, unsigned s, float mea
 // kernel.
 enum BlockUse : int { kNoBlock = 0, kGateOnly = 1, kBlockRms = 2, kBlockLayer = 3 };
 
-template <class T, bool PRE_LAYER, int POST>
+template <class T, class TB, bool PRE_LAYER, int POST>
 __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNormArgs a, int tpr) {
   constexpr bool TWO = POST != kNoBlock, NORM = POST >= kBlockRms, LAYER = POST == kBlockLayer;
   constexpr int B = TWO ? 16 : 1, L = PRE_LAYER ? 16 : 1, Z = LAYER ? 16 : 1;
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(512) block_norm_backward_kernel(const BlockNor
         for (int i = 0; i < 8; ++i) put(f, i, mul2(F2(stats.w), fma2(pair(bh, i), F2(-p1), LAYER ? add2(pair(f, i), F2(-p0)) : pair(f, i))));
       }
     }
-    if (in) store16(f, static_cast<T*>(a.dblock) + row * a.cols, col, a.cols, a.out_vec);
+    if (in) store16(f, static_cast<TB*>(a.dblock) + row * a.cols, col, a.cols, a.dblock_vec);
   }
   if (!a.sums) return;
   // This run's sums: [4][pitch] floats.  The CTA's row lanes are added in order, each on top of the one before it.
@@ -611,10 +612,10 @@ bool params_vec(const BlockNormArgs& a, size_t es) {
   return a.cols % 4 == 0 && all % (4 * (a.params_f32 ? 4 : es)) == 0;
 }
 
-template <class T>
+template <class T, class TB>
 cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   a.x_vec = row_align(a.x, a.x_stride, sizeof(T));
-  a.block_vec = row_align(a.block, a.block_stride, sizeof(T));
+  a.block_vec = row_align(a.block, a.block_stride, sizeof(TB));
   a.params_vec = params_vec(a, sizeof(T));
   a.out_vec = std::min(row_align(a.h, a.cols, sizeof(T)), row_align(a.y, a.cols, sizeof(T)));
   const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, false);
@@ -626,25 +627,25 @@ cudaError_t forward_typed(BlockNormArgs a, int sms, cudaStream_t stream) {
   auto go = [&](auto kernel) { return launch_shared(kernel, grid, block, smem, stream, a, shape.tpr); };
   if (block.x > 256) {
     switch (a.post * 2 + (layer ? 1 : 0)) {
-      case 0: return go(block_norm_forward_kernel<T, false, kNormNone, 512>);
-      case 1: return go(block_norm_forward_kernel<T, true, kNormNone, 512>);
-      case 2: return go(block_norm_forward_kernel<T, false, kNormRms, 512>);
-      case 3: return go(block_norm_forward_kernel<T, true, kNormRms, 512>);
-      case 4: return go(block_norm_forward_kernel<T, false, kNormLayer, 512>);
-      default: return go(block_norm_forward_kernel<T, true, kNormLayer, 512>);
+      case 0: return go(block_norm_forward_kernel<T, TB, false, kNormNone, 512>);
+      case 1: return go(block_norm_forward_kernel<T, TB, true, kNormNone, 512>);
+      case 2: return go(block_norm_forward_kernel<T, TB, false, kNormRms, 512>);
+      case 3: return go(block_norm_forward_kernel<T, TB, true, kNormRms, 512>);
+      case 4: return go(block_norm_forward_kernel<T, TB, false, kNormLayer, 512>);
+      default: return go(block_norm_forward_kernel<T, TB, true, kNormLayer, 512>);
     }
   }
   switch (a.post * 2 + (layer ? 1 : 0)) {
-    case 0: return go(block_norm_forward_kernel<T, false, kNormNone, 256>);
-    case 1: return go(block_norm_forward_kernel<T, true, kNormNone, 256>);
-    case 2: return go(block_norm_forward_kernel<T, false, kNormRms, 256>);
-    case 3: return go(block_norm_forward_kernel<T, true, kNormRms, 256>);
-    case 4: return go(block_norm_forward_kernel<T, false, kNormLayer, 256>);
-    default: return go(block_norm_forward_kernel<T, true, kNormLayer, 256>);
+    case 0: return go(block_norm_forward_kernel<T, TB, false, kNormNone, 256>);
+    case 1: return go(block_norm_forward_kernel<T, TB, true, kNormNone, 256>);
+    case 2: return go(block_norm_forward_kernel<T, TB, false, kNormRms, 256>);
+    case 3: return go(block_norm_forward_kernel<T, TB, true, kNormRms, 256>);
+    case 4: return go(block_norm_forward_kernel<T, TB, false, kNormLayer, 256>);
+    default: return go(block_norm_forward_kernel<T, TB, true, kNormLayer, 256>);
   }
 }
 
-template <class T>
+template <class T, class TB>
 cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape, cudaStream_t stream) {
   const dim3 block(shape.tpr * shape.rpb), grid(shape.runs);
   const int use = a.held_b.codes == nullptr ? kNoBlock : (a.post == kNormNone ? kGateOnly : (a.post == kNormRms ? kBlockRms : kBlockLayer));
@@ -656,25 +657,26 @@ cudaError_t backward_launch(const BlockNormArgs& a, const BlockNormShape& shape,
   const size_t smem = (size_t)rows * a.held_y.pitch * 4;
   auto go = [&](auto kernel) { return launch_shared(kernel, grid, block, smem, stream, a, shape.tpr); };
   switch (use * 2 + (layer ? 1 : 0)) {
-    case 0: return go(block_norm_backward_kernel<T, false, kNoBlock>);
-    case 1: return go(block_norm_backward_kernel<T, true, kNoBlock>);
-    case 2: return go(block_norm_backward_kernel<T, false, kGateOnly>);
-    case 3: return go(block_norm_backward_kernel<T, true, kGateOnly>);
-    case 4: return go(block_norm_backward_kernel<T, false, kBlockRms>);
-    case 5: return go(block_norm_backward_kernel<T, true, kBlockRms>);
-    case 6: return go(block_norm_backward_kernel<T, false, kBlockLayer>);
-    default: return go(block_norm_backward_kernel<T, true, kBlockLayer>);
+    case 0: return go(block_norm_backward_kernel<T, TB, false, kNoBlock>);
+    case 1: return go(block_norm_backward_kernel<T, TB, true, kNoBlock>);
+    case 2: return go(block_norm_backward_kernel<T, TB, false, kGateOnly>);
+    case 3: return go(block_norm_backward_kernel<T, TB, true, kGateOnly>);
+    case 4: return go(block_norm_backward_kernel<T, TB, false, kBlockRms>);
+    case 5: return go(block_norm_backward_kernel<T, TB, true, kBlockRms>);
+    case 6: return go(block_norm_backward_kernel<T, TB, false, kBlockLayer>);
+    default: return go(block_norm_backward_kernel<T, TB, true, kBlockLayer>);
   }
 }
 
-template <class T>
+template <class T, class TB>
 cudaError_t backward_typed(BlockNormArgs a, const BlockNormShape& shape, int sms, cudaStream_t stream) {
   a.grad_h_vec = row_align(a.grad_h, a.grad_h_stride, sizeof(T));
   a.grad_y_vec = row_align(a.grad_y, a.grad_y_stride, sizeof(T));
   a.params_vec = params_vec(a, sizeof(T));
-  a.out_vec = std::min(row_align(a.dblock, a.cols, sizeof(T)), row_align(a.dx, a.cols, sizeof(T)));
+  a.out_vec = row_align(a.dx, a.cols, sizeof(T));
+  a.dblock_vec = row_align(a.dblock, a.cols, sizeof(TB));
   a.parts = shape.parts;
-  const cudaError_t err = backward_launch<T>(a, shape, stream);
+  const cudaError_t err = backward_launch<T, TB>(a, shape, stream);
   const bool params = a.pre_weight_grad || a.pre_bias_grad || a.post_weight_grad || a.post_bias_grad || a.gate_grad;
   if (err != cudaSuccess || !a.sums || !params) return err;
   cudaLaunchConfig_t cfg{};     // (set up while the first kernel still runs; it waits for that one's end before it reads)
@@ -709,28 +711,40 @@ BlockNormShape block_norm_shape(long long rows, int cols, long long gate_rows, i
   return s;
 }
 
-cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
-  if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
-  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
-  switch (dtype) {
-    case kGradF32: return forward_typed<float>(a, sms, stream);
-    case kGradBF16: return forward_typed<__nv_bfloat16>(a, sms, stream);
-    case kGradF16: return forward_typed<__half>(a, sms, stream);
+namespace {
+
+// f(the stream's type, the block's)
+template <class F>
+cudaError_t by_types(int dtype, int block_dtype, F f) {
+  if (dtype == kGradF32) {
+    switch (block_dtype) {
+      case kGradF32: return f(float{}, float{});
+      case kGradBF16: return f(float{}, __nv_bfloat16{});
+      case kGradF16: return f(float{}, __half{});
+    }
+  } else if (dtype == block_dtype) {
+    switch (dtype) {
+      case kGradBF16: return f(__nv_bfloat16{}, __nv_bfloat16{});
+      case kGradF16: return f(__half{}, __half{});
+    }
   }
   return cudaErrorInvalidValue;
 }
 
-cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int sms, cudaStream_t stream) {
+}  // namespace
+
+cudaError_t launch_block_norm_forward(const BlockNormArgs& a, int dtype, int block_dtype, int sms, cudaStream_t stream) {
+  if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
+  if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
+  return by_types(dtype, block_dtype, [&](auto t, auto b) { return forward_typed<decltype(t), decltype(b)>(a, sms, stream); });
+}
+
+cudaError_t launch_block_norm_backward(const BlockNormArgs& a, int dtype, int block_dtype, int sms, cudaStream_t stream) {
   if (a.rows <= 0 || a.cols <= 0) return cudaSuccess;
   if (a.cols > kBlockNormMaxCols || a.rows > 0x7fffffffll) return cudaErrorInvalidValue;
   const BlockNormShape shape = block_norm_shape(a.rows, a.cols, a.gate_rows, sms, true);
   if (shape.sequences > 65531) return cudaErrorInvalidValue;
-  switch (dtype) {
-    case kGradF32: return backward_typed<float>(a, shape, sms, stream);
-    case kGradBF16: return backward_typed<__nv_bfloat16>(a, shape, sms, stream);
-    case kGradF16: return backward_typed<__half>(a, shape, sms, stream);
-  }
-  return cudaErrorInvalidValue;
+  return by_types(dtype, block_dtype, [&](auto t, auto b) { return backward_typed<decltype(t), decltype(b)>(a, shape, sms, stream); });
 }
 
 }  // namespace grace

@@ -36,11 +36,12 @@ class Saved:
     """What the backward pass takes from the forward pass: one allocation with the checkpoints and the statistics, the parameters, and the
     forms of the norms."""
 
-    __slots__ = ("data", "shape", "dtype", "rows", "pitch", "spitch", "two", "params", "pre", "post", "residual_scale", "return_stream", "held_h")
+    __slots__ = ("data", "shape", "dtype", "block_dtype", "rows", "pitch", "spitch", "two", "params", "pre", "post", "residual_scale", "return_stream", "held_h")
 
     def __init__(self, data: Optional[torch.Tensor], shape, dtype, device, params, pre, post, residual_scale, return_stream, held_h=None,
-                 keep=True):
+                 keep=True, block_dtype=None):
         self.shape, self.dtype, self.rows = shape, dtype, math.prod(shape[:-1])
+        self.block_dtype = block_dtype or dtype
         self.pitch, self.spitch = pitch_of(shape[-1])
         self.two = post is not None or params[4] is not None       # a checkpoint of block too
         self.params, self.pre, self.post = params, pre, post
@@ -66,7 +67,7 @@ class Saved:
 
     @property
     def held_block(self) -> Optional[Act8]:
-        return Act8._over(self.data, self._held(), self.shape, self.dtype) if self.two else None
+        return Act8._over(self.data, self._held(), self.shape, self.block_dtype) if self.two else None
 
     @property
     def stats(self) -> torch.Tensor:
@@ -74,12 +75,12 @@ class Saved:
         return self.data[self._stats_at() :].view(torch.float32).view(-1, 4)
 
 
-def _check(x, block, pre, post, params, residual_scale, eps) -> int:
-    """Rows of a sequence (0: the gate, if any, is the same for all rows)."""
+def _check(x, block, pre, post, params, residual_scale, eps, mixed) -> int:
+    """Rows of a sequence (0: the gate, if any, is the same for all rows).  ``mixed``: ``block`` may be of 16 bits beside ``x`` in fp32."""
     _check_tensor(x, "residual_norm: x")
     _check_tensor(block, "residual_norm: block")
     shape, dtype, device = x.shape, x.dtype, x.device
-    if shape != block.shape or dtype != block.dtype or device != block.device:
+    if shape != block.shape or (dtype != block.dtype and not (mixed and dtype == torch.float32)) or device != block.device:
         raise ValueError("residual_norm: x %s %s on %s and block %s %s on %s have to be alike"
                          % (tuple(shape), dtype, device, tuple(block.shape), block.dtype, block.device))
     if pre not in ("rms", "layer") or post not in NORMS:
@@ -130,12 +131,17 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     """``(h, y, saved)`` (``y`` None without ``return_stream``); with ``checkpoint_output`` ``saved.held_h`` is what ``act8.pack(h)`` gives.  With
     ``checkpoint=False``, where no backward pass follows, ``saved`` holds nothing else.  A row of which the squares' sum passes fp32's
     range has no deviation: NaN on the GPU."""
-    params = (pre_weight, pre_bias, post_weight, post_bias, gate)
-    gate_rows = _check(x, block, pre, post, params, residual_scale, eps)
+    return _forward(x, block, pre, post, (pre_weight, pre_bias, post_weight, post_bias, gate), residual_scale, eps, return_stream,
+                    checkpoint_output, checkpoint, False)
+
+
+def _forward(x, block, pre, post, params, residual_scale, eps, return_stream, checkpoint_output, checkpoint, mixed):
+    gate_rows = _check(x, block, pre, post, params, residual_scale, eps, mixed)
     shape, dtype, device = x.shape, x.dtype, x.device
     cols, rows = shape[-1], math.prod(shape[:-1])
     held_h = empty_like(shape, dtype, device) if checkpoint_output else None
-    saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h, checkpoint)
+    saved = Saved(None, shape, dtype, device, params, pre, post, float(residual_scale), return_stream, held_h, checkpoint,
+                  block.dtype)
     if not x.is_cuda:
         return _forward_cpu(x, block, saved, float(eps)) + (saved,)
     h = _new_like(x)
@@ -145,7 +151,7 @@ def residual_norm_forward(x: torch.Tensor, block: torch.Tensor, *, pre: str = "l
     ptrs, kept = _param_ptrs(params)
     *held, stats = saved.ptrs() if checkpoint else (0,) * 5
     _launch(device, native().block_norm_forward, x_at, x_stride, b_at, b_stride, h.data_ptr(), 0 if y is None else y.data_ptr(), stats, rows,
-            cols, GRAD_DTYPE[dtype], NORMS[pre], NORMS[post], _f32(params), float(residual_scale), float(eps), gate_rows, ptrs,
+            cols, GRAD_DTYPE[dtype], GRAD_DTYPE[block.dtype], NORMS[pre], NORMS[post], _f32(params), float(residual_scale), float(eps), gate_rows, ptrs,
             (*held, *_ptrs(held_h)), saved.pitch, saved.spitch, _sms(device))
     del kept
     return h, y, saved
@@ -179,9 +185,9 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
         return _backward_cpu(grad_h, grad_y, saved, want)
     if rows == 0 or cols == 0:
         empty = torch.empty(shape, dtype=dtype, device=device)
-        return dict(zip(("x", "block") + PARAMS, [empty, empty] + [torch.zeros_like(p) if w else None for p, w in zip(params, want)]))
-    one = not saved.two and saved.residual_scale == 1.0
-    block = _new_like(grad_h)
+        return dict(zip(("x", "block") + PARAMS, [empty, empty.to(saved.block_dtype)] + [torch.zeros_like(p) if w else None for p, w in zip(params, want)]))
+    one = not saved.two and saved.residual_scale == 1.0 and saved.block_dtype == dtype
+    block = _new_like(grad_h) if saved.block_dtype == dtype else torch.empty(shape, dtype=saved.block_dtype, device=device)
     dx = None if one else _new_like(grad_h)
     grads = [(torch.empty_like(p) if p.is_contiguous() else torch.empty(p.shape, dtype=p.dtype, device=device)) if w else None
              for p, w in zip(params, want)]
@@ -193,8 +199,8 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     *held, stats = saved.ptrs()
     sums = torch.empty(C.block_norm_sum_rows(rows, cols, gate_rows, sms) * 4 * saved.pitch, dtype=torch.float32, device=device) if any(want) else None
     _launch(device, C.block_norm_backward, g_at, g_stride, gy_at, gy_stride, 0 if dx is None else dx.data_ptr(), block.data_ptr(), stats,
-            0 if sums is None else sums.data_ptr(), rows, cols, GRAD_DTYPE[dtype], NORMS[saved.pre], NORMS[saved.post], _f32(params),
-            saved.residual_scale, gate_rows, ptrs, [0 if t is None else t.data_ptr() for t in grads], held, saved.pitch, saved.spitch, sms)
+            0 if sums is None else sums.data_ptr(), rows, cols, GRAD_DTYPE[dtype], GRAD_DTYPE[saved.block_dtype],
+            NORMS[saved.pre], NORMS[saved.post], _f32(params), saved.residual_scale, gate_rows, ptrs, [0 if t is None else t.data_ptr() for t in grads], held, saved.pitch, saved.spitch, sms)
     del kept
     got = dict(zip(PARAMS, grads))
     got["x"], got["block"] = block if dx is None else dx, block
@@ -264,7 +270,7 @@ def _backward_cpu(grad_h, grad_y, saved: Saved, want):
             got["post_weight"], got["post_bias"] = (e * bh).sum(leading), e.sum(leading)
             e = _norm_grad_cpu(e * _wide(post_w, shape, 1.0), bh, rb, saved.post)
     got = {k: got[k].to(p.dtype) if w else None for k, p, w in zip(PARAMS, saved.params, want)}
-    got["x"], got["block"] = (saved.residual_scale * g).to(dtype), e.to(dtype)
+    got["x"], got["block"] = (saved.residual_scale * g).to(dtype), e.to(saved.block_dtype)
     return got
 
 
@@ -272,29 +278,28 @@ def _backward_cpu(grad_h, grad_y, saved: Saved, want):
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, residual_scale, eps, return_stream,
-                checkpoint_output, box):
+                checkpoint_output, mixed, box):
         ctx.set_materialize_grads(False)
-        h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
-                                            post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps,
-                                            return_stream=return_stream, checkpoint_output=checkpoint_output)
+        h, y, saved = _forward(x, block, pre, post, (pre_weight, pre_bias, post_weight, post_bias, gate), residual_scale, eps, return_stream,
+                               checkpoint_output, True, mixed)
         box.append(saved.held_h)
         ctx.save_for_backward(*saved.params, saved.data)
-        ctx.kinds, ctx.shape, ctx.dtype = (pre, post, saved.residual_scale, return_stream), x.shape, x.dtype
+        ctx.kinds, ctx.shape, ctx.dtype, ctx.block_dtype = (pre, post, saved.residual_scale, return_stream), x.shape, x.dtype, block.dtype
         return (h, y) if return_stream else h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_h, grad_y=None):
         t = ctx.saved_tensors
-        saved = Saved(t[5], ctx.shape, ctx.dtype, t[5].device, tuple(t[:5]), *ctx.kinds)
+        saved = Saved(t[5], ctx.shape, ctx.dtype, t[5].device, tuple(t[:5]), *ctx.kinds, block_dtype=ctx.block_dtype)
         if not saved.return_stream:
             grad_y = None
         if grad_h is None and grad_y is None:
-            return (None,) * 14
+            return (None,) * 15
         if grad_h is None:
             grad_h = torch.zeros(ctx.shape, dtype=ctx.dtype, device=t[5].device)
         got = residual_norm_backward(grad_h, grad_y, saved, ctx.needs_input_grad[2:7])
-        return (got["x"], got["block"]) + tuple(got[k] for k in PARAMS) + (None,) * 7
+        return (got["x"], got["block"]) + tuple(got[k] for k in PARAMS) + (None,) * 8
 
 
 def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", pre_weight: Optional[torch.Tensor] = None,
@@ -302,23 +307,25 @@ def residual_norm(x: torch.Tensor, block: torch.Tensor, *, pre: str = "layer", p
                   post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
                   eps: float = 1e-5, return_stream: bool = True, checkpoint_output: bool = False):
     """``residual_norm_forward`` with autograd: ``h``, then ``y`` with ``return_stream``, then the ``Act8`` of ``h`` with ``checkpoint_output``; one of them
-    alone comes as it is, several as a tuple.  Under autocast ``x`` and ``block`` are taken, and results returned, in the wider of their two
-    types, as a sum of them has it: a stream in fp32 stays in fp32 where the blocks compute in 16 bits."""
-    if _autocast_type(x) is not None:
+    alone comes as it is, several as a tuple.  Under autocast ``x`` and results are of the wider type of ``x`` and ``block``, as their sum
+    is: a stream in fp32 stays in fp32 where the blocks compute in 16 bits."""
+    mixed = _autocast_type(x) is not None
+    if mixed:
         t = torch.promote_types(x.dtype, block.dtype)
         t = t if t in GRAD_DTYPE else torch.float32
-        x, block = x.to(t), block.to(t)
+        x = x.to(t)
+        if block.dtype != t and block.dtype not in GRAD_DTYPE:
+            block = block.to(t)
         pre_weight, pre_bias, post_weight, post_bias, gate = (
             p if p is None or p.dtype in (t, torch.float32) else p.to(t) for p in (pre_weight, pre_bias, post_weight, post_bias, gate))
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, pre_weight, pre_bias, post_weight, post_bias, gate))):
-        h, y, saved = residual_norm_forward(x, block, pre=pre, pre_weight=pre_weight, pre_bias=pre_bias, post=post, post_weight=post_weight,
-                                            post_bias=post_bias, gate=gate, residual_scale=residual_scale, eps=eps, return_stream=return_stream,
-                                            checkpoint_output=checkpoint_output, checkpoint=False)
+        h, y, saved = _forward(x, block, pre, post, (pre_weight, pre_bias, post_weight, post_bias, gate), residual_scale, eps, return_stream,
+                               checkpoint_output, False, mixed)
         out = (h,) + ((y,) if return_stream else ()) + ((saved.held_h,) if checkpoint_output else ())
         return out[0] if len(out) == 1 else out
     box = []
     out = _ResidualNorm.apply(x, block, pre_weight, pre_bias, post_weight, post_bias, gate, pre, post, float(residual_scale), float(eps),
-                              return_stream, checkpoint_output, box)
+                              return_stream, checkpoint_output, mixed, box)
     if not checkpoint_output:
         return out
     return (out if return_stream else (out,)) + (box[0],)

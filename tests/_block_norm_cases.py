@@ -3,6 +3,7 @@ import torch
 
 from _act8_oracle import block_norm_gradients, close, half_step, held_value, norm_stats, normed, stream
 from grace_b200.ops import act8, block_norm
+from grace_b200.ops.block_norm import PARAMS
 
 #: fp32 arithmetic relative to the size of the terms: a row's sums (a tree over up to 8192 values: 13 levels and 8 in order, 2^-24 each), the
 #: reciprocal root and the products, about 40 roundings in all
@@ -78,3 +79,30 @@ def check(d, p, alpha=1.0, eps=1e-5, with_stream=True):
         rel = 2 * REL if name in ("x", "block") else 2 * REL + rows * 2.0 ** -24
         close(out, w, own * w.abs() + rel * size + (2.0 ** -25 if out.dtype == torch.float16 else 0.0), name)
     return h, y, got
+
+
+def check_mixed(shape, kind, pre, post, gate, alpha, with_stream, device):
+    """A block in 16 bits beside a stream in fp32, under autocast: to the bit what the block gives in fp32, its gradient rounded once."""
+    d, p = make(shape, torch.float32, pre, post, gate, seed=27, device=device)
+    block = d["block"].to(kind)
+    q = dict(p, residual_scale=alpha, return_stream=with_stream, checkpoint_output=True)
+    wanted = [k for k in PARAMS if k in p]
+
+    def run(b, mixed):
+        leaves = [d["x"].clone().requires_grad_(), b.clone().requires_grad_()] + [p[k].clone().requires_grad_() for k in wanted]
+        with torch.autocast(device, dtype=kind, enabled=mixed):
+            out = block_norm.residual_norm(leaves[0], leaves[1], **dict(q, **dict(zip(wanted, leaves[2:]))))
+            with torch.no_grad():
+                again = block_norm.residual_norm(leaves[0], leaves[1], **dict(q, **dict(zip(wanted, leaves[2:]))))
+        assert all(torch.equal(a, b) for a, b in zip(out[:-1], again[:-1])) and torch.equal(out[-1].codes, again[-1].codes)
+        grads = torch.autograd.grad(out[:-1], leaves, (d["dh"], d["dy"])[: len(out) - 1])
+        return out, grads
+
+    got, grads = run(block, True)
+    want, ref = run(block.float(), False)
+    assert len(got) == (3 if with_stream else 2)
+    for a, b in zip(got[:-1], want[:-1]):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
+    assert got[-1].dtype == torch.float32 and torch.equal(got[-1].codes, want[-1].codes)
+    for i, (a, b) in enumerate(zip(grads, ref)):
+        assert a.dtype == (kind if i == 1 else torch.float32) and torch.equal(a, b.to(a.dtype)), i

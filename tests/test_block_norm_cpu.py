@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from _act8_oracle import block_norm_gradients, norm_stats, normed, stream
-from _block_norm_cases import check, make
+from _block_norm_cases import check, check_mixed, make
 from grace_b200.ops import act8, block_norm
 
 
@@ -148,3 +148,9 @@ def test_autocast_keeps_the_stream():
     assert h.dtype == y.dtype == held.dtype == torch.float32 and torch.equal(y, x + b)
     h.sum().backward()
     assert b.grad.dtype == torch.bfloat16 and b.grad.isfinite().all()
+
+
+@pytest.mark.parametrize("pre,post,gate,alpha,with_stream", [
+    ("layer", None, None, 1.0, False), ("rms", "rms", "sequence", 1.0, True), ("layer", "layer", "channel", 0.5, True), ("rms", None, "sequence", 1.0, False)])
+def test_a_block_in_16_bits_beside_an_fp32_stream(pre, post, gate, alpha, with_stream):
+    check_mixed((2, 3, 70), torch.bfloat16, pre, post, gate, alpha, with_stream, "cpu")

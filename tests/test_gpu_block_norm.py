@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _act8_oracle import half_step
-from _block_norm_cases import check, make
+from _block_norm_cases import check, check_mixed, make
 from grace_b200.ops import act8, block_norm
 
 pytestmark = pytest.mark.gpu
@@ -252,3 +252,23 @@ def test_views_that_change_the_sign():
         assert torch.equal(h, h2) and torch.equal(y, y2)
         a, b = block_norm.residual_norm_backward(v, v, saved), block_norm.residual_norm_backward(c, c, saved2)
         assert torch.equal(a["x"], b["x"]) and torch.equal(a["pre_weight"], b["pre_weight"])
+
+
+@pytest.mark.parametrize("kind", [BF16, FP16])
+@pytest.mark.parametrize("pre,post,gate,alpha,with_stream", FORMS)
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 3, 70), (3, 37, 256), (2, 5, 1000), (2, 9, 5001), (1, 3, 8192)])
+def test_a_block_in_16_bits_beside_an_fp32_stream(shape, pre, post, gate, alpha, with_stream, kind):
+    check_mixed(shape, kind, pre, post, gate, alpha, with_stream, "cuda")
+
+
+def test_a_block_in_16_bits_without_rows_and_as_slices():
+    with torch.autocast("cuda", dtype=BF16):
+        x, b = torch.empty(0, 64, device="cuda").requires_grad_(), torch.empty(0, 64, dtype=BF16, device="cuda").requires_grad_()
+        gx, gb = torch.autograd.grad(block_norm.residual_norm(x, b, pre="rms", return_stream=False), (x, b), torch.empty(0, 64, device="cuda"))
+        assert gx.shape == gb.shape == (0, 64) and gx.dtype == FP32 and gb.dtype == BF16
+        wide = torch.randn(6, 130, generator=torch.Generator().manual_seed(28)).to("cuda", BF16)
+        x = torch.randn(6, 96, generator=torch.Generator().manual_seed(29)).cuda()
+        for off in (0, 1, 8, 16):        # rows off their boundaries
+            a = block_norm.residual_norm(x, wide[:, off:off + 96], pre="layer")
+            c = block_norm.residual_norm(x, wide[:, off:off + 96].contiguous(), pre="layer")
+            assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
