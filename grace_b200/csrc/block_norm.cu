@@ -252,11 +252,20 @@ __device__ __forceinline__ void put_codes(const Held& h, long long row, int col,
 // v += alpha x, where alpha is the sum of two fp32 numbers (a caller's 2.63 is none) of which the second is mostly zero.  Where
 // x or the product is infinite the second part says nothing, and of the other sign it would make a NaN of the sum.
 __device__ __forceinline__ void add_scaled(float alpha, float alpha_low, const float (&x)[16], float (&v)[16]) {
+  constexpr float kMax = 3.4028235e38f;
   if (alpha_low != 0.f) {
+    float top = max_abs(x[0], x[1], x[2]);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float low = alpha_low * x[j];
-      v[j] += fabsf(low) <= 3.4028235e38f ? low : 0.f;      // (a NaN comes with the other part)
+    for (int j = 3; j < 15; j += 2) top = max_abs(top, x[j], x[j + 1]);
+    top = max_abs(top, x[15], 0.f);
+    if (fabsf(alpha_low) * top <= kMax) {      // (not where one of them is a NaN)
+      add_scaled16(v, alpha_low, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float low = alpha_low * x[j];
+        v[j] += fabsf(low) <= kMax ? low : 0.f;      // (a NaN comes with the other part)
+      }
     }
   }
   add_scaled16(v, alpha, x);
