@@ -252,10 +252,11 @@ def _backward_cpu(grad_h, grad_y, saved: Saved, want):
     pre_w, _, post_w, post_b, gate = saved.params
     m, r, mb, rb = (t.reshape(shape[:-1] + (1,)) for t in saved.stats.unbind(-1))
     leading = tuple(range(len(shape) - 1))
+    over = lambda t, axes: t.sum(axes) if axes else t  # noqa: E731  (no axes would mean all of them)
     got = dict.fromkeys(PARAMS)
     dh = grad_h.detach().float()
     hat = (_decode_cpu(saved.held_y) - m) * r
-    got["pre_weight"], got["pre_bias"] = (dh * hat).sum(leading), dh.sum(leading)
+    got["pre_weight"], got["pre_bias"] = over(dh * hat, leading), over(dh, leading)
     g = _norm_grad_cpu(dh * _wide(pre_w, shape, 1.0), hat, r, saved.pre)
     if grad_y is not None:
         g = g + grad_y.detach().float()
@@ -265,9 +266,9 @@ def _backward_cpu(grad_h, grad_y, saved: Saved, want):
         bh = b if saved.post is None else (b - mb) * rb
         if gate is not None:
             n = bh * _wide(post_w, shape, 1.0) + _wide(post_b, shape, 0.0)
-            got["gate"] = (g * n).sum(leading if gate.dim() == 1 else leading[1:])
+            got["gate"] = over(g * n, leading if gate.dim() == 1 else leading[1:])
         if saved.post is not None:
-            got["post_weight"], got["post_bias"] = (e * bh).sum(leading), e.sum(leading)
+            got["post_weight"], got["post_bias"] = over(e * bh, leading), over(e, leading)
             e = _norm_grad_cpu(e * _wide(post_w, shape, 1.0), bh, rb, saved.post)
     got = {k: got[k].to(p.dtype) if w else None for k, p, w in zip(PARAMS, saved.params, want)}
     got["x"], got["block"] = (saved.residual_scale * g).to(dtype), e.to(saved.block_dtype)

@@ -106,3 +106,20 @@ def check_mixed(shape, kind, pre, post, gate, alpha, with_stream, device):
     assert got[-1].dtype == torch.float32 and torch.equal(got[-1].codes, want[-1].codes)
     for i, (a, b) in enumerate(zip(grads, ref)):
         assert a.dtype == (kind if i == 1 else torch.float32) and torch.equal(a, b.to(a.dtype)), i
+
+
+def check_one_row(device):
+    """A row without leading axes gives what it gives as the one row of a matrix."""
+    for pre, post, gate in (("layer", None, None), ("rms", "layer", "channel"), ("layer", "rms", "channel")):
+        d, p = make((1, 72), torch.float32, pre, post, gate, seed=30, device=device)
+        want = block_norm.residual_norm_forward(d["x"], d["block"], **p)
+        got = block_norm.residual_norm_forward(d["x"][0], d["block"][0], **p)
+        assert torch.equal(got[0], want[0][0]) and torch.equal(got[1], want[1][0])
+        want = block_norm.residual_norm_backward(d["dh"], d["dy"], want[2])
+        got = block_norm.residual_norm_backward(d["dh"][0], d["dy"][0], got[2])
+        for k, v in want.items():
+            assert (got[k] is None) == (v is None) and (v is None or torch.equal(got[k], v[0] if k in ("x", "block") else v)), k
+        leaves = [d["x"][0].requires_grad_(), d["block"][0].requires_grad_(), p["pre_weight"].requires_grad_()]
+        h, y = block_norm.residual_norm(*leaves[:2], **p)
+        grads = torch.autograd.grad((h, y), leaves, (d["dh"][0], d["dy"][0]))
+        assert all(torch.equal(a, b) for a, b in zip(grads, (got["x"], got["block"], got["pre_weight"])))

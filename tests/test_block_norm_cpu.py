@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from _act8_oracle import block_norm_gradients, norm_stats, normed, stream
-from _block_norm_cases import check, check_mixed, make
+from _block_norm_cases import check, check_mixed, check_one_row, make
 from grace_b200.ops import act8, block_norm
 
 
@@ -154,3 +154,7 @@ def test_autocast_keeps_the_stream():
     ("layer", None, None, 1.0, False), ("rms", "rms", "sequence", 1.0, True), ("layer", "layer", "channel", 0.5, True), ("rms", None, "sequence", 1.0, False)])
 def test_a_block_in_16_bits_beside_an_fp32_stream(pre, post, gate, alpha, with_stream):
     check_mixed((2, 3, 70), torch.bfloat16, pre, post, gate, alpha, with_stream, "cpu")
+
+
+def test_one_row_without_leading_axes():
+    check_one_row("cpu")

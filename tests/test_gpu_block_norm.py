@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _act8_oracle import half_step
-from _block_norm_cases import check, check_mixed, make
+from _block_norm_cases import check, check_mixed, check_one_row, make
 from grace_b200.ops import act8, block_norm
 
 pytestmark = pytest.mark.gpu
@@ -272,3 +272,7 @@ def test_a_block_in_16_bits_without_rows_and_as_slices():
             a = block_norm.residual_norm(x, wide[:, off:off + 96], pre="layer")
             c = block_norm.residual_norm(x, wide[:, off:off + 96].contiguous(), pre="layer")
             assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+def test_one_row_without_leading_axes():
+    check_one_row("cuda")
