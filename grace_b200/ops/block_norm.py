@@ -181,7 +181,7 @@ def residual_norm_backward(grad_h: torch.Tensor, grad_y: Optional[torch.Tensor],
     gate = params[4]
     want = [p is not None and n for p, n in zip(params, needs)]
     cols, rows = shape[-1], math.prod(shape[:-1])
-    if device.type != "cuda":
+    if device.type != "cuda" and rows and cols:
         return _backward_cpu(grad_h, grad_y, saved, want)
     if rows == 0 or cols == 0:
         empty = torch.empty(shape, dtype=dtype, device=device)
@@ -223,6 +223,8 @@ def _stats_cpu(v, kind, eps):
 
 
 def _forward_cpu(x, block, saved: Saved, eps: float):
+    if x.numel() == 0:
+        return torch.empty_like(x), torch.empty_like(x) if saved.return_stream else None
     pre_w, pre_b, post_w, post_b, gate = saved.params
     b = block.detach().float()
     mb, rb = _stats_cpu(b, saved.post, eps)

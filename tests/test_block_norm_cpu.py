@@ -158,3 +158,14 @@ def test_a_block_in_16_bits_beside_an_fp32_stream(pre, post, gate, alpha, with_s
 
 def test_one_row_without_leading_axes():
     check_one_row("cpu")
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (2, 0, 32), (3, 0), (0,)])
+def test_empty(shape):
+    x, w = torch.empty(shape).requires_grad_(), torch.ones(shape[-1]).requires_grad_()
+    h, y, held = block_norm.residual_norm(x, x.detach(), pre="layer", pre_weight=w, pre_bias=w, checkpoint_output=True)
+    assert h.shape == y.shape == held.shape == shape
+    (h.sum() + y.sum()).backward()
+    assert x.grad.shape == shape and w.grad.shape == w.shape and not w.grad.any()
+    with torch.no_grad():
+        assert block_norm.residual_norm(x, x, pre="rms", return_stream=False).shape == shape
