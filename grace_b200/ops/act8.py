@@ -435,6 +435,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if not (torch.is_grad_enabled() and weight.requires_grad):
         return F.linear(x, weight, bias)       # nothing reads x again
     _check_tensor(x, "act8.linear")
+    if weight.dim() != 2:      # (the library's layer takes a vector too; its gradient is no product of matrices)
+        raise ValueError("act8.linear: a weight of [outs, ins], not %s" % (tuple(weight.shape),))
     if x.is_cuda and x.dtype == torch.float32:
         raise TypeError("act8.linear: bf16 or fp16 on the GPU (or fp32 under autocast): the weight gradient runs on the tensor cores")
     if checkpoint is None:

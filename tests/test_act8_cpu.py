@@ -216,3 +216,9 @@ def check_fp16_operand(dtype, device):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_weight_grad_with_an_fp16_gradient_of_another_types_checkpoint(dtype):
     check_fp16_operand(dtype, "cpu")
+
+
+def test_linear_refuses_a_vector_for_its_weight():
+    """Before the forward pass, not in the backward pass."""
+    with pytest.raises(ValueError, match="outs, ins"):
+        act8.linear(rand(4, 64), rand(64).requires_grad_())
