@@ -7,16 +7,20 @@
 //             gated: x = [a | b], y = f(a) b, checkpoints of a and b      3 es + 2 1/16 (+ 1 1/32), for an element of y
 //   backward  dx = dy f'(x~);  gated: da = dy b~ f'(a~), db = dy f(a~)    2 es + 1 1/32;  3 es + 2 1/16
 //
-// All four are bound by memory, the GELU forward pass with both checkpoints by its issue slots: a thread takes a chunk of
-// sixteen neighbouring elements (32 bytes of a 16-bit type in, 16 bytes of codes out; with eight, half of both, pack took a
+// All four are bound by memory where rows start on 16-byte boundaries (others: below), the GELU forward pass with both
+// checkpoints by its issue slots: a thread takes a chunk of sixteen neighbouring elements (32 bytes of a 16-bit type in, 16 bytes of codes out; with eight, half of both, pack took a
 // fifth longer), two lanes share a group of 32 and agree on its largest magnitude by one shuffle.  What hides the latency is
 // the number of threads: with two chunks each, all loads first, the gated backward pass took 89 us for 77, the others as
 // long as with one.  At 6.5 TB/s an SM has about 16 issue slots an element of a bf16 pack and 25 of a forward pass, so
 // arithmetic is on pairs of numbers, the encoder clamps only where a group needs it (together 34.6 -> 29.2 us for
 // pack), and the functions take one exponential and one reciprocal.
 // Measured, bf16 16384 x 4096 (L2 cold): pack 29.2 us, 7.0 TB/s; unpack 28.8 us, 7.1 TB/s; gated SiLU forward 78 us, 6.9
-// TB/s, and backward 77 us, 7.0 TB/s; 4096 x 4096 GELU forward with both checkpoints 19.8 us, 5.1 TB/s, backward 16.1 us,
-// 5.3 TB/s.  (Above the copy rate of 6.5 where the last writes are still in L2.)
+// TB/s, and backward 77 us, 7.0 TB/s; 4096 x 4096 GELU forward with both checkpoints 19.9 us, 5.1 TB/s, backward 16.4 us,
+// 5.2 TB/s.  (Above the copy rate of 6.5 where the last writes are still in L2.)  fp32 16384 x 4096, with the launch: pack 57,
+// unpack 55, GELU forward 170 and backward 270 us (CUDA's erfc).
+// Rows off 16-byte boundaries (a width that is no multiple of 8 of a 16-bit type, a slice that starts between) are read and
+// written by single elements, 32 bytes apart from lane to lane: 16384 x 4095 against x 4096, with the launch, pack 74 and 37 us,
+// unpack 371 and 35, gated forward 371 and 85, gated backward 766 and 86.
 //
 // f is GELU (erf form), GELU (tanh form) or SiLU.  For 16-bit tensors the exponential and the reciprocal are the hardware's,
 // and the normal distribution function of the erf form is, for x <= 0,

@@ -3,7 +3,9 @@
 // A row is cut into groups of 32 neighbouring elements.  With E the biased fp32 exponent of the group's largest
 // magnitude, the group's scale byte is s = clamp(E, 7, 252) - 6 and stands for 2^(s - 127) (E8M0); an element x is
 // held as the int8 code  q = rint(x * 2^(127 - s))  (ties to even), kept within [-127, 127], and reads back as
-// q * 2^(s - 127).  This is the MXINT8 format of the OCP Microscaling Formats specification 1.0.  Scaling by a power
+// q * 2^(s - 127).  The codes are those of MXINT8 of the OCP Microscaling Formats specification 1.0; the scale byte is that
+// format's less 6, since its elements carry an implied factor of 2^-6 that is part of the scale here (who reads these bytes as
+// MXINT8 gets values 64 times too small).  Scaling by a power
 // of two is exact, so the only rounding is the one to an integer, and 7 bits of magnitude fit bf16's significand: a
 // held value is exact in fp32 and in bf16 (in fp16 too unless it is subnormal there).  The largest error is half a
 // code step, 2^-7 of the group's leading power of two (one step, 2^-6, within the last 1/128 below the next power).

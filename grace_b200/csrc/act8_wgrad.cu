@@ -30,12 +30,16 @@
 // the output instead, that cost 40 % more traffic through L2 and as much time.  What is left of the bias (some 1e-6) does not
 // grow any more.  Sums are fp32 throughout, rounded once to the output's type.
 //
-// What bounds it: shared memory. A step moves 96 KB in and out of an SM's (dY and codes in, codes out and operand in for the
-// decoders, both operands out for the product), 750 cycles at its 128 bytes a cycle, where the product itself takes 512; a
-// step takes 800 to 860.  Measured with cold caches: 16384 tokens, 4096 x 4096, bf16 400 us (1373 TFLOP/s, 0.86 of
-// the measured library rate; the library's product of two bf16 matrices takes 335), fp32 result 454 us; 4096 tokens, 4096 x
-// 1024 fp32 50 us (64 tiles for 74 pairs; library 29), 1024 x 1024 with its bias 27 us (library 14), a third of it the
-// second kernel.
+// What bounds it: in a large product, shared memory. A step moves 96 KB in and out of an SM's (dY and codes in, codes out and
+// operand in for the decoders, both operands out for the product), 750 cycles at its 128 bytes a cycle, where the product
+// itself takes 512; a step takes 800 to 860, and emptying the accumulator, when the products stop, 8 % on top of that.  Measured
+// with cold caches: 16384 tokens, 4096 x 4096, bf16 430 us (1279 TFLOP/s, 0.80 of the measured library rate; the library's product
+// of two bf16 matrices takes 336), fp16 470, fp32 result 453 us.  A call of less than a wave of tiles takes longer a step: 4096
+// tokens, 4096 x 1024, fp32 result 50 us, 1500 cycles for each of its 64 steps (64 tiles for 74 pairs, library 31); the
+// accumulator is emptied three times in them, which explains a part of it, and the rest has not been found.  1024 x 1024 with its
+// bias 19 + 9 us (library 16): runs of 14 steps, and a second kernel for their sums.  One warp adds up the bias columns: free where
+// many tiles along the inputs share them, not where few do (16384 tokens, 4096 outputs, without and with it: 128 inputs 45 and 77
+// us, 512 inputs 71 and 98, 1024 inputs 128 and 147, 4096 inputs 430 and 439).
 //
 // Every wait is bounded; when one runs out the status block says which and the outputs are NaN.
 #include <type_traits>
@@ -738,8 +742,10 @@ Plan make_plan(long long tokens, int outs, int ins, bool out_f32, int sms) {
   p.pairs = sms / 2;
   p.whole = p.tiles / p.pairs;
   p.rest = p.tiles % p.pairs;
-  // The last wave's tiles are shared out where that saves more steps than the second kernel and the partial sums cost,
-  // at least four steps for each pair.
+  // The last wave's tiles are shared out where that saves more steps than the second kernel and the partial sums cost, at least
+  // four steps for each pair: 24 steps, or any where the results' rows are off 16-byte boundaries, since whole tiles then go out
+  // by single elements and shared ones through the second kernel in fours (fp16, us with 1 and with 24: 777 tokens 1000 x 1003 19.6
+  // and 26.6; 1024 tokens 768 x 771 18.4 and 26.6; 2048 tokens 2000 x 2002 38.9 and 36.9; 4096 tokens 1000 x 1001 26.6 and 25.8).
   p.rest_pairs = p.rest;
   if (p.rest) {
     const long long total = (long long)p.rest * p.steps;

@@ -22,9 +22,15 @@
 // Sums over tokens: a CTA keeps its columns' sums in registers over its run and stores them once; a second kernel
 // adds the runs' sums in a fixed order (no atomics: the same bits on every run).
 // Measured, bf16, L2 cold: RMS sandwich with a gate a sequence, 16384 x 4096: forward 124 us (5.4 TB/s), backward 164 us
-// (4.1 TB/s) and 15 us for the sums; "add and norm" 4096 x 1024: 11.7, 10.8 and 5.5 us.  The backward pass is short of
+// (4.1 TB/s) and 15 us for the sums (forward with a residual factor that fp32 does not hold 2 us more); "add and norm" 4096 x
+// 1024: 11.8, 10.8 and 5.6 us.  The backward pass is short of
 // registers: 128 a thread allow two CTAs, whose 16 warps an SM leave a third of the issue slots empty.  A variant without
-// the ragged forms of loads and stores, and one that fetched the next row into shared memory, took 14 % longer.
+// the ragged forms of loads and stores, and one that fetched the next row into shared memory, took 14 % longer.  Rows off 16-byte
+// boundaries are accessed by single elements: bf16 16384 x 4095 against x 4096, RMS norm alone, with the launch, forward 825
+// and 85 us, backward 454 and 79.
+// A run never crosses from one sequence to the next where each has a gate, so a number of sequences just above the number of
+// places for runs (two CTAs an SM at 4096 columns) leaves most of a second wave empty, and the workspace of the sums, 16 bytes a
+// column for each run, is at least that for each sequence.
 #include <algorithm>
 
 #include "act8.cuh"

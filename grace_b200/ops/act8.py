@@ -2,8 +2,8 @@
 
 The exchange kernels shrink what ranks send to each other; these shrink what a rank keeps to itself between forward
 and backward, which is what bounds its batch.  A checkpoint holds groups of 32 neighbours of the last axis as int8
-codes with one power-of-two scale (the MXINT8 format of the OCP Microscaling specification, see ``csrc/act8.cuh``): 33
-bytes for 32 values.  The forward pass computes with the full-precision tensors; only the backward pass sees the
+codes with one power-of-two scale (MXINT8 of the OCP Microscaling specification but for the scale byte, which is 6 less, see
+``csrc/act8.cuh``): 33 bytes for 32 values.  The forward pass computes with the full-precision tensors; only the backward pass sees the
 rounded ones, so outputs are untouched and gradients carry an error of at most half a code step (2^-7 of the leading
 power of two of a value's group) in the values they are made of.
 
@@ -42,7 +42,8 @@ def pitch_of(cols: int) -> Tuple[int, int]:
 
 class Act8:
     """A checkpoint of a tensor of ``shape`` and ``dtype``: ``codes`` int8 ``[rows, pitch]`` and ``scales`` uint8
-    ``[rows, spitch]`` (``pitch_of``), rows being the product of all axes but the last."""
+    ``[rows, spitch]`` (``pitch_of``), rows being the product of all axes but the last.  A scale byte is 1 to 246 or, for a group that reads
+    as NaN, 255; bytes past a row's groups are not specified."""
 
     __slots__ = ("shape", "dtype", "rows", "pitch", "spitch", "_data", "_at", "_codes", "_scales")
 
