@@ -8,8 +8,9 @@
 //   backward  dx = dy f'(x~);  gated: da = dy b~ f'(a~), db = dy f(a~)    2 es + 1 1/32;  3 es + 2 1/16
 //
 // All four are bound by memory where rows start on 16-byte boundaries (others: below), the GELU forward pass with both
-// checkpoints by its issue slots: a thread takes a chunk of sixteen neighbouring elements (32 bytes of a 16-bit type in, 16 bytes of codes out; with eight, half of both, pack took a
-// fifth longer), two lanes share a group of 32 and agree on its largest magnitude by one shuffle.  What hides the latency is
+// checkpoints by its issue slots: a thread takes a chunk of sixteen neighbouring elements (32 bytes of a 16-bit type in, 16
+// bytes of codes out; with eight, half of both, pack took a fifth longer), two lanes share a group of 32 and agree on its
+// largest magnitude by one shuffle.  What hides the latency is
 // the number of threads: with two chunks each, all loads first, the gated backward pass took 89 us for 77, the others as
 // long as with one.  At 6.5 TB/s an SM has about 16 issue slots an element of a bf16 pack and 25 of a forward pass, so
 // arithmetic is on pairs of numbers, the encoder clamps only where a group needs it (together 34.6 -> 29.2 us for
